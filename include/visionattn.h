@@ -472,6 +472,67 @@ VA_API int va_gemm_f16(const void *a, int a_mn, long long lda, long long a_batch
                        void *c, int c_type, long long ldc, long long c_batch, int M, int N, int K,
                        int Z, float alpha, va_stream_t stream);
 
+/* ── Packed token sequences: the layers around attention ──────────────────── */
+/* Rotary positions.  Each pair (a, b) of a head's first rot_dim dimensions
+ * (x[2i], x[2i+1] with `interleaved`, else x[i], x[i + rot_dim/2]) becomes
+ * factor·(a·cos θ − b·sin θ, a·sin θ + b·cos θ) with θ = position · inv_freq[i]
+ * (reduced in 64 bits); with `backward` θ is negated, the gradient's map.  The
+ * other dimensions are copied.  q [tokens, num_heads, head_dim] and
+ * k [tokens, num_kv_heads, head_dim] (num_kv_heads 0: no k) turn in one launch.
+ * strides (host, elements): q row, q head, k row, k head, q_out row, q_out
+ * head, k_out row, k_out head; a head's dimensions are contiguous.  An output
+ * may be its input with the same strides.  positions: int32 or int64
+ * (position_bytes 4 or 8) [tokens]; inv_freq: f64 [rot_dim/2], both on the
+ * device.  rot_dim even, ≤ head_dim and ≤ 512.  f16 tensors are raw words. */
+VA_API int va_rotary_bf16(const va_bf16 *q, const va_bf16 *k, va_bf16 *q_out, va_bf16 *k_out,
+                          const int64_t *strides, const void *positions, int position_bytes,
+                          const double *inv_freq, int tokens, int num_heads, int num_kv_heads, int head_dim,
+                          int rot_dim, int interleaved, int backward, float factor, va_stream_t stream);
+VA_API int va_rotary_f16(const void *q, const void *k, void *q_out, void *k_out, const int64_t *strides,
+                         const void *positions, int position_bytes, const double *inv_freq, int tokens,
+                         int num_heads, int num_kv_heads, int head_dim, int rot_dim, int interleaved,
+                         int backward, float factor, va_stream_t stream);
+VA_API int va_rotary_f32(const float *q, const float *k, float *q_out, float *k_out, const int64_t *strides,
+                         const void *positions, int position_bytes, const double *inv_freq, int tokens,
+                         int num_heads, int num_kv_heads, int head_dim, int rot_dim, int interleaved,
+                         int backward, float factor, va_stream_t stream);
+
+/* Root-mean-square norm with the residual's addition over rows of `cols`:
+ * h = x + residual (residual NULL: h = x), r = 1/√(mean(h²) + eps), y = h·r·w,
+ * computed from the f32 sum.  h (optional, may be x or residual itself) stores the
+ * sum for the next layer.  w [cols] has x's type, or f32 with w_is_f32.
+ * _f8: q = y / scale in e4m3 with scale = max|y| / 448 over each `group`
+ * columns (0: the row; else a divisor of cols), f32 [rows, cols/group]; max|y|
+ * counts as at least 2^-100.
+ * bwd: dh = r·(g − h·r²·mean(g·h)) + grad_h with g = dy·w (grad_h optional,
+ * the gradient that reaches h along the residual), dw f32 [cols] = Σ dy·h·r,
+ * summed in an order that depends on the sizes alone.  All rows contiguous. */
+VA_API int va_rms_norm_fwd_bf16(const va_bf16 *x, const va_bf16 *residual, const void *w, int w_is_f32,
+                                va_bf16 *h, va_bf16 *y, long long rows, int cols, float eps, va_stream_t stream);
+VA_API int va_rms_norm_fwd_f16(const void *x, const void *residual, const void *w, int w_is_f32, void *h,
+                               void *y, long long rows, int cols, float eps, va_stream_t stream);
+VA_API int va_rms_norm_fwd_f32(const float *x, const float *residual, const void *w, int w_is_f32, float *h,
+                               float *y, long long rows, int cols, float eps, va_stream_t stream);
+VA_API int va_rms_norm_fwd_f8_bf16(const va_bf16 *x, const va_bf16 *residual, const void *w, int w_is_f32,
+                                   va_bf16 *h, uint8_t *q, float *scale, long long rows, int cols, int group,
+                                   float eps, va_stream_t stream);
+VA_API int va_rms_norm_fwd_f8_f16(const void *x, const void *residual, const void *w, int w_is_f32, void *h,
+                                  uint8_t *q, float *scale, long long rows, int cols, int group, float eps,
+                                  va_stream_t stream);
+VA_API int va_rms_norm_fwd_f8_f32(const float *x, const float *residual, const void *w, int w_is_f32, float *h,
+                                  uint8_t *q, float *scale, long long rows, int cols, int group, float eps,
+                                  va_stream_t stream);
+VA_API size_t va_rms_norm_bwd_workspace_bytes(long long rows, int cols);
+VA_API int va_rms_norm_bwd_bf16(const va_bf16 *dy, const va_bf16 *h, const void *w, int w_is_f32,
+                                const va_bf16 *grad_h, va_bf16 *dh, float *dw, long long rows, int cols,
+                                float eps, void *workspace, size_t ws_bytes, va_stream_t stream);
+VA_API int va_rms_norm_bwd_f16(const void *dy, const void *h, const void *w, int w_is_f32, const void *grad_h,
+                               void *dh, float *dw, long long rows, int cols, float eps, void *workspace,
+                               size_t ws_bytes, va_stream_t stream);
+VA_API int va_rms_norm_bwd_f32(const float *dy, const float *h, const void *w, int w_is_f32, const float *grad_h,
+                               float *dh, float *dw, long long rows, int cols, float eps, void *workspace,
+                               size_t ws_bytes, va_stream_t stream);
+
 /* Device status word of the tensor-core kernels: 0, or 1000+site of the
  * first bounded wait that gave up.  read: copies it to *status (synchronises
  * `stream`); clear: resets it to 0. */

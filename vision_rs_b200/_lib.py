@@ -91,6 +91,11 @@ SIGNATURES: dict[str, tuple] = {
     "va_dp_comm_disconnect": (I, [P]),
     "va_dp_comm_destroy": (I, [P]),
     "va_psa_dp_allreduce_sgd": (I, [P, P, P, F, P, P, P, P, P, P, S]),
+    **{f"va_rotary_{t}": (I, [P, P, P, P, I64P, P, I, P, I, I, I, I, I, I, I, F, S]) for t in ("bf16", "f16", "f32")},
+    **{f"va_rms_norm_fwd_{t}": (I, [P, P, P, I, P, P, LL, I, F, S]) for t in ("bf16", "f16", "f32")},
+    **{f"va_rms_norm_fwd_f8_{t}": (I, [P, P, P, I, P, P, P, LL, I, I, F, S]) for t in ("bf16", "f16", "f32")},
+    "va_rms_norm_bwd_workspace_bytes": (SZ, [LL, I]),
+    **{f"va_rms_norm_bwd_{t}": (I, [P, P, P, I, P, P, P, LL, I, F, P, SZ, S]) for t in ("bf16", "f16", "f32")},
     "va_device_status_read": (I, [C.POINTER(C.c_int), S]),
     "va_device_status_clear": (I, [S]),
 }
