@@ -533,6 +533,40 @@ VA_API int va_rms_norm_bwd_f32(const float *dy, const float *h, const void *w, i
                                float *dh, float *dw, long long rows, int cols, float eps, void *workspace,
                                size_t ws_bytes, va_stream_t stream);
 
+/* Attention over packed sequences: O_i = Σ_j softmax_j(softmax_scale·q_i·k_j) v_j
+ * over the keys of query i's own sequence, query head h reading key head
+ * h / (num_heads/num_kv_heads); causal: query i of lq sees key j of lk when
+ * j ≤ i + lk − lq (the last query sees every key).  A query that sees no key gets
+ * O = 0 and lse = −∞.  q [total_q, num_heads, head_dim], k and v
+ * [total_k, num_kv_heads, head_dim], 16-bit types, rows and heads strided
+ * (strides, host, elements: q row, q head, k row, k head, v row, v head;
+ * 16-byte multiples, base 16-byte aligned, a head's dimensions contiguous),
+ * head_dim a multiple of 8 up to 128; out [total_q, num_heads, head_dim]
+ * contiguous; lse f32 [num_heads, total_q] (natural log).
+ * The sequences are given to va_packed_plan_build: cu_q and cu_k, int32
+ * [num_seqs + 1] on the device, the rows where each sequence's queries and
+ * keys begin (cu[0] = 0, cu[num_seqs] = total).  It fills the plan (256-byte
+ * aligned, va_packed_plan_bytes) on the stream, without a copy to the host;
+ * later calls with the same sizes read it, layer after layer, and keep their
+ * partial results in it: calls that share a plan must not overlap.
+ * va_packed_plan_status reads whether offsets were out of order or range (they
+ * are clamped; synchronises). */
+VA_API size_t va_packed_plan_bytes(int num_seqs, int total_q, int total_k, int num_heads, int num_kv_heads,
+                                   int head_dim, int causal, int training);
+VA_API int va_packed_plan_build(const int32_t *cu_q, const int32_t *cu_k, int num_seqs, int total_q, int total_k,
+                                int num_heads, int num_kv_heads, int head_dim, int causal, int training,
+                                void *plan, size_t plan_bytes, va_stream_t stream);
+VA_API int va_packed_plan_status(const void *plan, int training, int *bad_offsets, va_stream_t stream);
+VA_API int va_packed_attention_fwd_bf16(const va_bf16 *q, const va_bf16 *k, const va_bf16 *v, va_bf16 *out,
+                                        float *lse, const int64_t *strides, int num_seqs, int total_q,
+                                        int total_k, int num_heads, int num_kv_heads, int head_dim, int causal,
+                                        int training, float softmax_scale, void *plan, size_t plan_bytes,
+                                        va_stream_t stream);
+VA_API int va_packed_attention_fwd_f16(const void *q, const void *k, const void *v, void *out, float *lse,
+                                       const int64_t *strides, int num_seqs, int total_q, int total_k,
+                                       int num_heads, int num_kv_heads, int head_dim, int causal, int training,
+                                       float softmax_scale, void *plan, size_t plan_bytes, va_stream_t stream);
+
 /* Device status word of the tensor-core kernels: 0, or 1000+site of the
  * first bounded wait that gave up.  read: copies it to *status (synchronises
  * `stream`); clear: resets it to 0. */

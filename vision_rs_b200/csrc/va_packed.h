@@ -1,0 +1,98 @@
+// Work lists of the packed-sequence attention: what the plan kernel writes and
+// the forward and backward kernels read (va_packed_plan.cu, va_packed_attn.cu,
+// va_packed_attn_bwd.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace va {
+
+constexpr int kPackBlock = 128;   // keys (and rows of a tile) a step
+constexpr int kMaxSeqs = 1 << 20;
+constexpr int kPlanSeqs = 2048;   // sequences whose tile counts fit the plan kernel's shared memory
+
+// One unit of forward or dQ work: up to `tokens` queries of one sequence
+// against its key blocks [kb0, kb1).  Query t of the unit sees keys
+// j ≤ see + t (not causal: all `lk` of them).
+struct alignas(16) QItem {
+  int q0, tokens;   // first query (row of the packed tensor) and their number
+  int k0, lk;       // the sequence's first key (row of the packed tensor) and its length
+  int see;          // causal: last key that query 0 sees
+  int kb0, kb1;     // key blocks
+  int slot;         // partial result's slot, -1: the unit is the whole tile and writes the output
+  int slot0, parts; // the tile's first slot and number of parts
+  int counter;      // the tile's arrival counter
+  int pad;
+};
+// One unit of dK/dV work: up to 128 keys of one sequence against its query blocks [qb0, qb1).
+struct alignas(16) KItem {
+  int k0, keys;     // first key (row of the packed tensor) and their number
+  int j0;           // its index in the sequence
+  int q0, lq, lk;   // the sequence's first query (row) and lengths
+  int qb0, qb1;
+};
+
+// Sizes that host and device agree on, from the call's sizes alone.
+struct PackedShape {
+  int num_seqs, total_q, total_k, heads, kv_heads, dim, causal, training;
+  int group;        // query heads a key head
+  // Forward: rows of a 128-row tile are the queries of one head, two tiles a
+  // unit (few = 0), or (query, head of the group) pairs, one tile a unit
+  // with its keys split over units (few = 1).
+  int few;
+  int q_tile;       // queries a forward unit
+  int units;        // heads (or key heads) that each forward unit is run for
+  int max_tiles, max_items, max_slots, split_budget;
+  int max_dq_items, max_dkv_items;
+  // byte offsets in the plan
+  size_t items, dq_items, dkv_items, counters, scratch, part_o, part_lse, total;
+};
+
+// Header words of the plan, one of each for the three lists: the number of
+// units, and whether the sequences' offsets had to be clamped.
+enum { kHdrItems = 0, kHdrDq = 1, kHdrDkv = 2, kHdrBad = 4 };
+
+inline size_t pk_align(size_t x) { return (x + 255) & ~(size_t)255; }
+
+inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim, int causal,
+                                int training) {
+  PackedShape s{};
+  s.num_seqs = num_seqs, s.total_q = total_q, s.total_k = total_k;
+  s.heads = heads, s.kv_heads = kv_heads, s.dim = dim, s.causal = causal, s.training = training;
+  s.group = heads / kv_heads;
+  // One tile of (query, head) rows a unit when the sequences' queries are few on
+  // average, or when units of 256 queries would leave SMs idle.
+  const long long big = ((long long)total_q / 256 + num_seqs) * heads;
+  s.few = (long long)total_q * s.group <= 128LL * num_seqs || big < 148 ? 1 : 0;
+  s.q_tile = s.few ? kPackBlock / s.group : 2 * kPackBlock;
+  s.units = s.few ? kv_heads : heads;
+  s.max_tiles = (int)std::min<long long>((total_q + s.q_tile - 1) / s.q_tile + (long long)num_seqs, total_q);
+  s.split_budget = s.few ? (592 + s.units - 1) / s.units : 0;
+  s.max_items = s.max_tiles + s.split_budget;
+  s.max_slots = 2 * s.split_budget;
+  s.max_dq_items = training ? (int)std::min<long long>((total_q + 127) / 128 + (long long)num_seqs, total_q) : 0;
+  s.max_dkv_items = training ? (int)std::min<long long>((total_k + 127) / 128 + (long long)num_seqs, total_k) : 0;
+  size_t o = 256;
+  s.items = o, o += pk_align((size_t)s.max_items * sizeof(QItem));
+  s.dq_items = o, o += pk_align((size_t)s.max_dq_items * sizeof(QItem));
+  s.dkv_items = o, o += pk_align((size_t)s.max_dkv_items * sizeof(KItem));
+  s.counters = o, o += pk_align(s.few ? (size_t)s.max_tiles * s.units * 4 : 0);
+  s.scratch = o, o += pk_align(num_seqs > kPlanSeqs ? (size_t)3 * (num_seqs + 1) * 4 : 0);
+  s.part_o = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * dim * 4);
+  s.part_lse = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * 4);
+  s.total = o;
+  return s;
+}
+
+int packed_status_read(int* out, cudaStream_t st);
+int packed_status_clear(cudaStream_t st);
+int packed_bwd_status_read(int* out, cudaStream_t st);
+int packed_bwd_status_clear(cudaStream_t st);
+// Argument checks shared by the entry points (VA_OK or an error that is set).
+int packed_check(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim);
+
+}  // namespace va

@@ -1,0 +1,540 @@
+// Attention over packed sequences of different lengths (tcgen05 + TMEM + TMA):
+//
+//   O_i = Σ_j P_ij v_j,  P_ij = exp(scale·q_i·k_j − lse_i),
+//   lse_i = log Σ_j exp(scale·q_i·k_j)
+//
+// over the keys j of query i's own sequence (causal: j ≤ i + lk − lq), query
+// head h reading key head h / group.  One pass over the keys with a running
+// maximum and sum (f32); a row that sees no key gets O = 0 and lse = −∞.
+//
+// A CTA takes one unit of the plan (va_packed_plan.cu) for one head:
+//   TILES = 2: 256 queries of one head as two 128-row tiles that share the
+//     K/V stream (whole prompts, training);
+//   TILES = 1: one tile whose rows are (query, head of the group) pairs, so
+//     the query heads of a key head read its keys once, over a part of the
+//     keys; two CTAs an SM.  The last CTA of a tile's parts to arrive joins
+//     them in the parts' order (single tokens, few queries).
+// Warps: 4 a tile for the softmax (a thread owns a row), 1 TMA producer, 1
+// MMA issuer.  Per 128-key step: S = Q·Kᵀ into TMEM, the row's p = 2^(s −
+// reference) back into the same columns as 16-bit P, O += P·V with P as the
+// TMEM operand.  The reference only follows the row maximum when it grows by
+// more than 2^8, so O is rarely rescaled.  P is held in the inputs' 16-bit
+// type: its rounding adds about as much error as that of the output; sums,
+// maxima and O stay f32.
+//
+// Rows of other sequences that a tile's boxes bring in: scores of keys past
+// the end are replaced, not added to; V rows past the last key that the unit sees are zeroed in
+// shared memory (0 · NaN would be NaN), and the MMAs stop at the last 16-key
+// group in use.
+#include <cudaTypedefs.h>
+
+#include <type_traits>
+
+#include "va_common.cuh"
+#include "va_packed.h"
+#include "va_sm100.cuh"
+
+namespace va {
+using namespace sm100;
+
+__device__ int g_packed_status;
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kRescaleAt = 8.0f;  // the reference follows the maximum once it is 2^8 ahead
+
+// DP: head size in shared memory and TMEM (64 or 128; the TMA boxes fill what is past `dim` with zeros).
+template <int DP, int TILES> struct FwdCfg {
+  static constexpr int kSlotBytes = kPackBlock * DP * 2;
+  static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 5);
+  static constexpr int kThreads = TILES * 128 + 64;
+  static constexpr int kCtas = TILES == 2 ? 1 : 2;  // an SM
+  static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
+  static constexpr uint32_t kColS = 0, kColO = TILES * 128;  // S_m at 128·m, O_m at kColO + DP·m
+};
+
+template <int DP, int TILES> struct FwdSmem {
+  using C = FwdCfg<DP, TILES>;
+  uint8_t q[TILES][C::kSlotBytes];      // per 64 dims: 128 rows × 128 bytes, SW128
+  uint8_t kv[C::kSlots][C::kSlotBytes];
+  uint64_t q_full, kv_full[C::kSlots], kv_empty[C::kSlots];
+  uint64_t s_full[TILES], p_full[TILES], o_done[TILES], fin;
+  uint32_t tmem_base;
+  int abort;
+  int last;
+};
+
+struct FwdArgs {
+  const uint8_t* plan;
+  PackedShape s;
+  void* out;
+  float* lse;
+  float scale;  // softmax scale · log2 e
+};
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) return pack_bf16x2(a, b);
+  else return pack_f16x2(a, b);
+}
+
+template <int DP, int TILES, bool BF16>
+__global__ void __launch_bounds__(FwdCfg<DP, TILES>::kThreads, FwdCfg<DP, TILES>::kCtas)
+packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, FwdArgs a) {
+  using C = FwdCfg<DP, TILES>;
+  extern __shared__ uint8_t smem_raw[];
+  FwdSmem<DP, TILES>& sm = *reinterpret_cast<FwdSmem<DP, TILES>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const PackedShape& ps = a.s;
+  const int unit = blockIdx.x / ps.units, head = blockIdx.x - unit * ps.units;
+  if (unit >= reinterpret_cast<const int*>(a.plan)[kHdrItems]) return;
+  const QItem it = reinterpret_cast<const QItem*>(a.plan + ps.items)[unit];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = ps.few ? ps.group : 1;        // rows of a query in a tile
+  const int kv_head = ps.few ? head : head / ps.group;
+  const int rows = it.tokens * group;
+  // key blocks of each tile: a causal first tile ends before the second
+  int kb_end[TILES], see_end = 0;  // see_end: one past the last key that any row of the unit sees
+#pragma unroll
+  for (int m = 0; m < TILES; ++m) {
+    const int n = TILES == 2 ? min(kPackBlock, it.tokens - m * kPackBlock) : it.tokens;
+    int end = 0;
+    if (n > 0) end = ps.causal ? min(it.lk, max(0, it.see + m * kPackBlock + n)) : it.lk;
+    kb_end[m] = max(it.kb0, min(it.kb1, (end + kPackBlock - 1) / kPackBlock));
+    see_end = max(see_end, end);
+  }
+  const int kb_all = TILES == 2 ? max(kb_end[0], kb_end[TILES - 1]) : kb_end[0];
+  const int nkb = kb_all - it.kb0;
+  const int dim16 = (ps.dim + 15) & ~15;
+
+  if (tid == 0) {
+    mbar_init(&sm.q_full, 1);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&sm.kv_full[i], 1);
+      mbar_init(&sm.kv_empty[i], 1);
+    }
+    for (int m = 0; m < TILES; ++m) {
+      mbar_init(&sm.s_full[m], 1);
+      mbar_init(&sm.p_full[m], 128);
+      mbar_init(&sm.o_done[m], 1);
+    }
+    mbar_init(&sm.fin, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == TILES * 4) {
+    tmem_alloc(&sm.tmem_base, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == TILES * 4) {
+    // ── TMA producer: Q, then K and V blocks alternately through the slot ring ──
+    if (lane == 0 && nkb > 0) {
+      constexpr int NB = DP / 64;
+      const uint32_t q_bytes = (uint32_t)(ps.few ? (kPackBlock / group) * group : kPackBlock) * 128 * NB;
+      mbar_arrive_expect_tx(&sm.q_full, q_bytes * TILES);
+      for (int m = 0; m < TILES; ++m)
+        for (int b = 0; b < NB; ++b)
+          tma_load_3d(sm.q[m] + b * kPackBlock * 128, &map_q, &sm.q_full, b * 64, ps.few ? head * group : head,
+                      it.q0 + m * kPackBlock);
+      bool ok = true;
+      int issued = 0;
+      for (int g = 0; g < 2 * nkb; ++g) {
+        const int st = g % C::kSlots, row = it.k0 + (it.kb0 + (g >> 1)) * kPackBlock;
+        if (g >= C::kSlots &&
+            !(ok = mbar_wait(&sm.kv_empty[st], (g / C::kSlots - 1) & 1, &sm.abort, &g_packed_status, 1)))
+          break;
+        mbar_arrive_expect_tx(&sm.kv_full[st], C::kSlotBytes);
+        for (int b = 0; b < NB; ++b)
+          tma_load_3d(sm.kv[st] + b * kPackBlock * 128, (g & 1) ? &map_v : &map_k, &sm.kv_full[st], b * 64, kv_head,
+                      row);
+        ++issued;
+      }
+      if (!ok) {  // loads issued here land (bounded) before the CTA can exit
+        for (int g = max(0, issued - C::kSlots); g < issued; ++g) {
+          const long long c0 = clock64();
+          while (!mbar_try_wait(&sm.kv_full[g % C::kSlots], (g / C::kSlots) & 1) && clock64() - c0 < kSpinCycles) {
+          }
+        }
+        const long long c0 = clock64();
+        while (!mbar_try_wait(&sm.q_full, 0) && clock64() - c0 < kSpinCycles) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == TILES * 4 + 1) {
+    // ── MMA issuer (converged warp, one elected lane issues) ──
+    if (nkb > 0) {
+      const uint32_t fmt = BF16 ? AB_BF16 : AB_F16;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &sm.abort, &g_packed_status, where));
+      };
+      const uint32_t idesc_o = idesc_f32acc(kPackBlock, dim16, fmt, false, true);
+      // keys of block kb that some row of the unit sees, as the MMAs' extent
+      auto keys16 = [&](int kb) { return (min(kPackBlock, see_end - kb * kPackBlock) + 15) & ~15; };
+      auto issue_s = [&](int m, int st, int kb) {
+        const uint32_t idesc = idesc_f32acc(kPackBlock, keys16(kb), fmt, false, false);
+        const uint64_t dq = sdesc(smem_u32(sm.q[m]), 16, 1024, SW_128B), dk = sdesc(smem_u32(sm.kv[st]), 16, 1024, SW_128B);
+        for (int s = 0; s < dim16 / 16; ++s) {
+          const uint64_t off = (uint64_t)((s >> 2) * ((kPackBlock * 128) >> 4) + (s & 3) * 2);
+          mma_ss_w(tmem + C::kColS + m * 128, dq + off, dk + off, idesc, s > 0 ? 1u : 0u);
+        }
+        mma_commit_w(&sm.s_full[m]);
+      };
+      bool ok = wait(&sm.q_full, 0, 2) && wait(&sm.kv_full[0], 0, 3);
+      tc_fence_after();
+      if (ok) {
+        for (int m = 0; m < TILES; ++m)
+          if (it.kb0 < kb_end[m]) issue_s(m, 0, it.kb0);
+        mma_commit_w(&sm.kv_empty[0]);
+      }
+      for (int j = 0; ok && j < nkb; ++j) {
+        const int kb = it.kb0 + j, gv = 2 * j + 1, gk = 2 * j + 2;
+        const int sv = gv % C::kSlots, sk = gk % C::kSlots;
+        if (!(ok = wait(&sm.kv_full[sv], (gv / C::kSlots) & 1, 4))) break;
+        const int used = min(kPackBlock, see_end - kb * kPackBlock), steps = (used + 15) >> 4;
+        if (used & 15) {  // V rows past the last key in its 16-key group: zeros
+          for (int i = lane; i < ((used + 15) / 16 * 16 - used) * (DP / 8); i += 32) {
+            const int r = used + i / (DP / 8), c = i % (DP / 8);
+            *reinterpret_cast<uint4*>(sm.kv[sv] + (c >> 3) * kPackBlock * 128 + sw128_off(r, c & 7)) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const uint64_t dv = sdesc(smem_u32(sm.kv[sv]), kPackBlock * 128, 1024, SW_128B);
+        bool have_k = false;
+        for (int m = 0; m < TILES; ++m) {
+          if (kb >= kb_end[m]) continue;
+          if (!(ok = wait(&sm.p_full[m], j & 1, 5))) break;
+          tc_fence_after();
+          for (int s = 0; s < steps; ++s)
+            mma_ts_w(tmem + C::kColO + m * DP, tmem + C::kColS + m * 128 + s * 8, dv + (uint64_t)(s * (2048 >> 4)),
+                     idesc_o, (j > 0 || s > 0) ? 1u : 0u);
+          mma_commit_w(&sm.o_done[m]);
+          if (kb + 1 < kb_end[m]) {
+            if (!have_k && !(ok = wait(&sm.kv_full[sk], (gk / C::kSlots) & 1, 6))) break;
+            have_k = true;
+            // the next scores overwrite P's columns: P·V has to be done with them
+            if (!(ok = wait(&sm.o_done[m], j & 1, 7))) break;
+            tc_fence_after();
+            issue_s(m, sk, kb + 1);
+          }
+        }
+        if (!ok) break;
+        mma_commit_w(&sm.kv_empty[sv]);
+        if (have_k) mma_commit_w(&sm.kv_empty[sk]);
+      }
+      mma_commit_w(&sm.fin);  // every MMA issued here completes before the CTA tears down
+      const long long c0 = clock64();
+      while (!mbar_try_wait(&sm.fin, 0) && clock64() - c0 < kSpinCycles) {
+      }
+    }
+    __syncwarp();
+  } else {
+    // ── softmax: thread = row of tile m ──
+    const int m = TILES == 2 ? warp >> 2 : 0, row = tid - m * 128;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + C::kColS + m * 128, to = tmem + lanes + C::kColO + m * DP;
+    const int my_row = m * kPackBlock + row;
+    const bool mine = my_row < rows;
+    // one past the last key this row sees
+    const int see = !mine ? 0 : ps.causal ? min(it.lk, it.see + my_row / group + 1) : it.lk;
+    const float scale = a.scale;
+    float ref = -INFINITY, sum = 0.0f;  // reference in log2 units
+    bool ok = true;
+    // warps without a row of the unit only keep the barriers going
+    const bool idle = (m * kPackBlock + (warp & 3) * 32) >= rows;
+    const int n = kb_end[m] - it.kb0;
+    for (int j = 0; j < n; ++j) {
+      if (!(ok = mbar_wait(&sm.s_full[m], j & 1, &sm.abort, &g_packed_status, 8))) break;
+      if (!idle) {
+        tc_fence_after();
+        const int limit = see - (it.kb0 + j) * kPackBlock;  // columns ≥ limit are hidden
+        uint32_t u[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, u[c]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) reg_fence(u[c]);
+        if (__any_sync(0xffffffffu, limit < kPackBlock)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= limit) u[c][i] = 0xff800000u;  // −∞
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(u[c][i]), __uint_as_float(u[c][i + 1]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        const bool grow = mine && (top > ref + kRescaleAt || ref == -INFINITY);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float next = fmaxf(ref, top);
+          if (j > 0) {
+            const float f = next == -INFINITY ? 1.0f : ex2(ref - next);
+            if (!(ok = mbar_wait(&sm.o_done[m], (j - 1) & 1, &sm.abort, &g_packed_status, 9))) break;
+            tc_fence_after();
+            for (int c = 0; c < dim16; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(to + c, o);
+              tmem_ld_wait();
+              reg_fence(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(to + c, o);
+            }
+            sum *= f;
+          }
+          ref = next;
+        }
+        const float base = ref == -INFINITY ? 0.0f : ref;
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float p0 = ex2(fmaf(__uint_as_float(u[c][i]), scale, -base));
+            const float p1 = ex2(fmaf(__uint_as_float(u[c][i + 1]), scale, -base));
+            part[(i >> 1) & 3] += p0 + p1;
+            p[i >> 1] = pack2<BF16>(p0, p1);
+          }
+          tmem_st16(ts + c * 16, p);
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tmem_st_wait();
+        tc_fence_before();
+      }
+      mbar_arrive(&sm.p_full[m]);
+    }
+    // ── output ──
+    if (ok && n > 0) ok = mbar_wait(&sm.o_done[m], (n - 1) & 1, &sm.abort, &g_packed_status, 10);
+    if (ok && !idle) {
+      tc_fence_after();
+      const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+      const float lse = n > 0 && ref != -INFINITY ? (ref + log2f(sum)) * kLn2 : -INFINITY;
+      const int t = my_row / group, h = ps.few ? head * group + my_row - t * group : head;
+      if (it.slot < 0) {
+        const long long at = (long long)(it.q0 + t) * ps.heads + h;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + at * ps.dim;
+        for (int c = 0; c < dim16; c += 16) {
+          uint32_t o[16];
+          if (n > 0) {
+            tmem_ld16(to + c, o);
+            tmem_ld_wait();
+            reg_fence(o);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = n > 0 ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack2<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+          if (mine) {
+            *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (c + 8 < ps.dim) *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+          __syncwarp();
+        }
+        if (mine) a.lse[(long long)h * ps.total_q + it.q0 + t] = lse;
+      } else {
+        const long long at = ((long long)it.slot * ps.units + head) * kPackBlock + row;
+        float* out = reinterpret_cast<float*>(const_cast<uint8_t*>(a.plan) + ps.part_o) + at * ps.dim;
+        for (int c = 0; c < dim16; c += 16) {
+          uint32_t o[16];
+          if (n > 0) {
+            tmem_ld16(to + c, o);
+            tmem_ld_wait();
+            reg_fence(o);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            if (!mine || c + i >= ps.dim) continue;
+            float4 f;
+            f.x = n > 0 ? __uint_as_float(o[i]) * inv : 0.0f;
+            f.y = n > 0 ? __uint_as_float(o[i + 1]) * inv : 0.0f;
+            f.z = n > 0 ? __uint_as_float(o[i + 2]) * inv : 0.0f;
+            f.w = n > 0 ? __uint_as_float(o[i + 3]) * inv : 0.0f;
+            *reinterpret_cast<float4*>(out + c + i) = f;
+          }
+          __syncwarp();
+        }
+        if (mine) reinterpret_cast<float*>(const_cast<uint8_t*>(a.plan) + ps.part_lse)[at] = lse;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == TILES * 4) tmem_dealloc(tmem, C::kTmemCols);
+
+  if constexpr (TILES == 1) {
+    if (it.slot < 0 || sm.abort) return;
+    // ── the last of a tile's parts joins them: O = Σ w_k O_k, w_k = exp(lse_k − lse) ──
+    if (tid == 0) {
+      __threadfence();
+      int* cnt = reinterpret_cast<int*>(const_cast<uint8_t*>(a.plan) + ps.counters) + (long long)it.counter * ps.units + head;
+      sm.last = atomicAdd(cnt, 1) == it.parts - 1;
+      if (sm.last) *cnt = 0;  // for the next call with this plan
+      __threadfence();
+    }
+    __syncthreads();
+    if (!sm.last) return;
+    const float* plse = reinterpret_cast<const float*>(a.plan + ps.part_lse);
+    const float* po = reinterpret_cast<const float*>(a.plan + ps.part_o);
+    const long long base = ((long long)it.slot0 * ps.units + head) * kPackBlock, step = (long long)ps.units * kPackBlock;
+    for (int r = warp; r < rows; r += C::kThreads / 32) {
+      float top = -INFINITY;
+      for (int k = lane; k < it.parts; k += 32) top = fmaxf(top, __ldcg(plse + base + k * step + r));
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float total = 0.0f;
+      for (int k = lane; k < it.parts; k += 32) total += exp2f((__ldcg(plse + base + k * step + r) - ref) * kLog2e);
+      for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+      const int t = r / group, h = head * group + r - t * group;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + ((long long)(it.q0 + t) * ps.heads + h) * ps.dim;
+      for (int c = lane * 4; c < ps.dim; c += 128) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < it.parts; ++k) {
+          const float w = exp2f((__ldcg(plse + base + k * step + r) - ref) * kLog2e) * inv;
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(po + (base + k * step + r) * ps.dim + c));
+          acc.x = fmaf(w, f.x, acc.x);
+          acc.y = fmaf(w, f.y, acc.y);
+          acc.z = fmaf(w, f.z, acc.z);
+          acc.w = fmaf(w, f.w, acc.w);
+        }
+        *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
+      }
+      if (lane == 0) a.lse[(long long)h * ps.total_q + it.q0 + t] = top == -INFINITY ? -INFINITY : ref + logf(total);
+    }
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+}  // namespace
+
+// [rows, heads, dim] (strides in elements) in boxes of 64 dims × box_heads × box_rows.
+int packed_map(CUtensorMap* m, const void* base, bool bf16, int rows, int heads, int dim, long long row_stride,
+               long long head_stride, int box_heads, int box_rows, const char* what) {
+  auto fn = encode_fn();
+  if (!fn) return set_error(VA_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
+  if (heads == 1) head_stride = dim;
+  if (rows <= 1) row_stride = (long long)heads * dim;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || row_stride % 8 || head_stride % 8 || row_stride <= 0 || head_stride <= 0)
+    return set_error(VA_ERR_ALIGN, "packed attention: %s needs a 16-byte aligned base and strides of 16 bytes", what);
+  const cuuint64_t d[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t s[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+  const cuuint32_t bx[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows}, es[3] = {1, 1, 1};
+  CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(base), d, s, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(VA_ERR_ALIGN, "packed attention: tensor map for %s rejected (CUresult %d)", what, (int)r);
+  return VA_OK;
+}
+
+namespace {
+
+template <int DP, int TILES, bool BF16>
+int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdArgs& a, cudaStream_t st) {
+  using C = FwdCfg<DP, TILES>;
+  auto kernel = packed_attn_kernel<DP, TILES, BF16>;
+  constexpr int smem = (int)sizeof(FwdSmem<DP, TILES>) + 1024;
+  static PerDeviceOnce once;
+  if (int rc = once.run([&]() -> int {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return e == cudaSuccess ? VA_OK : set_error(VA_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      }))
+    return rc;
+  const long long grid = (long long)a.s.max_items * a.s.units;
+  VA_CHECK_ARG(grid < (1LL << 31), "packed attention: too many units");
+  kernel<<<(unsigned)grid, C::kThreads, smem, st>>>(mq, mk, mv, a);
+  return check_launch("packed attention");
+}
+
+template <bool BF16>
+int packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides, int num_seqs,
+               int total_q, int total_k, int heads, int kv_heads, int dim, int causal, int training, float scale,
+               void* plan, size_t plan_bytes, cudaStream_t st) {
+  if (int rc = packed_check(num_seqs, total_q, total_k, heads, kv_heads, dim)) return rc;
+  VA_CHECK_ARG(scale > 0.0f && scale < INFINITY, "packed attention: the scale must be positive and finite");
+  if (total_q == 0) return VA_OK;
+  VA_CHECK_ARG(q && out && lse && strides && (total_k == 0 || (k && v)), "packed attention: null pointer");
+  FwdArgs a{static_cast<const uint8_t*>(plan),
+            packed_shape(num_seqs, total_q, total_k, heads, kv_heads, dim, causal != 0, training != 0), out, lse,
+            scale * kLog2e};
+  if (!plan || plan_bytes < a.s.total)
+    return set_error(VA_ERR_WORKSPACE, "packed attention: plan of %zu < %zu bytes", plan_bytes, a.s.total);
+  if ((reinterpret_cast<uintptr_t>(plan) & 255) || (reinterpret_cast<uintptr_t>(out) & 15))
+    return set_error(VA_ERR_ALIGN, "packed attention: the plan needs 256-byte and the output 16-byte alignment");
+  CUtensorMap mq, mk, mv;
+  const PackedShape& s = a.s;
+  if (int rc = packed_map(&mq, q, BF16, total_q, heads, dim, strides[0], strides[1], s.few ? s.group : 1,
+                          s.few ? s.q_tile : kPackBlock, "q"))
+    return rc;
+  if (total_k > 0) {
+    if (int rc = packed_map(&mk, k, BF16, total_k, kv_heads, dim, strides[2], strides[3], 1, kPackBlock, "k")) return rc;
+    if (int rc = packed_map(&mv, v, BF16, total_k, kv_heads, dim, strides[4], strides[5], 1, kPackBlock, "v")) return rc;
+  } else {
+    mk = mv = mq;  // no unit has a key block: never read
+  }
+  if (dim <= 64) return s.few ? launch_fwd<64, 1, BF16>(mq, mk, mv, a, st) : launch_fwd<64, 2, BF16>(mq, mk, mv, a, st);
+  return s.few ? launch_fwd<128, 1, BF16>(mq, mk, mv, a, st) : launch_fwd<128, 2, BF16>(mq, mk, mv, a, st);
+}
+
+}  // namespace
+
+int packed_status_read(int* out, cudaStream_t st) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(out, g_packed_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return set_error(VA_ERR_LAUNCH, "device status read: %s", cudaGetErrorString(e));
+  return VA_OK;
+}
+
+int packed_status_clear(cudaStream_t st) {
+  static const int zero = 0;
+  cudaError_t e = cudaMemcpyToSymbolAsync(g_packed_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+  if (e != cudaSuccess) return set_error(VA_ERR_LAUNCH, "device status clear: %s", cudaGetErrorString(e));
+  return VA_OK;
+}
+
+}  // namespace va
+
+using namespace va;
+
+extern "C" {
+
+int va_packed_attention_fwd_bf16(const va_bf16* q, const va_bf16* k, const va_bf16* v, va_bf16* out, float* lse,
+                                 const int64_t* strides, int num_seqs, int total_q, int total_k, int num_heads,
+                                 int num_kv_heads, int head_dim, int causal, int training, float softmax_scale,
+                                 void* plan, size_t plan_bytes, va_stream_t stream) {
+  return packed_fwd<true>(q, k, v, out, lse, strides, num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim,
+                          causal, training, softmax_scale, plan, plan_bytes, (cudaStream_t)stream);
+}
+
+int va_packed_attention_fwd_f16(const void* q, const void* k, const void* v, void* out, float* lse,
+                                const int64_t* strides, int num_seqs, int total_q, int total_k, int num_heads,
+                                int num_kv_heads, int head_dim, int causal, int training, float softmax_scale,
+                                void* plan, size_t plan_bytes, va_stream_t stream) {
+  return packed_fwd<false>(q, k, v, out, lse, strides, num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim,
+                           causal, training, softmax_scale, plan, plan_bytes, (cudaStream_t)stream);
+}
+
+}  // extern "C"

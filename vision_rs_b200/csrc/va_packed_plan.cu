@@ -1,0 +1,275 @@
+// The plan of a packed-sequence attention: from the sequences' offsets (on the
+// device) to the lists of work units that the attention kernels walk, without
+// a copy to the host.  One launch, one block for each list:
+//
+//   list 0  forward units,  list 1  dQ units,  list 2  dK/dV units (training)
+//
+// A block counts its tiles (prefix sum over the sequences), sums their key
+// (or query) blocks, cuts the forward tiles' key ranges into parts when there
+// are few tiles (`split_budget` parts over all), and writes the units sorted
+// by their size, longest first (a counting sort over 256 size classes), so
+// that the last blocks of the attention's grid are its shortest.  Units of a
+// class may come in any order: each writes results of its own.
+//
+// Offsets that decrease or pass the packed tensors' ends are clamped (no
+// access leaves the tensors) and reported in the header.
+#include "va_common.cuh"
+#include "va_packed.h"
+
+namespace va {
+namespace {
+
+constexpr int kPlanThreads = 512, kClasses = 256;
+
+struct Seq {
+  int q0, lq, k0, lk;
+};
+
+__device__ __forceinline__ Seq load_seq(const int* cu_q, const int* cu_k, int b, int total_q, int total_k, int* bad) {
+  const int a0 = cu_q[b], a1 = cu_q[b + 1], c0 = cu_k[b], c1 = cu_k[b + 1];
+  Seq s;
+  s.q0 = min(max(a0, 0), total_q);
+  s.lq = max(min(max(a1, 0), total_q) - s.q0, 0);
+  s.k0 = min(max(c0, 0), total_k);
+  s.lk = max(min(max(c1, 0), total_k) - s.k0, 0);
+  if (s.q0 != a0 || s.lq != a1 - a0 || s.k0 != c0 || s.lk != c1 - c0 || (b == 0 && (a0 != 0 || c0 != 0))) *bad = 1;
+  return s;
+}
+
+// Exclusive sum over the block's threads; *total: of all.
+__device__ int block_scan(int v, int* total) {
+  __shared__ int warp_sum[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the previous call's readers are done
+  if (lane == 31) warp_sum[w] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int i = 0; i < kPlanThreads / 32; ++i) {
+    const int t = warp_sum[i];
+    if (i < w) before += t;
+    all += t;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+struct PlanArgs {
+  const int *cu_q, *cu_k;
+  uint8_t* plan;
+  PackedShape s;
+};
+
+// Tile t of a list: its sequence and index in it.  first[b] = tiles before sequence b (first[num_seqs] = all).
+__device__ __forceinline__ int seq_of_tile(const int* first, int num_seqs, int t) {
+  int lo = 0, hi = num_seqs;  // the last b with first[b] <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct Range {
+  int b0, b1;
+};
+// Key blocks that the queries [i0, i0 + n) of a sequence see.
+__device__ __forceinline__ Range key_blocks(const Seq& s, int i0, int n, int causal) {
+  const int end = causal ? min(s.lk, max(0, i0 + n + s.lk - s.lq)) : s.lk;
+  return {0, (end + kPackBlock - 1) / kPackBlock};
+}
+// Query blocks that see any of the keys from j0 on.
+__device__ __forceinline__ Range query_blocks(const Seq& s, int j0, int causal) {
+  const int n = (s.lq + kPackBlock - 1) / kPackBlock;
+  const int i0 = causal ? max(0, j0 - (s.lk - s.lq)) : 0;
+  return {min(n, i0 / kPackBlock), n};
+}
+
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
+  __shared__ int hist[kClasses], cursor[kClasses];
+  __shared__ int bad, most, first_smem[kPlanSeqs + 1];
+  const PackedShape& s = a.s;
+  const int list = blockIdx.x, tid = threadIdx.x;
+  int* hdr = reinterpret_cast<int*>(a.plan);
+  // tiles before each sequence
+  int* first = s.num_seqs <= kPlanSeqs
+                   ? first_smem
+                   : reinterpret_cast<int*>(a.plan + s.scratch) + (size_t)list * (s.num_seqs + 1);
+  const int tile = list == 0 ? s.q_tile : kPackBlock;
+  if (tid == 0) bad = 0, most = 0;
+  for (int c = tid; c < kClasses; c += kPlanThreads) hist[c] = 0;
+  __syncthreads();
+
+  int tiles = 0;
+  for (int b0 = 0; b0 < s.num_seqs; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < s.num_seqs) {
+      const Seq q = load_seq(a.cu_q, a.cu_k, b, s.total_q, s.total_k, &bad);
+      n = ((list == 2 ? q.lk : q.lq) + tile - 1) / tile;
+    }
+    int sum;
+    const int before = block_scan(n, &sum);
+    if (b < s.num_seqs) first[b] = tiles + before;
+    tiles += sum;
+  }
+  if (tid == 0) first[s.num_seqs] = tiles;
+  __syncthreads();
+  // offsets that run backwards could name more rows than there are: keep to the lists' room
+  const int room = list == 0 ? s.max_tiles : list == 1 ? s.max_dq_items : s.max_dkv_items;
+  if (tiles > room) {
+    if (tid == 0) bad = 1;
+    tiles = room;
+  }
+
+  Seq own_seq{};  // the thread's first tile, which every pass below asks for
+  int own_i0 = 0;
+  Range own_range{-1, 0};
+  auto tile_of = [&](int t, Seq* q, int* i0) -> Range {
+    if (t == tid && own_range.b0 >= 0) {
+      *q = own_seq, *i0 = own_i0;
+      return own_range;
+    }
+    const int b = seq_of_tile(first, s.num_seqs, t);
+    *q = load_seq(a.cu_q, a.cu_k, b, s.total_q, s.total_k, &bad);
+    *i0 = (t - first[b]) * tile;
+    const Range r =
+        list == 2 ? query_blocks(*q, *i0, s.causal) : key_blocks(*q, *i0, min(tile, q->lq - *i0), s.causal);
+    if (t == tid) own_seq = *q, own_i0 = *i0, own_range = r;
+    return r;
+  };
+
+  int mine = 0, mine_most = 0;
+  for (int t = tid; t < tiles; t += kPlanThreads) {
+    Seq q;
+    int i0;
+    const Range r = tile_of(t, &q, &i0);
+    mine += r.b1 - r.b0;
+    mine_most = max(mine_most, r.b1 - r.b0);
+  }
+  atomicMax(&most, mine_most);
+  int blocks;
+  block_scan(mine, &blocks);
+  // parts of at most `chunk` blocks: Σ ceil(b / chunk) ≤ tiles + blocks / chunk ≤ tiles + split_budget
+  const int chunk = list == 0 && s.split_budget ? max((blocks + s.split_budget - 1) / s.split_budget, 2) : 1 << 30;
+  const int top = max(1, min(most, chunk));
+
+  auto parts_of = [&](const Range& r) { return max(1, (r.b1 - r.b0 + chunk - 1) / chunk); };
+  auto size_class = [&](int n, int parts) { return kClasses - 1 - (int)((long long)(n / parts) * (kClasses - 1) / top); };
+  int slots = 0, items = 0;
+  for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
+    const int t = t0 + tid;
+    if (t < tiles) {
+      Seq q;
+      int i0;
+      const Range r = tile_of(t, &q, &i0);
+      const int p = parts_of(r);
+      atomicAdd(&hist[size_class(r.b1 - r.b0, p)], p);
+    }
+  }
+  __syncthreads();
+  {
+    int sum;
+    const int n = tid < kClasses ? hist[tid] : 0, before = block_scan(n, &sum);
+    if (tid < kClasses) cursor[tid] = before;
+    items = sum;
+  }
+  __syncthreads();
+  for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
+    const int t = t0 + tid;
+    Seq q{};
+    int i0 = 0, p = 0;
+    Range r{0, 0};
+    if (t < tiles) {
+      r = tile_of(t, &q, &i0);
+      p = parts_of(r);
+    }
+    int sum;
+    const int slot0 = slots + block_scan(p > 1 ? p : 0, &sum);
+    slots += sum;
+    if (t >= tiles) continue;
+    const int n = r.b1 - r.b0;
+    int at = atomicAdd(&cursor[size_class(n, p)], p);
+    if (list == 2) {
+      reinterpret_cast<KItem*>(a.plan + s.dkv_items)[at] =
+          KItem{q.k0 + i0, min(tile, q.lk - i0), i0, q.q0, q.lq, q.lk, r.b0, r.b1};
+      continue;
+    }
+    QItem* out = reinterpret_cast<QItem*>(a.plan + (list == 0 ? s.items : s.dq_items));
+    for (int k = 0; k < p; ++k, ++at)
+      out[at] = QItem{q.q0 + i0, min(tile, q.lq - i0), q.k0, q.lk, i0 + q.lk - q.lq,
+                      r.b0 + (int)((long long)n * k / p), r.b0 + (int)((long long)n * (k + 1) / p),
+                      p > 1 ? slot0 + k : -1, slot0, p, t, 0};
+  }
+  if (list == 0) {  // arrival counters of the split tiles
+    int* cnt = reinterpret_cast<int*>(a.plan + s.counters);
+    if (s.few)
+      for (int i = tid; i < tiles * s.units; i += kPlanThreads) cnt[i] = 0;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    hdr[list] = items;
+    hdr[kHdrBad + list] = bad;
+  }
+}
+
+
+}  // namespace
+
+int packed_check(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim) {
+  VA_CHECK_ARG(num_seqs > 0 && num_seqs <= kMaxSeqs && total_q >= 0 && total_k >= 0,
+               "packed attention: %d sequences, %d queries, %d keys", num_seqs, total_q, total_k);
+  VA_CHECK_ARG(total_q <= (1 << 30) && total_k <= (1 << 30), "packed attention: more than 2^30 tokens");
+  VA_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= kPackBlock && heads <= 4096,
+               "packed attention: %d query heads over %d key heads", heads, kv_heads);
+  VA_CHECK_ARG(dim >= 8 && dim <= 128 && dim % 8 == 0, "packed attention: head size %d (a multiple of 8 up to 128)",
+               dim);
+  return VA_OK;
+}
+
+}  // namespace va
+
+using namespace va;
+
+extern "C" {
+
+size_t va_packed_plan_bytes(int num_seqs, int total_q, int total_k, int num_heads, int num_kv_heads, int head_dim,
+                            int causal, int training) {
+  if (packed_check(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim)) return 0;
+  return packed_shape(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim, causal != 0, training != 0).total;
+}
+
+int va_packed_plan_build(const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int total_q, int total_k,
+                         int num_heads, int num_kv_heads, int head_dim, int causal, int training, void* plan,
+                         size_t plan_bytes, va_stream_t stream) {
+  if (int rc = packed_check(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim)) return rc;
+  VA_CHECK_ARG(cu_q && cu_k, "packed plan: null offsets");
+  PlanArgs a{cu_q, cu_k, static_cast<uint8_t*>(plan),
+             packed_shape(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim, causal != 0, training != 0)};
+  if (!plan || plan_bytes < a.s.total)
+    return set_error(VA_ERR_WORKSPACE, "packed plan: %zu < %zu bytes", plan_bytes, a.s.total);
+  if (reinterpret_cast<uintptr_t>(plan) & 255)
+    return set_error(VA_ERR_ALIGN, "packed plan: the buffer needs 256-byte alignment");
+  packed_plan_kernel<<<training ? 3 : 1, kPlanThreads, 0, (cudaStream_t)stream>>>(a);
+  return check_launch("packed plan");
+}
+
+int va_packed_plan_status(const void* plan, int training, int* bad_offsets, va_stream_t stream) {
+  VA_CHECK_ARG(plan && bad_offsets, "packed plan status: null pointer");
+  int bad[3] = {0, 0, 0};
+  const int lists = training ? 3 : 1;
+  cudaError_t e = cudaMemcpyAsync(bad, static_cast<const int*>(plan) + kHdrBad, lists * sizeof(int),
+                                  cudaMemcpyDeviceToHost, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
+  if (e != cudaSuccess) return set_error(VA_ERR_LAUNCH, "packed plan status: %s", cudaGetErrorString(e));
+  *bad_offsets = bad[0] | bad[1] | bad[2];
+  return VA_OK;
+}
+
+}  // extern "C"
