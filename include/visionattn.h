@@ -567,6 +567,22 @@ VA_API int va_packed_attention_fwd_f16(const void *q, const void *k, const void 
                                        int num_heads, int num_kv_heads, int head_dim, int causal, int training,
                                        float softmax_scale, void *plan, size_t plan_bytes, va_stream_t stream);
 
+/* Gradients of q, k and v (the latter two summed over the query heads that
+ * share a key head) from grad_out and the forward's out and lse; the plan must
+ * be built with `training`.  strides: as the forward's six, then grad_out row,
+ * head, grad_q row, head, grad_k row, head, grad_v row, head.  Rows of keys
+ * and queries that see nothing get zeros.  No atomics: the same bits each time. */
+VA_API int va_packed_attention_bwd_bf16(const va_bf16 *grad_out, const va_bf16 *q, const va_bf16 *k, const va_bf16 *v,
+                                        const va_bf16 *out, const float *lse, va_bf16 *grad_q, va_bf16 *grad_k, va_bf16 *grad_v,
+                                        const int64_t *strides, int num_seqs, int total_q, int total_k,
+                                        int num_heads, int num_kv_heads, int head_dim, int causal, int training,
+                                        float softmax_scale, void *plan, size_t plan_bytes, va_stream_t stream);
+VA_API int va_packed_attention_bwd_f16(const void *grad_out, const void *q, const void *k, const void *v,
+                                        const void *out, const float *lse, void *grad_q, void *grad_k, void *grad_v,
+                                        const int64_t *strides, int num_seqs, int total_q, int total_k,
+                                        int num_heads, int num_kv_heads, int head_dim, int causal, int training,
+                                        float softmax_scale, void *plan, size_t plan_bytes, va_stream_t stream);
+
 /* Device status word of the tensor-core kernels: 0, or 1000+site of the
  * first bounded wait that gave up.  read: copies it to *status (synchronises
  * `stream`); clear: resets it to 0. */

@@ -101,6 +101,8 @@ SIGNATURES: dict[str, tuple] = {
     "va_packed_plan_status": (I, [P, I, C.POINTER(C.c_int), S]),
     **{f"va_packed_attention_fwd_{t}": (I, [P, P, P, P, P, I64P, I, I, I, I, I, I, I, I, F, P, SZ, S])
        for t in ("bf16", "f16")},
+    **{f"va_packed_attention_bwd_{t}": (I, [P] * 9 + [I64P, I, I, I, I, I, I, I, I, F, P, SZ, S])
+       for t in ("bf16", "f16")},
     "va_device_status_read": (I, [C.POINTER(C.c_int), S]),
     "va_device_status_clear": (I, [S]),
 }

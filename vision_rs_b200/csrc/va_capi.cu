@@ -134,15 +134,16 @@ int va_psa_flash_attention_fwd_f16(const void* qk, const void* v, void* o, float
 
 int va_device_status_read(int* status, va_stream_t s) {  // first non-zero word of the tensor-core kernels
   if (!status) return set_error(VA_ERR_SHAPE, "device_status_read: null output");
-  int v[6] = {0, 0, 0, 0, 0, 0};
+  int v[7] = {0, 0, 0, 0, 0, 0, 0};
   if (int rc = tc_status_read(&v[0], (cudaStream_t)s)) return rc;
   if (int rc = dino_status_read(&v[1], (cudaStream_t)s)) return rc;
   if (int rc = gemm_status_read(&v[2], (cudaStream_t)s)) return rc;
   if (int rc = bwd_status_read(&v[3], (cudaStream_t)s)) return rc;
   if (int rc = conv_status_read(&v[4], (cudaStream_t)s)) return rc;
   if (int rc = packed_status_read(&v[5], (cudaStream_t)s)) return rc;
+  if (int rc = packed_bwd_status_read(&v[6], (cudaStream_t)s)) return rc;
   *status = 0;
-  for (int i = 0; i < 6 && !*status; ++i) *status = v[i];
+  for (int i = 0; i < 7 && !*status; ++i) *status = v[i];
   return VA_OK;
 }
 
@@ -152,6 +153,7 @@ int va_device_status_clear(va_stream_t s) {
   if (int rc = gemm_status_clear((cudaStream_t)s)) return rc;
   if (int rc = conv_status_clear((cudaStream_t)s)) return rc;
   if (int rc = packed_status_clear((cudaStream_t)s)) return rc;
+  if (int rc = packed_bwd_status_clear((cudaStream_t)s)) return rc;
   return bwd_status_clear((cudaStream_t)s);
 }
 

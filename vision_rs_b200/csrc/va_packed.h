@@ -3,6 +3,7 @@
 // va_packed_attn_bwd.cu).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -49,7 +50,7 @@ struct PackedShape {
   int max_tiles, max_items, max_slots, split_budget;
   int max_dq_items, max_dkv_items;
   // byte offsets in the plan
-  size_t items, dq_items, dkv_items, counters, scratch, part_o, part_lse, total;
+  size_t items, dq_items, dkv_items, counters, scratch, part_o, part_lse, rows, do_norm, v_norm, total;
 };
 
 // Header words of the plan, one of each for the three lists: the number of
@@ -84,6 +85,10 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   s.scratch = o, o += pk_align(num_seqs > kPlanSeqs ? (size_t)3 * (num_seqs + 1) * 4 : 0);
   s.part_o = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * dim * 4);
   s.part_lse = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * 4);
+  // training: (lse·log2 e, Δ) a query and head, ‖dO_i‖ and ‖V_j‖ (the f16 backward's)
+  s.rows = o, o += pk_align(training ? (size_t)total_q * heads * 8 : 0);
+  s.do_norm = o, o += pk_align(training ? (size_t)total_q * heads * 4 : 0);
+  s.v_norm = o, o += pk_align(training ? (size_t)total_k * kv_heads * 4 : 0);
   s.total = o;
   return s;
 }
@@ -92,6 +97,9 @@ int packed_status_read(int* out, cudaStream_t st);
 int packed_status_clear(cudaStream_t st);
 int packed_bwd_status_read(int* out, cudaStream_t st);
 int packed_bwd_status_clear(cudaStream_t st);
+// Tensor map over [rows, heads, dim] (strides in elements) in boxes of 64 dims × box_heads × box_rows.
+int packed_map(CUtensorMap* m, const void* base, bool bf16, int rows, int heads, int dim, long long row_stride,
+               long long head_stride, int box_heads, int box_rows, const char* what);
 // Argument checks shared by the entry points (VA_OK or an error that is set).
 int packed_check(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim);
 

@@ -43,6 +43,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.0f;  // the reference follows the maximum once it is 2^8 ahead
+constexpr float kF16Shift = 7.0f;   // f16: P is held times 2^7 (at most 2^15), so small ones keep their bits
 
 // DP: head size in shared memory and TMEM (64 or 128; the TMA boxes fill what is past `dim` with zeros).
 template <int DP, int TILES> struct FwdCfg {
@@ -295,7 +296,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           }
           ref = next;
         }
-        const float base = ref == -INFINITY ? 0.0f : ref;
+        const float base = ref == -INFINITY ? 0.0f : BF16 ? ref : ref - kF16Shift;
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -320,7 +321,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (ok && !idle) {
       tc_fence_after();
       const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-      const float lse = n > 0 && ref != -INFINITY ? (ref + log2f(sum)) * kLn2 : -INFINITY;
+      const float lse = n > 0 && ref != -INFINITY ? (ref - (BF16 ? 0.0f : kF16Shift) + log2f(sum)) * kLn2 : -INFINITY;
       const int t = my_row / group, h = ps.few ? head * group + my_row - t * group : head;
       if (it.slot < 0) {
         const long long at = (long long)(it.q0 + t) * ps.heads + h;
@@ -431,7 +432,6 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 }  // namespace
 
-// [rows, heads, dim] (strides in elements) in boxes of 64 dims × box_heads × box_rows.
 int packed_map(CUtensorMap* m, const void* base, bool bf16, int rows, int heads, int dim, long long row_stride,
                long long head_stride, int box_heads, int box_rows, const char* what) {
   auto fn = encode_fn();

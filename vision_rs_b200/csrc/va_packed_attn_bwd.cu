@@ -1,0 +1,732 @@
+// Gradient of the packed-sequence attention (tcgen05 + TMEM + TMA).  With
+// P = exp(scale·q·k − lse) and Δ_i = dO_i·O_i, per head:
+//
+//   dV_j = Σ_i P_ij dO_i,   dS = P ⊙ (dO Vᵀ − Δ),
+//   dQ_i = scale Σ_j dS_ij k_j,   dK_j = scale Σ_i dS_ij q_i
+//
+// (dK and dV summed over the query heads that share the key head).  Three
+// launches, no atomics, so the results do not depend on scheduling:
+//
+//   row kernel   (lse·log2 e, Δ) of every query and head
+//   dK/dV kernel a CTA per (128 keys, key head) walks the group's heads and
+//                their queries in steps of 64: Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ in
+//                TMEM, Pᵀ and dSᵀ back into the same columns in 16 bits, then
+//                dV += Pᵀ·dO, dK += dSᵀ·Q with the TMEM operand
+//   dQ kernel    a CTA per (128 queries, head) walks the keys in steps of 64:
+//                S = Q·Kᵀ, dP = dO·Vᵀ with Q and dO as TMEM operands, dS in
+//                TMEM, dQ += dS·K
+//
+// S and dP are computed twice (7 products instead of 5); the one-kernel form
+// would add f32 dQ partials to memory from every key tile, in an order that
+// changes from run to run, or write and read all of them.  Two score buffers
+// and two softmax groups alternate, so the MMAs of one step run under the
+// exponentials of the other.  Steps are 64 wide because dV, dK (256 columns)
+// and two buffers of S and dP (4 × 64) fill the 512 TMEM columns at 128 dims.
+//
+// P and dS are 16-bit operands.  f16 has few exponents, so there P carries
+// 2^15 and dS a power of two chosen for its row (key or query) such that the
+// largest possible |dS| stays below 2^15: |dO_i·V_j| ≤ ‖dO_i‖·‖V_j‖; the f32
+// sums are scaled back at the end.  bf16 needs neither.
+//
+// Rows of other sequences in a tile are masked by selection, and the rows of
+// the summed operand past the sequence's end are zeroed (0 · NaN is NaN).
+#include <cudaTypedefs.h>
+
+#include "va_common.cuh"
+#include "va_packed.h"
+#include "va_sm100.cuh"
+
+namespace va {
+using namespace sm100;
+
+__device__ int g_packed_bwd_status;
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kHalf = 64;     // queries (or keys) a step
+constexpr int kStages = 4;    // ring of 64-row (Q, dO) or (K, V) pairs
+constexpr int kThreads = 320; // 2 × 4 warps of scores, 1 TMA, 1 MMA
+constexpr float kPShift = 15.0f;     // f16: P is held times 2^15
+constexpr uint32_t kColAcc = 256;    // score buffers at 0 (S 64, dP 64) and 128; accumulators from here
+
+template <int DP> struct BwdSmem {
+  static constexpr int kTile = kPackBlock * DP * 2, kStep = kHalf * DP * 2;
+  uint8_t a[2][kTile];               // K and V of the keys, or Q and dO of the queries: per 64 dims 128 rows × 128 bytes
+  uint8_t ring[kStages][2][kStep];   // per 64 dims 64 rows × 128 bytes
+  float4 stats[2][2][kHalf / 2];     // dK/dV: (lse, Δ) of the step's queries, per group, two steps
+  float red[8];
+  uint64_t a_full, a_ready, full[kStages], empty[kStages], s_full[2], p_full[2], g_done[2], fin;
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct BwdArgs {
+  uint8_t* plan;
+  PackedShape s;
+  void *dq, *dk, *dv;
+  long long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  float scale;
+};
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) return pack_bf16x2(a, b);
+  else return pack_f16x2(a, b);
+}
+__device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
+
+// Largest power of two p with bound·p < 2^15 (1 for a bound of zero; the exponent is kept within ±60).
+__device__ __forceinline__ float pow2_below(float bound) {
+  if (!(bound > 0.0f) || !(bound < INFINITY)) return 1.0f;
+  const int e = min(60, max(-60, 14 - ilogbf(bound)));
+  return __int_as_float((127 + e) << 23);
+}
+
+// Zeroes rows [used, 16·ceil(used/16)) of a 64-row tile, whole warp.
+template <int DP> __device__ __forceinline__ void zero_tail(uint8_t* tile, int used, int lane) {
+  const int n = ((used + 15) / 16 * 16 - used) * (DP / 8);
+  for (int i = lane; i < n; i += 32) {
+    const int r = used + i / (DP / 8), c = i % (DP / 8);
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kHalf * 128 + sw128_off(r, c & 7)) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Set-up shared by both kernels: barriers and TMEM.
+template <int DP> __device__ __forceinline__ uint32_t bwd_setup(BwdSmem<DP>& sm, int tid, int warp) {
+  if (tid == 0) {
+    mbar_init(&sm.a_full, 1);
+    mbar_init(&sm.a_ready, 256);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.s_full[b], 1);
+      mbar_init(&sm.p_full[b], 128);
+      mbar_init(&sm.g_done[b], 1);
+    }
+    mbar_init(&sm.fin, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&sm.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return sm.tmem_base;
+}
+
+// 16 accumulator columns of the thread's row → out[c .. c+16) times f (rows that are stored, dims below dim).
+template <bool BF16>
+__device__ __forceinline__ void store16(uint32_t taddr, bool zero, float f, bool mine, uint16_t* out, int c, int dim) {
+  uint32_t o[16] = {};
+  if (!zero) {
+    tmem_ld16(taddr + c, o);
+    tmem_ld_wait();
+    reg_fence(o);
+  }
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    w[i] = zero ? 0u : pack2<BF16>(__uint_as_float(o[2 * i]) * f, __uint_as_float(o[2 * i + 1]) * f);
+  if (mine) {
+    *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (c + 8 < dim) *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  __syncwarp();
+}
+
+// Producer: the ring's steps, each two 64-row tiles.  at(h, &head, &row) says where step h begins.
+template <int DP, typename At>
+__device__ __forceinline__ void produce(BwdSmem<DP>& sm, const CUtensorMap* m0, const CUtensorMap* m1, int n, At at) {
+  constexpr int NB = DP / 64;
+  bool ok = true;
+  int issued = 0;
+  for (int h = 0; h < n; ++h) {
+    const int st = h % kStages;
+    if (h >= kStages && !(ok = mbar_wait(&sm.empty[st], (h / kStages - 1) & 1, &sm.abort, &g_packed_bwd_status, 1)))
+      break;
+    int head, row;
+    at(h, &head, &row);
+    mbar_arrive_expect_tx(&sm.full[st], 2 * BwdSmem<DP>::kStep);
+    for (int b = 0; b < NB; ++b) {
+      tma_load_3d(sm.ring[st][0] + b * kHalf * 128, m0, &sm.full[st], b * 64, head, row);
+      tma_load_3d(sm.ring[st][1] + b * kHalf * 128, m1, &sm.full[st], b * 64, head, row);
+    }
+    ++issued;
+  }
+  if (!ok) {  // loads issued here land (bounded) before the CTA can exit
+    for (int h = max(0, issued - kStages); h < issued; ++h) {
+      const long long c0 = clock64();
+      while (!mbar_try_wait(&sm.full[h % kStages], (h / kStages) & 1) && clock64() - c0 < kSpinCycles) {
+      }
+    }
+    const long long c0 = clock64();
+    while (!mbar_try_wait(&sm.a_full, 0) && clock64() - c0 < kSpinCycles) {
+    }
+  }
+}
+
+// ── (lse·log2 e, Δ) and, for f16, the norms that bound dS ───────────────────
+template <bool BF16>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
+}
+
+// 16 lanes a (token, head) row.  Rows below nq: Δ of a query; the rest (f16): ‖V_j‖.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+packed_rows_kernel(const uint16_t* __restrict__ out, const uint16_t* __restrict__ d_out, long long do_row,
+                   long long do_head, const uint16_t* __restrict__ v, long long v_row, long long v_head,
+                   const float* __restrict__ lse, float2* __restrict__ pairs, float* __restrict__ do_norm,
+                   float* __restrict__ v_norm, int total_q, int total_k, int heads, int kv_heads, int dim) {
+  const long long r = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), nq = (long long)total_q * heads;
+  const int c = (threadIdx.x & 15) * 8;
+  float dot = 0.0f, sq = 0.0f;
+  const bool is_q = r < nq, in = r < nq + (BF16 ? 0 : (long long)total_k * kv_heads);
+  int t = 0, h = 0;
+  if (in) {
+    const int hn = is_q ? heads : kv_heads;
+    const long long rr = is_q ? r : r - nq;
+    t = (int)(rr / hn), h = (int)(rr - (long long)t * hn);
+    if (c < dim) {
+      float a[8], b[8];
+      if (is_q) {
+        unpack8<BF16>(*reinterpret_cast<const uint4*>(out + r * dim + c), a);
+        unpack8<BF16>(*reinterpret_cast<const uint4*>(d_out + t * do_row + h * do_head + c), b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot = fmaf(a[i], b[i], dot);
+      } else {
+        unpack8<BF16>(*reinterpret_cast<const uint4*>(v + t * v_row + h * v_head + c), b);
+      }
+      if constexpr (!BF16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq = fmaf(b[i], b[i], sq);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) {
+    dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if constexpr (!BF16) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+  }
+  if (!in || (threadIdx.x & 15)) return;
+  if (is_q) {
+    const long long at = (long long)h * total_q + t;
+    pairs[at] = make_float2(lse[at] * kLog2e, dot);
+    if constexpr (!BF16) do_norm[at] = sqrtf(sq);
+  } else if constexpr (!BF16) {
+    v_norm[(long long)h * total_k + t] = sqrtf(sq);
+  }
+}
+
+// ── dK and dV ────────────────────────────────────────────────────────────────
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, BwdArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const PackedShape& ps = a.s;
+  const int unit = blockIdx.x / ps.kv_heads, kvh = blockIdx.x - unit * ps.kv_heads;
+  if (unit >= reinterpret_cast<const int*>(a.plan)[kHdrDkv]) return;
+  const KItem it = reinterpret_cast<const KItem*>(a.plan + ps.dkv_items)[unit];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int dim16 = (ps.dim + 15) & ~15;
+  // steps of 64 queries: from the first that sees a key of the tile
+  const int first_q = ps.causal ? max(0, it.j0 - (it.lk - it.lq)) : 0;
+  const int hb0 = first_q / kHalf, nh = max(0, (it.lq + kHalf - 1) / kHalf - hb0), n = nh * ps.group;
+  const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
+
+  if (warp == 8) {
+    if (lane == 0 && n > 0) {
+      constexpr int NB = DP / 64;
+      mbar_arrive_expect_tx(&sm.a_full, 2 * BwdSmem<DP>::kTile);
+      for (int b = 0; b < NB; ++b) {
+        tma_load_3d(sm.a[0] + b * kPackBlock * 128, &map_k, &sm.a_full, b * 64, kvh, it.k0);
+        tma_load_3d(sm.a[1] + b * kPackBlock * 128, &map_v, &sm.a_full, b * 64, kvh, it.k0);
+      }
+      produce<DP>(sm, &map_q, &map_do, n, [&](int h, int* head, int* row) {
+        *head = kvh * ps.group + h / nh;
+        *row = it.q0 + (hb0 + h % nh) * kHalf;
+      });
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (n > 0) {
+      const uint32_t fmt = BF16 ? AB_BF16 : AB_F16;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &sm.abort, &g_packed_bwd_status, where));
+      };
+      const uint32_t id_s = idesc_f32acc(kPackBlock, kHalf, fmt, false, false);
+      const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, fmt, false, true);
+      const uint64_t dk = sdesc(smem_u32(sm.a[0]), 16, 1024, SW_128B), dv = sdesc(smem_u32(sm.a[1]), 16, 1024, SW_128B);
+      auto used_of = [&](int h) { return min(kHalf, it.lq - (hb0 + h % nh) * kHalf); };
+      auto issue_s = [&](int h) {  // Sᵀ = K·Qᵀ, dPᵀ = V·dOᵀ
+        const int st = h % kStages, used = used_of(h);
+        if (used & 15) {
+          zero_tail<DP>(sm.ring[st][0], used, lane);
+          zero_tail<DP>(sm.ring[st][1], used, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const uint64_t bq = sdesc(smem_u32(sm.ring[st][0]), 16, 1024, SW_128B);
+        const uint64_t bo = sdesc(smem_u32(sm.ring[st][1]), 16, 1024, SW_128B);
+        const uint32_t ts = tmem + (h & 1) * 128;
+        for (int s = 0; s < dim16 / 16; ++s) {
+          const uint64_t oa = (uint64_t)((s >> 2) * ((kPackBlock * 128) >> 4) + (s & 3) * 2);
+          const uint64_t ob = (uint64_t)((s >> 2) * ((kHalf * 128) >> 4) + (s & 3) * 2);
+          mma_ss_w(ts, dk + oa, bq + ob, id_s, s > 0 ? 1u : 0u);
+          mma_ss_w(ts + kHalf, dv + oa, bo + ob, id_s, s > 0 ? 1u : 0u);
+        }
+        mma_commit_w(&sm.s_full[h & 1]);
+      };
+      bool ok = wait(&sm.a_full, 0, 2);
+      for (int h = 0; ok && h < min(2, n); ++h) {
+        if (!(ok = wait(&sm.full[h], 0, 3))) break;
+        tc_fence_after();
+        issue_s(h);
+      }
+      for (int h = 0; ok && h < n; ++h) {
+        const int b = h & 1, st = h % kStages, steps = (used_of(h) + 15) >> 4;
+        if (!(ok = wait(&sm.p_full[b], (h >> 1) & 1, 4))) break;
+        tc_fence_after();
+        const uint64_t gq = sdesc(smem_u32(sm.ring[st][0]), kHalf * 128, 1024, SW_128B);
+        const uint64_t go = sdesc(smem_u32(sm.ring[st][1]), kHalf * 128, 1024, SW_128B);
+        const uint32_t tp = tmem + b * 128;
+        for (int s = 0; s < steps; ++s) {
+          const uint32_t acc = (h > 0 || s > 0) ? 1u : 0u;
+          mma_ts_w(tmem + kColAcc, tp + s * 8, go + (uint64_t)(s * (2048 >> 4)), id_g, acc);
+          mma_ts_w(tmem + kColAcc + DP, tp + kHalf + s * 8, gq + (uint64_t)(s * (2048 >> 4)), id_g, acc);
+        }
+        mma_commit_w(&sm.empty[st]);
+        mma_commit_w(&sm.g_done[b]);
+        if (h + 2 < n) {
+          const int h2 = h + 2;
+          // the next scores overwrite P's and dS's columns: the products have to be done with them
+          if (!(ok = wait(&sm.full[h2 % kStages], (h2 / kStages) & 1, 5) && wait(&sm.g_done[b], (h >> 1) & 1, 6))) break;
+          tc_fence_after();
+          issue_s(h2);
+        }
+      }
+      mma_commit_w(&sm.fin);  // every MMA issued here completes before the CTA tears down
+      const long long c0 = clock64();
+      while (!mbar_try_wait(&sm.fin, 0) && clock64() - c0 < kSpinCycles) {
+      }
+    }
+    __syncwarp();
+  } else {
+    // ── scores: group g takes steps h ≡ g (mod 2), thread = key ──
+    const int g = warp >> 2, key = tid - g * 128;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + g * 128;
+    const float2* pairs = reinterpret_cast<const float2*>(a.plan + ps.rows);
+    const float scale2 = a.scale * kLog2e;
+    const bool mine = key < it.keys;
+    float mult = 1.0f;
+    if constexpr (!BF16) {  // |dS_ij| ≤ max_i ‖dO_i‖ · ‖V_j‖ + max_i |Δ_i|
+      const float* norms = reinterpret_cast<const float*>(a.plan + ps.do_norm);
+      float top_n = 0.0f, top_d = 0.0f;
+      for (int i = tid; i < nh * kHalf * ps.group; i += 256) {
+        const int gh = i / (nh * kHalf), q = hb0 * kHalf + i - gh * nh * kHalf;
+        if (q >= it.lq) continue;
+        const long long at = (long long)(kvh * ps.group + gh) * ps.total_q + it.q0 + q;
+        top_n = fmaxf(top_n, norms[at]);
+        top_d = fmaxf(top_d, fabsf(pairs[at].y));
+      }
+      for (int o = 16; o; o >>= 1) {
+        top_n = fmaxf(top_n, __shfl_xor_sync(0xffffffffu, top_n, o));
+        top_d = fmaxf(top_d, __shfl_xor_sync(0xffffffffu, top_d, o));
+      }
+      float* red = reinterpret_cast<float*>(sm.stats);
+      if (lane == 0) red[warp] = top_n, red[8 + warp] = top_d;
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      for (int i = 0; i < 8; ++i) top_n = fmaxf(top_n, red[i]), top_d = fmaxf(top_d, red[8 + i]);
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      const float vn = mine ? reinterpret_cast<const float*>(a.plan + ps.v_norm)[(long long)kvh * ps.total_k + it.k0 + key] : 0.0f;
+      mult = pow2_below(top_n * vn + top_d);
+    }
+    const float mult_p = BF16 ? 1.0f : mult * 3.0517578125e-05f;  // dS from P·2^15
+    const int off = it.lk - it.lq, j = it.j0 + key;
+    bool ok = true;
+    // (lse, Δ) of a step's query, fetched a step ahead by the group's first 64 threads
+    auto fetch = [&](int h) -> float2 {
+      float2 f = make_float2(INFINITY, 0.0f);  // past the sequence: P = 2^−∞
+      if (h < n && key < kHalf) {
+        const int i = (hb0 + h % nh) * kHalf + key;
+        if (i < it.lq) f = pairs[(long long)(kvh * ps.group + h / nh) * ps.total_q + it.q0 + i];
+        if constexpr (!BF16) f.x -= kPShift;
+      }
+      return f;
+    };
+    float2 ahead = fetch(g);
+    for (int h = g; h < n; h += 2) {
+      const int k = h >> 1;
+      float4* st = sm.stats[g][k & 1];
+      if (key < kHalf) reinterpret_cast<float2*>(st)[key] = ahead;
+      group_sync(g);
+      ahead = fetch(h + 2);
+      const int i0 = (hb0 + h % nh) * kHalf;
+      // queries [lo, hi) of the step see this key
+      const int lo = ps.causal ? j - off - i0 : 0, hi = it.lq - i0;
+      const bool whole = hi >= kHalf && (!ps.causal || it.j0 + it.keys - 1 - off <= i0);
+      if (!(ok = mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 8))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], d[32];
+        tmem_ld32(ts + c * 32, s);
+        tmem_ld32(ts + kHalf + c * 32, d);
+        tmem_ld_wait();
+        reg_fence(s);
+        reg_fence(d);
+        uint32_t pp[16], pd[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float4 q = st[(c * 32 + i) >> 1];
+          float p0 = ex2(fmaf(__uint_as_float(s[i]), scale2, -q.x));
+          float p1 = ex2(fmaf(__uint_as_float(s[i + 1]), scale2, -q.z));
+          float d0 = p0 * (__uint_as_float(d[i]) - q.y);
+          float d1 = p1 * (__uint_as_float(d[i + 1]) - q.w);
+          if (!whole) {
+            const bool v0 = c * 32 + i >= lo && c * 32 + i < hi, v1 = c * 32 + i + 1 >= lo && c * 32 + i + 1 < hi;
+            p0 = v0 ? p0 : 0.0f;
+            d0 = v0 ? d0 : 0.0f;
+            p1 = v1 ? p1 : 0.0f;
+            d1 = v1 ? d1 : 0.0f;
+          }
+          if constexpr (!BF16) d0 *= mult_p, d1 *= mult_p;
+          pp[i >> 1] = pack2<BF16>(p0, p1);
+          pd[i >> 1] = pack2<BF16>(d0, d1);
+        }
+        tmem_st16(ts + c * 16, pp);
+        tmem_st16(ts + kHalf + c * 16, pd);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[g]);
+    }
+    if (n > 0) ok = mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 9) && ok;
+    if (ok && !sm.abort) {  // group 0 stores dV, group 1 dK
+      tc_fence_after();
+      const long long row = it.k0 + key;
+      uint16_t* out = g == 0 ? static_cast<uint16_t*>(a.dv) + row * a.dv_row + kvh * a.dv_head
+                             : static_cast<uint16_t*>(a.dk) + row * a.dk_row + kvh * a.dk_head;
+      const float f = g == 0 ? (BF16 ? 1.0f : 3.0517578125e-05f) : a.scale / mult;
+      for (int c = 0; c < dim16; c += 16)
+        store16<BF16>(tmem + lanes + kColAcc + g * DP, n == 0, f, mine, out, c, ps.dim);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+// ── dQ ───────────────────────────────────────────────────────────────────────
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, BwdArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const PackedShape& ps = a.s;
+  const int unit = blockIdx.x / ps.heads, head = blockIdx.x - unit * ps.heads, kvh = head / ps.group;
+  if (unit >= reinterpret_cast<const int*>(a.plan)[kHdrDq]) return;
+  const QItem it = reinterpret_cast<const QItem*>(a.plan + ps.dq_items)[unit];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int dim16 = (ps.dim + 15) & ~15;
+  const int see_end = ps.causal ? min(it.lk, max(0, it.see + it.tokens)) : it.lk;  // one past the last key that is seen
+  const int n = (see_end + kHalf - 1) / kHalf;
+  constexpr uint32_t kColQ = kColAcc + DP, kColDO = kColQ + DP / 2;
+  const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
+
+  if (warp == 8) {
+    if (lane == 0 && n > 0) {
+      constexpr int NB = DP / 64;
+      mbar_arrive_expect_tx(&sm.a_full, 2 * BwdSmem<DP>::kTile);
+      for (int b = 0; b < NB; ++b) {
+        tma_load_3d(sm.a[0] + b * kPackBlock * 128, &map_q, &sm.a_full, b * 64, head, it.q0);
+        tma_load_3d(sm.a[1] + b * kPackBlock * 128, &map_do, &sm.a_full, b * 64, head, it.q0);
+      }
+      produce<DP>(sm, &map_k, &map_v, n, [&](int h, int* hd, int* row) {
+        *hd = kvh;
+        *row = it.k0 + h * kHalf;
+      });
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (n > 0) {
+      const uint32_t fmt = BF16 ? AB_BF16 : AB_F16;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &sm.abort, &g_packed_bwd_status, where));
+      };
+      const uint32_t id_s = idesc_f32acc(kPackBlock, kHalf, fmt, false, false);
+      const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, fmt, false, true);
+      auto used_of = [&](int h) { return min(kHalf, see_end - h * kHalf); };
+      auto issue_s = [&](int h) {  // S = Q·Kᵀ, dP = dO·Vᵀ
+        const int st = h % kStages, used = used_of(h);
+        if (used & 15) {
+          zero_tail<DP>(sm.ring[st][0], used, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const uint64_t bk = sdesc(smem_u32(sm.ring[st][0]), 16, 1024, SW_128B);
+        const uint64_t bv = sdesc(smem_u32(sm.ring[st][1]), 16, 1024, SW_128B);
+        const uint32_t ts = tmem + (h & 1) * 128;
+        for (int s = 0; s < dim16 / 16; ++s) {
+          const uint64_t ob = (uint64_t)((s >> 2) * ((kHalf * 128) >> 4) + (s & 3) * 2);
+          mma_ts_w(ts, tmem + kColQ + s * 8, bk + ob, id_s, s > 0 ? 1u : 0u);
+          mma_ts_w(ts + kHalf, tmem + kColDO + s * 8, bv + ob, id_s, s > 0 ? 1u : 0u);
+        }
+        mma_commit_w(&sm.s_full[h & 1]);
+      };
+      bool ok = wait(&sm.a_ready, 0, 12);
+      for (int h = 0; ok && h < min(2, n); ++h) {
+        if (!(ok = wait(&sm.full[h], 0, 13))) break;
+        tc_fence_after();
+        issue_s(h);
+      }
+      for (int h = 0; ok && h < n; ++h) {
+        const int b = h & 1, st = h % kStages, steps = (used_of(h) + 15) >> 4;
+        if (!(ok = wait(&sm.p_full[b], (h >> 1) & 1, 14))) break;
+        tc_fence_after();
+        const uint64_t gk = sdesc(smem_u32(sm.ring[st][0]), kHalf * 128, 1024, SW_128B);
+        for (int s = 0; s < steps; ++s)
+          mma_ts_w(tmem + kColAcc, tmem + b * 128 + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g,
+                   (h > 0 || s > 0) ? 1u : 0u);
+        mma_commit_w(&sm.empty[st]);
+        mma_commit_w(&sm.g_done[b]);
+        if (h + 2 < n) {
+          const int h2 = h + 2;
+          if (!(ok = wait(&sm.full[h2 % kStages], (h2 / kStages) & 1, 15) && wait(&sm.g_done[b], (h >> 1) & 1, 16)))
+            break;
+          tc_fence_after();
+          issue_s(h2);
+        }
+      }
+      mma_commit_w(&sm.fin);
+      const long long c0 = clock64();
+      while (!mbar_try_wait(&sm.fin, 0) && clock64() - c0 < kSpinCycles) {
+      }
+    }
+    __syncwarp();
+  } else {
+    const int g = warp >> 2, row = tid - g * 128;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + g * 128;
+    const bool mine = row < it.tokens;
+    const int see = !mine ? 0 : ps.causal ? min(it.lk, it.see + row + 1) : it.lk;
+    float2 stat = make_float2(INFINITY, 0.0f);
+    const long long at = (long long)head * ps.total_q + it.q0 + row;
+    if (mine) stat = reinterpret_cast<const float2*>(a.plan + ps.rows)[at];
+    float mult = 1.0f;
+    if constexpr (!BF16) {  // |dS_ij| ≤ ‖dO_i‖ · max_j ‖V_j‖ + |Δ_i|
+      const float* vn = reinterpret_cast<const float*>(a.plan + ps.v_norm) + (long long)kvh * ps.total_k + it.k0;
+      float top = 0.0f;
+      for (int i = tid; i < see_end; i += 256) top = fmaxf(top, vn[i]);
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) sm.red[warp] = top;
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, sm.red[i]);
+      if (mine) mult = pow2_below(reinterpret_cast<const float*>(a.plan + ps.do_norm)[at] * top + fabsf(stat.y));
+    }
+    const float scale2 = a.scale * kLog2e;
+    bool ok = true;
+    if (n > 0) {
+      // group 0 moves Q, group 1 dO from shared memory to TMEM: a thread its row
+      ok = mbar_wait(&sm.a_full, 0, &sm.abort, &g_packed_bwd_status, 17);
+      if (ok) {
+#pragma unroll
+        for (int b = 0; b < DP / 64; ++b) {
+          uint32_t u[32];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(sm.a[g] + b * kPackBlock * 128 + sw128_off(row, c));
+            u[4 * c] = w.x, u[4 * c + 1] = w.y, u[4 * c + 2] = w.z, u[4 * c + 3] = w.w;
+          }
+          tmem_st32(tmem + lanes + (g == 0 ? kColQ : kColDO) + b * 32, u);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sm.a_ready);
+      }
+    }
+    for (int h = g; ok && h < n; h += 2) {
+      if (!(ok = mbar_wait(&sm.s_full[g], (h >> 1) & 1, &sm.abort, &g_packed_bwd_status, 18))) break;
+      tc_fence_after();
+      const int limit = see - h * kHalf;
+      const bool whole = __all_sync(0xffffffffu, limit >= kHalf);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], d[32];
+        tmem_ld32(ts + c * 32, s);
+        tmem_ld32(ts + kHalf + c * 32, d);
+        tmem_ld_wait();
+        reg_fence(s);
+        reg_fence(d);
+        uint32_t pd[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float d0 = ex2(fmaf(__uint_as_float(s[i]), scale2, -stat.x)) * (__uint_as_float(d[i]) - stat.y);
+          float d1 = ex2(fmaf(__uint_as_float(s[i + 1]), scale2, -stat.x)) * (__uint_as_float(d[i + 1]) - stat.y);
+          if (!whole) {
+            d0 = c * 32 + i < limit ? d0 : 0.0f;
+            d1 = c * 32 + i + 1 < limit ? d1 : 0.0f;
+          }
+          if constexpr (!BF16) d0 *= mult, d1 *= mult;
+          pd[i >> 1] = pack2<BF16>(d0, d1);
+        }
+        tmem_st16(ts + c * 16, pd);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[g]);
+    }
+    if (n > 0) ok = mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 19) && ok;
+    if (ok && !sm.abort) {  // each group stores half of the 16-column chunks
+      tc_fence_after();
+      uint16_t* out = static_cast<uint16_t*>(a.dq) + (it.q0 + row) * a.dq_row + head * a.dq_head;
+      for (int c = g * 16; c < dim16; c += 32)
+        store16<BF16>(tmem + lanes + kColAcc, n == 0, a.scale / mult, mine, out, c, ps.dim);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+template <typename K> int set_smem(K kernel, int smem) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  return e == cudaSuccess ? VA_OK : set_error(VA_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+}
+
+struct BwdMaps {
+  CUtensorMap q_tile, do_tile, k_tile, v_tile, q_step, do_step, k_step, v_step;
+};
+
+template <int DP, bool BF16> int launch_bwd(const BwdMaps& m, const BwdArgs& a, cudaStream_t st) {
+  constexpr int smem = (int)sizeof(BwdSmem<DP>) + 1024;
+  static PerDeviceOnce once;
+  if (int rc = once.run([&]() -> int {
+        if (int rc = set_smem(packed_dkv_kernel<DP, BF16>, smem)) return rc;
+        return set_smem(packed_dq_kernel<DP, BF16>, smem);
+      }))
+    return rc;
+  const long long g1 = (long long)a.s.max_dkv_items * a.s.kv_heads, g2 = (long long)a.s.max_dq_items * a.s.heads;
+  VA_CHECK_ARG(g1 < (1LL << 31) && g2 < (1LL << 31), "packed attention backward: too many units");
+  if (g1 > 0) {
+    packed_dkv_kernel<DP, BF16><<<(unsigned)g1, kThreads, smem, st>>>(m.q_step, m.do_step, m.k_tile, m.v_tile, a);
+    if (int rc = check_launch("packed attention dK/dV")) return rc;
+  }
+  if (g2 > 0) {
+    packed_dq_kernel<DP, BF16><<<(unsigned)g2, kThreads, smem, st>>>(m.q_tile, m.do_tile, m.k_step, m.v_step, a);
+    if (int rc = check_launch("packed attention dQ")) return rc;
+  }
+  return VA_OK;
+}
+
+template <bool BF16>
+int packed_bwd(const void* d_out, const void* q, const void* k, const void* v, const void* out, const float* lse,
+               void* dq, void* dk, void* dv, const int64_t* strides, int num_seqs, int total_q, int total_k, int heads,
+               int kv_heads, int dim, int causal, int training, float scale, void* plan, size_t plan_bytes,
+               cudaStream_t st) {
+  if (int rc = packed_check(num_seqs, total_q, total_k, heads, kv_heads, dim)) return rc;
+  VA_CHECK_ARG(training, "packed attention backward: the plan must be built for training");
+  VA_CHECK_ARG(scale > 0.0f && scale < INFINITY, "packed attention: the scale must be positive and finite");
+  VA_CHECK_ARG(strides && (total_q == 0 || (d_out && q && out && lse && dq)) && (total_k == 0 || (k && v && dk && dv)),
+               "packed attention backward: null pointer");
+  BwdArgs a{};
+  a.plan = static_cast<uint8_t*>(plan);
+  a.s = packed_shape(num_seqs, total_q, total_k, heads, kv_heads, dim, causal != 0, 1);
+  if (!plan || plan_bytes < a.s.total)
+    return set_error(VA_ERR_WORKSPACE, "packed attention backward: plan of %zu < %zu bytes", plan_bytes, a.s.total);
+  if (reinterpret_cast<uintptr_t>(plan) & 255)
+    return set_error(VA_ERR_ALIGN, "packed attention backward: the plan needs 256-byte alignment");
+  a.dq = dq, a.dk = dk, a.dv = dv, a.scale = scale;
+  a.dq_row = strides[8], a.dq_head = strides[9], a.dk_row = strides[10], a.dk_head = strides[11];
+  a.dv_row = strides[12], a.dv_head = strides[13];
+  for (int i = 8; i < 14; ++i)
+    if (strides[i] % 8) return set_error(VA_ERR_ALIGN, "packed attention backward: gradients need strides of 16 bytes");
+  if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) |
+       reinterpret_cast<uintptr_t>(out)) & 15)
+    return set_error(VA_ERR_ALIGN, "packed attention backward: out and the gradients need 16-byte alignment");
+  BwdMaps m;
+  // a side without rows is never read: its maps may be any valid ones
+  const void *mq = total_q ? q : k, *mo = total_q ? d_out : k, *mk = total_k ? k : q, *mv = total_k ? v : q;
+  if (total_q == 0 && total_k == 0) return VA_OK;
+  const int hq = total_q ? heads : kv_heads, hk = total_k ? kv_heads : heads;
+  const int nq = total_q ? total_q : total_k, nk = total_k ? total_k : total_q;
+  const int64_t* sq = total_q ? strides : strides + 2;
+  const int64_t* so = total_q ? strides + 6 : strides + 2;
+  const int64_t* sk = total_k ? strides + 2 : strides;
+  const int64_t* sv = total_k ? strides + 4 : strides;
+  for (int step = 0; step < 2; ++step) {
+    const int rows = step ? kHalf : kPackBlock;
+    if (int rc = packed_map(step ? &m.q_step : &m.q_tile, mq, BF16, nq, hq, dim, sq[0], sq[1], 1, rows, "q")) return rc;
+    if (int rc = packed_map(step ? &m.do_step : &m.do_tile, mo, BF16, nq, hq, dim, so[0], so[1], 1, rows, "grad_out"))
+      return rc;
+    if (int rc = packed_map(step ? &m.k_step : &m.k_tile, mk, BF16, nk, hk, dim, sk[0], sk[1], 1, rows, "k")) return rc;
+    if (int rc = packed_map(step ? &m.v_step : &m.v_tile, mv, BF16, nk, hk, dim, sv[0], sv[1], 1, rows, "v")) return rc;
+  }
+  const long long rows = (long long)total_q * heads + (BF16 ? 0 : (long long)total_k * kv_heads);
+  VA_CHECK_ARG((rows + 15) / 16 < (1LL << 31), "packed attention backward: too many rows");
+  if (rows > 0) {
+    packed_rows_kernel<BF16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(
+        static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(d_out), strides[6], strides[7],
+        static_cast<const uint16_t*>(v), strides[4], strides[5], lse, reinterpret_cast<float2*>(a.plan + a.s.rows),
+        reinterpret_cast<float*>(a.plan + a.s.do_norm), reinterpret_cast<float*>(a.plan + a.s.v_norm), total_q, total_k,
+        heads, kv_heads, dim);
+    if (int rc = check_launch("packed attention backward rows")) return rc;
+  }
+  return dim <= 64 ? launch_bwd<64, BF16>(m, a, st) : launch_bwd<128, BF16>(m, a, st);
+}
+
+}  // namespace
+
+int packed_bwd_status_read(int* out, cudaStream_t st) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(out, g_packed_bwd_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return set_error(VA_ERR_LAUNCH, "device status read: %s", cudaGetErrorString(e));
+  return VA_OK;
+}
+
+int packed_bwd_status_clear(cudaStream_t st) {
+  static const int zero = 0;
+  cudaError_t e = cudaMemcpyToSymbolAsync(g_packed_bwd_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+  if (e != cudaSuccess) return set_error(VA_ERR_LAUNCH, "device status clear: %s", cudaGetErrorString(e));
+  return VA_OK;
+}
+
+}  // namespace va
+
+using namespace va;
+
+#define VA_PACKED_BWD(sfx, T, BF)                                                                                    \
+  int va_packed_attention_bwd_##sfx(const T* grad_out, const T* q, const T* k, const T* v, const T* out,             \
+                                    const float* lse, T* grad_q, T* grad_k, T* grad_v, const int64_t* strides,       \
+                                    int num_seqs, int total_q, int total_k, int num_heads, int num_kv_heads,         \
+                                    int head_dim, int causal, int training, float softmax_scale, void* plan,         \
+                                    size_t plan_bytes, va_stream_t stream) {                                         \
+    return packed_bwd<BF>(grad_out, q, k, v, out, lse, grad_q, grad_k, grad_v, strides, num_seqs, total_q, total_k,  \
+                          num_heads, num_kv_heads, head_dim, causal, training, softmax_scale, plan, plan_bytes,      \
+                          (cudaStream_t)stream);                                                                     \
+  }
+
+extern "C" {
+VA_PACKED_BWD(bf16, va_bf16, true)
+VA_PACKED_BWD(f16, void, false)
+}  // extern "C"

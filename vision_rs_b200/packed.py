@@ -20,6 +20,7 @@ from .psa import _stream
 
 _SFX = {torch.bfloat16: "bf16", torch.float16: "f16"}
 _Strides6 = C.c_int64 * 6
+_Strides14 = C.c_int64 * 14
 
 
 def cu_seqlens(lengths, device="cuda") -> torch.Tensor:
@@ -101,3 +102,26 @@ def packed_attention_forward(q, k, v, plan: PackedPlan, scale: float | None = No
               lse.data_ptr(), st, *plan.sizes, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes,
               _stream(stream))
     return out, lse
+
+
+def packed_attention_backward(grad_out, q, k, v, out, lse, plan: PackedPlan, scale: float | None = None, grads=None,
+                              stream=None):
+    """``(grad_q, grad_k, grad_v)`` from the forward's inputs and results; the
+    plan must be built with ``training=True``.  ``grads``: three tensors to
+    write, which may be slices of one packed gradient."""
+    st = _inputs(q, k, v, plan)
+    _, tq, tk, h, hk, d, _, training = plan.sizes
+    if not training:
+        raise ValueError("the plan was not built with training=True")
+    _dense(out, "out", (tq, h, d), q.dtype, q.device)
+    _dense(lse, "lse", (h, tq), torch.float32, q.device)
+    so = _heads(grad_out, "grad_out", (tq, h, d), q)
+    if grads is None:
+        grads = tuple(torch.empty(s, dtype=q.dtype, device=q.device) for s in ((tq, h, d), (tk, hk, d), (tk, hk, d)))
+    gq, gk, gv = grads
+    sg = (*_heads(gq, "grad_q", (tq, h, d), q), *_heads(gk, "grad_k", (tk, hk, d), q),
+          *_heads(gv, "grad_v", (tk, hk, d), q))
+    _lib.call("va_packed_attention_bwd_" + _SFX[q.dtype], grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+              out.data_ptr(), lse.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _Strides14(*st, *so, *sg),
+              *plan.sizes, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes, _stream(stream))
+    return gq, gk, gv
