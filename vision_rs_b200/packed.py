@@ -12,13 +12,14 @@ layers.  No CPU path.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 
 import torch
 
-from . import _lib
-from .psa import _stream
+from . import _launch, _lib
 
-_SFX = {torch.bfloat16: "bf16", torch.float16: "f16"}
+_FWD = {torch.bfloat16: "va_packed_attention_fwd_bf16", torch.float16: "va_packed_attention_fwd_f16"}
+_BWD = {torch.bfloat16: "va_packed_attention_bwd_bf16", torch.float16: "va_packed_attention_bwd_f16"}
 _Strides6 = C.c_int64 * 6
 _Strides14 = C.c_int64 * 14
 
@@ -33,6 +34,15 @@ def cu_seqlens(lengths, device="cuda") -> torch.Tensor:
     return torch.tensor(off, dtype=torch.int32).to(device)
 
 
+@lru_cache(maxsize=256)
+def _plan_bytes(*sizes) -> int:
+    need = _lib.lib().va_packed_plan_bytes(*sizes)
+    if need == 0:
+        raise _lib.VisionAttnError("va_packed_plan_bytes", 1,
+                                   _lib.lib().va_get_last_error_string().decode(errors="replace"))
+    return need
+
+
 class PackedPlan:
     """Work lists of packed-sequence attention for one batch's sequences and
     one head layout (with the kernels' partial results: calls that share a
@@ -42,65 +52,77 @@ class PackedPlan:
 
     def __init__(self, cu_q, cu_k, total_q: int, total_k: int, num_heads: int, num_kv_heads: int, head_dim: int,
                  causal: bool = False, training: bool = False, stream=None):
-        for name, t in (("cu_q", cu_q), ("cu_k", cu_k)):
-            if not t.is_cuda or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < 2 or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous CUDA int32 [sequences + 1] tensor")
-        if cu_q.shape != cu_k.shape or cu_q.device != cu_k.device:
-            raise ValueError("cu_q and cu_k must have the same sequences and device")
-        self.sizes = (cu_q.shape[0] - 1, total_q, total_k, num_heads, num_kv_heads, head_dim, int(causal),
-                      int(training))
-        need = _lib.lib().va_packed_plan_bytes(*self.sizes)
-        if need == 0:
-            raise _lib.VisionAttnError("va_packed_plan_bytes", 1,
-                                       _lib.lib().va_get_last_error_string().decode(errors="replace"))
-        self.buf = torch.empty(need, dtype=torch.uint8, device=cu_q.device)
-        self.nbytes = need
-        _lib.call("va_packed_plan_build", cu_q.data_ptr(), cu_k.data_ptr(), *self.sizes, self.buf.data_ptr(), need,
-                  _stream(stream))
+        if stream is not None:
+            with _launch.on(stream):
+                return self.__init__(cu_q, cu_k, total_q, total_k, num_heads, num_kv_heads, head_dim, causal, training)
+        index = cu_q.get_device()
+        for t in (cu_q, cu_k):
+            if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != index or index < 0 \
+                    or not t.is_contiguous():
+                raise ValueError("cu_q and cu_k must be contiguous int32 [sequences + 1] tensors of one CUDA device")
+        n = cu_q.shape[0] - 1
+        if n < 1 or cu_k.shape[0] != n + 1:
+            raise ValueError("cu_q and cu_k must have the same sequences, one at least")
+        self.sizes = sizes = (n, total_q, total_k, num_heads, num_kv_heads, head_dim, int(causal), int(training))
+        self.nbytes = need = _plan_bytes(*sizes)
+        self.index = index
+        self.buf = cu_q.new_empty(need, dtype=torch.uint8)
+        self.ptr = self.buf.data_ptr()
+        self.stream = _launch.raw_stream(index)
+        _launch.run("va_packed_plan_build", index, cu_q.data_ptr(), cu_k.data_ptr(), *sizes, self.ptr, need)
 
     def check(self, stream=None):
         """Raises if the offsets were out of order or range (synchronises)."""
+        if stream is not None:
+            with _launch.on(stream):
+                return self.check()
         bad = C.c_int(0)
-        _lib.call("va_packed_plan_status", self.buf.data_ptr(), self.sizes[7], C.byref(bad), _stream(stream))
+        _launch.run("va_packed_plan_status", self.index, self.ptr, self.sizes[7], C.byref(bad))
         if bad.value:
             raise ValueError("cu_q or cu_k are not ascending offsets from 0 to the number of tokens")
 
+    def _use(self):
+        """The buffer must outlive a call on another stream than the plan's own."""
+        if _launch.raw_stream(self.index) != self.stream:
+            self.buf.record_stream(torch.cuda.current_stream(self.index))
 
-def _heads(t, name, shape, like):
-    if not t.is_cuda or t.dtype not in _SFX or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be a CUDA bf16 or f16 tensor of q's type and device")
+
+def _heads(t, name, dtype, index, shape):
+    if t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be a CUDA tensor of q's type on the plan's device")
     if t.shape != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-    if t.stride(2) != 1:
+    row, head, one = t.stride()
+    if one != 1:
         raise ValueError(f"{name}: a head's dimensions must be contiguous")
-    return t.stride(0), t.stride(1)
+    return row, head
 
 
-def _dense(t, name, shape, dtype, device):
-    if not t.is_cuda or t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
+def _dense(t, name, shape, dtype, index):
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous CUDA {dtype} tensor of {shape}")
     return t
-
-
-def _inputs(q, k, v, plan):
-    _, tq, tk, h, hk, d, _, _ = plan.sizes
-    if plan.buf.device != q.device:
-        raise ValueError("the plan is on another device")
-    return _Strides6(*_heads(q, "q", (tq, h, d), q), *_heads(k, "k", (tk, hk, d), q), *_heads(v, "v", (tk, hk, d), q))
 
 
 def packed_attention_forward(q, k, v, plan: PackedPlan, scale: float | None = None, out=None, lse=None, stream=None):
     """``(out [total_q, heads, dim], lse f32 [heads, total_q])``; ``scale``
     defaults to dim^-½.  A query that sees no key has out 0 and lse −∞."""
-    st = _inputs(q, k, v, plan)
-    _, tq, _, h, _, d, _, _ = plan.sizes
-    out = torch.empty((tq, h, d), dtype=q.dtype, device=q.device) if out is None else \
-        _dense(out, "out", (tq, h, d), q.dtype, q.device)
-    lse = torch.empty((h, tq), dtype=torch.float32, device=q.device) if lse is None else \
-        _dense(lse, "lse", (h, tq), torch.float32, q.device)
-    _lib.call("va_packed_attention_fwd_" + _SFX[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-              lse.data_ptr(), st, *plan.sizes, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes,
-              _stream(stream))
+    if stream is not None:
+        with _launch.on(stream):
+            return packed_attention_forward(q, k, v, plan, scale, out, lse)
+    sizes, index, dtype = plan.sizes, plan.index, q.dtype
+    name = _FWD.get(dtype)
+    if name is None:
+        raise ValueError("q must be bf16 or f16")
+    _, tq, tk, h, hk, d, _, _ = sizes
+    sq, sk = (tq, h, d), (tk, hk, d)
+    strides = _Strides6(*_heads(q, "q", dtype, index, sq), *_heads(k, "k", dtype, index, sk),
+                        *_heads(v, "v", dtype, index, sk))
+    out = q.new_empty(sq) if out is None else _dense(out, "out", sq, dtype, index)
+    lse = q.new_empty((h, tq), dtype=torch.float32) if lse is None else _dense(lse, "lse", (h, tq), torch.float32, index)
+    plan._use()
+    _launch.run(name, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), strides, *sizes,
+                d ** -0.5 if scale is None else scale, plan.ptr, plan.nbytes)
     return out, lse
 
 
@@ -109,19 +131,26 @@ def packed_attention_backward(grad_out, q, k, v, out, lse, plan: PackedPlan, sca
     """``(grad_q, grad_k, grad_v)`` from the forward's inputs and results; the
     plan must be built with ``training=True``.  ``grads``: three tensors to
     write, which may be slices of one packed gradient."""
-    st = _inputs(q, k, v, plan)
-    _, tq, tk, h, hk, d, _, training = plan.sizes
+    if stream is not None:
+        with _launch.on(stream):
+            return packed_attention_backward(grad_out, q, k, v, out, lse, plan, scale, grads)
+    sizes, index, dtype = plan.sizes, plan.index, q.dtype
+    name = _BWD.get(dtype)
+    if name is None:
+        raise ValueError("q must be bf16 or f16")
+    _, tq, tk, h, hk, d, _, training = sizes
     if not training:
         raise ValueError("the plan was not built with training=True")
-    _dense(out, "out", (tq, h, d), q.dtype, q.device)
-    _dense(lse, "lse", (h, tq), torch.float32, q.device)
-    so = _heads(grad_out, "grad_out", (tq, h, d), q)
-    if grads is None:
-        grads = tuple(torch.empty(s, dtype=q.dtype, device=q.device) for s in ((tq, h, d), (tk, hk, d), (tk, hk, d)))
-    gq, gk, gv = grads
-    sg = (*_heads(gq, "grad_q", (tq, h, d), q), *_heads(gk, "grad_k", (tk, hk, d), q),
-          *_heads(gv, "grad_v", (tk, hk, d), q))
-    _lib.call("va_packed_attention_bwd_" + _SFX[q.dtype], grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-              out.data_ptr(), lse.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _Strides14(*st, *so, *sg),
-              *plan.sizes, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes, _stream(stream))
+    sq, sk = (tq, h, d), (tk, hk, d)
+    _dense(out, "out", sq, dtype, index)
+    _dense(lse, "lse", (h, tq), torch.float32, index)
+    gq, gk, gv = (q.new_empty(sq), k.new_empty(sk), v.new_empty(sk)) if grads is None else grads
+    strides = _Strides14(*_heads(q, "q", dtype, index, sq), *_heads(k, "k", dtype, index, sk),
+                         *_heads(v, "v", dtype, index, sk), *_heads(grad_out, "grad_out", dtype, index, sq),
+                         *_heads(gq, "grad_q", dtype, index, sq), *_heads(gk, "grad_k", dtype, index, sk),
+                         *_heads(gv, "grad_v", dtype, index, sk))
+    plan._use()
+    _launch.run(name, index, grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                lse.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), strides, *sizes,
+                d ** -0.5 if scale is None else scale, plan.ptr, plan.nbytes)
     return gq, gk, gv

@@ -9,74 +9,96 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
-from .psa import _stream
+from . import _launch
 
 _SFX = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+_FWD, _F8, _BWD = ({t: f"va_rms_norm_{kind}_{s}" for t, s in _SFX.items()} for kind in ("fwd", "fwd_f8", "bwd"))
 
 
-def _check(t, name, like=None):
-    if not t.is_cuda or t.dtype not in _SFX or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous CUDA tensor of bf16, f16 or f32")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} must have the shape, type and device of the other rows")
+def _rows(t):
+    """(device index, rows, cols) of the tensor that the others are held to."""
+    index = t.get_device()
+    if index < 0 or t.dtype not in _SFX or not t.is_contiguous() or t.dim() == 0:
+        raise ValueError("rows must be contiguous CUDA tensors of bf16, f16 or f32")
+    cols = t.shape[-1]
+    return index, (t.numel() // cols if cols else 0), cols
+
+
+def _same(t, name, like, index):
+    if t.dtype is not like.dtype or t.get_device() != index or t.shape != like.shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, with the shape, type and device of the other rows")
     return t.data_ptr()
 
 
-def _weight(w, x):
-    if not w.is_cuda or w.device != x.device or w.dtype not in (x.dtype, torch.float32) or not w.is_contiguous() \
-            or x.dim() == 0 or w.shape != x.shape[-1:]:
+def _weight(w, x, index, cols):
+    f32 = w.dtype is torch.float32
+    if not (f32 or w.dtype is x.dtype) or w.get_device() != index or w.shape != (cols,) or not w.is_contiguous():
         raise ValueError("w must be a contiguous CUDA [cols] tensor of the rows' type or f32")
-    return w.data_ptr(), int(w.dtype == torch.float32)
+    return w.data_ptr(), f32
 
 
-def _sizes(x):
-    cols = x.shape[-1]
-    return (x.numel() // cols if cols else 0), cols
+def _sum(x, residual, out_h, index):
+    """Addresses of the residual and of the tensor for the sum, and that tensor (x itself without either)."""
+    pr = None if residual is None else _same(residual, "residual", x, index)
+    if out_h is not None:
+        return pr, _same(out_h, "out_h", x, index), out_h
+    if residual is None:
+        return None, None, x
+    h = torch.empty_like(x)
+    return pr, h.data_ptr(), h
 
 
 def rms_norm_forward(x, w, residual=None, eps: float = 1e-6, out=None, out_h=None, stream=None):
     """``(y, h)``; without a residual ``h`` is ``x`` itself.  ``out_h`` may be
     ``x`` or ``residual`` (the sum is then updated in place)."""
-    px, (pw, w32) = _check(x, "x"), _weight(w, x)
-    pr = None if residual is None else _check(residual, "residual", x)
+    if stream is not None:
+        with _launch.on(stream):
+            return rms_norm_forward(x, w, residual, eps, out, out_h)
+    index, rows, cols = _rows(x)
+    pw, w32 = _weight(w, x, index, cols)
+    pr, ph, h = _sum(x, residual, out_h, index)
     y = torch.empty_like(x) if out is None else out
-    h = out_h if out_h is not None else None if residual is None else torch.empty_like(x)
-    rows, cols = _sizes(x)
-    _lib.call("va_rms_norm_fwd_" + _SFX[x.dtype], px, pr, pw, w32, None if h is None else _check(h, "out_h", x),
-              _check(y, "out", x), rows, cols, eps, _stream(stream))
-    return y, x if h is None else h
+    _launch.run(_FWD[x.dtype], index, x.data_ptr(), pr, pw, w32, ph,
+                y.data_ptr() if out is None else _same(out, "out", x, index), rows, cols, eps)
+    return y, h
 
 
 def rms_norm_forward_f8(x, w, residual=None, eps: float = 1e-6, group: int = 0, out_h=None, stream=None):
     """``(q, scale, h)``: ``q`` float8_e4m3fn of x's shape and ``scale`` f32
     ``[..., cols/group]`` (``group`` 0: one for each row) with
     ``y ≈ q · scale`` and the largest magnitude of each group at 448."""
-    px, (pw, w32) = _check(x, "x"), _weight(w, x)
-    pr = None if residual is None else _check(residual, "residual", x)
-    h = out_h if out_h is not None else None if residual is None else torch.empty_like(x)
-    rows, cols = _sizes(x)
+    if stream is not None:
+        with _launch.on(stream):
+            return rms_norm_forward_f8(x, w, residual, eps, group, out_h)
+    index, rows, cols = _rows(x)
     if group < 0 or (group and cols % group):
         raise ValueError(f"{cols} columns do not split into groups of {group}")
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(*x.shape[:-1], cols // group if group else 1, dtype=torch.float32, device=x.device)
-    _lib.call("va_rms_norm_fwd_f8_" + _SFX[x.dtype], px, pr, pw, w32, None if h is None else _check(h, "out_h", x),
-              q.data_ptr(), scale.data_ptr(), rows, cols, group, eps, _stream(stream))
-    return q, scale, x if h is None else h
+    pw, w32 = _weight(w, x, index, cols)
+    pr, ph, h = _sum(x, residual, out_h, index)
+    shape = x.shape
+    q = x.new_empty(shape, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(shape[:-1] + (cols // group if group else 1,), dtype=torch.float32)
+    _launch.run(_F8[x.dtype], index, x.data_ptr(), pr, pw, w32, ph, q.data_ptr(), scale.data_ptr(), rows, cols, group,
+                eps)
+    return q, scale, h
 
 
 def rms_norm_backward(grad_y, h, w, eps: float = 1e-6, grad_h=None, workspace=None, stream=None):
     """``(grad, grad_w)``: the gradient of ``x`` and of ``residual`` alike
     (with ``grad_h``, the gradient that reaches ``h`` itself, added), and
     f32 ``[cols]`` of the weight.  ``h`` is the sum that the forward returned."""
-    ph, (pw, w32) = _check(h, "h"), _weight(w, h)
-    pg = None if grad_h is None else _check(grad_h, "grad_h", h)
-    rows, cols = _sizes(h)
-    need = int(_lib.lib().va_rms_norm_bwd_workspace_bytes(rows, cols))
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=h.device)
+    if stream is not None:
+        with _launch.on(stream):
+            return rms_norm_backward(grad_y, h, w, eps, grad_h, workspace)
+    index, rows, cols = _rows(h)
+    pw, w32 = _weight(w, h, index, cols)
+    py = _same(grad_y, "grad_y", h, index)
+    pg = None if grad_h is None else _same(grad_h, "grad_h", h, index)
+    need = _launch.entry("va_rms_norm_bwd_workspace_bytes")(rows, cols)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = h.new_empty(need, dtype=torch.uint8)
     grad = torch.empty_like(h)
-    grad_w = torch.empty(cols, dtype=torch.float32, device=h.device)
-    _lib.call("va_rms_norm_bwd_" + _SFX[h.dtype], _check(grad_y, "grad_y", h), ph, pw, w32, pg, grad.data_ptr(),
-              grad_w.data_ptr(), rows, cols, eps, workspace.data_ptr(), workspace.numel(), _stream(stream))
+    grad_w = h.new_empty(cols, dtype=torch.float32)
+    _launch.run(_BWD[h.dtype], index, py, h.data_ptr(), pw, w32, pg, grad.data_ptr(), grad_w.data_ptr(), rows, cols,
+                eps, workspace.data_ptr(), need)
     return grad, grad_w

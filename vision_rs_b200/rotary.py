@@ -13,10 +13,10 @@ import math
 
 import torch
 
-from . import _lib
-from .psa import _stream
+from . import _launch
 
-_SFX = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+_ENTRY = {torch.bfloat16: "va_rotary_bf16", torch.float16: "va_rotary_f16", torch.float32: "va_rotary_f32"}
+_POSITION = {torch.int32: 4, torch.int64: 8}  # bytes
 _Strides = C.c_int64 * 8
 
 
@@ -45,41 +45,61 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, stretch: float = 1.0
     return inv.to(device)
 
 
-def _heads(t, name, ref=None):
-    if not t.is_cuda or t.dim() != 3 or t.dtype not in _SFX:
-        raise ValueError(f"{name} must be a CUDA [tokens, heads, head_dim] tensor of bf16, f16 or f32")
+def _heads(t, name, dtype, index):
+    if t.dtype is not dtype or t.get_device() != index or t.dim() != 3:
+        raise ValueError(f"{name} must be a CUDA [tokens, heads, head_dim] tensor of q's type and device")
     if t.stride(2) != 1 and t.shape[2] > 1:
         raise ValueError(f"{name}: a head's dimensions must be contiguous")
-    if ref is not None and (t.dtype != ref.dtype or t.device != ref.device):
-        raise ValueError(f"{name} must have q's type and device")
-    return t
 
 
 def _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, stream):
-    _heads(q, "q")
-    tokens, hq, dim = q.shape
-    if k is not None and (_heads(k, "k", q).shape[0] != tokens or k.shape[2] != dim):
-        raise ValueError("q and k must have the same tokens and head_dim")
-    if not positions.is_cuda or positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
+    if stream is not None:
+        with _launch.on(stream):
+            return _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, None)
+    dtype, index = q.dtype, q.get_device()
+    name = _ENTRY.get(dtype)
+    if name is None or index < 0:
+        raise ValueError("q must be a CUDA tensor of bf16, f16 or f32")
+    _heads(q, "q", dtype, index)
+    tokens, hq, dim = shape = q.shape
+    hk = 0
+    if k is not None:
+        _heads(k, "k", dtype, index)
+        tk, hk, dk = k.shape
+        if tk != tokens or dk != dim:
+            raise ValueError("q and k must have the same tokens and head_dim")
+    if positions.get_device() != index or positions.dtype not in _POSITION or positions.shape != (tokens,) \
             or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous CUDA int32 or int64 [tokens] tensor")
-    if not inv_freq.is_cuda or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    if inv_freq.get_device() != index or inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 \
+            or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous CUDA float64 [rot_dim/2] tensor")
-    if 2 * inv_freq.shape[0] > dim:
-        raise ValueError(f"{2 * inv_freq.shape[0]} rotated dimensions in heads of {dim}")
+    rot = 2 * inv_freq.shape[0]
+    if rot > dim:
+        raise ValueError(f"{rot} rotated dimensions in heads of {dim}")
     if out is None:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        qo = q.new_empty(shape)
+        ko = None if k is None else k.new_empty(k.shape)
     else:
         qo, ko = out
-        if _heads(qo, "q output", q).shape != q.shape or (k is None) != (ko is None) or \
-                (k is not None and _heads(ko, "k output", q).shape != k.shape):
+        if (k is None) != (ko is None):
             raise ValueError("outputs must have the inputs' shapes")
-    st = (q.stride(), (0, 0) if k is None else k.stride(), qo.stride(), (0, 0) if k is None else ko.stride())
-    _lib.call("va_rotary_" + _SFX[q.dtype], q.data_ptr(), None if k is None else k.data_ptr(), qo.data_ptr(),
-              None if k is None else ko.data_ptr(), _Strides(*(s for x in st for s in x[:2])), positions.data_ptr(),
-              positions.element_size(), inv_freq.data_ptr(), tokens, hq, 0 if k is None else k.shape[1], dim,
-              2 * inv_freq.shape[0], bool(interleaved), backward, factor, _stream(stream))
+        for o, x in ((qo, q), (ko, k)):
+            if o is not None:
+                _heads(o, "an output", dtype, index)
+                if o.shape != x.shape:
+                    raise ValueError("outputs must have the inputs' shapes")
+    a, b, _ = q.stride()
+    e, f, _ = qo.stride()
+    if k is None:
+        strides, pk, pko = _Strides(a, b, 0, 0, e, f, 0, 0), None, None
+    else:
+        c, d, _ = k.stride()
+        g, h, _ = ko.stride()
+        strides, pk, pko = _Strides(a, b, c, d, e, f, g, h), k.data_ptr(), ko.data_ptr()
+    _launch.run(name, index, q.data_ptr(), pk, qo.data_ptr(), pko, strides, positions.data_ptr(),
+                _POSITION[positions.dtype], inv_freq.data_ptr(), tokens, hq, hk, dim, rot, int(interleaved), backward,
+                factor)
     return qo, ko
 
 
