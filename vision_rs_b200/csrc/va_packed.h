@@ -29,12 +29,15 @@ struct alignas(16) QItem {
   int counter;      // the tile's arrival counter
   int pad;
 };
-// One unit of dK/dV work: up to 128 keys of one sequence against its query blocks [qb0, qb1).
+// One unit of dK/dV work: up to 128 keys of one sequence and key head against
+// steps [h0, h1) of those that see them: step h is 64 queries of head h / nh of
+// the group, nh steps a head from the first that sees a key of the unit on.
 struct alignas(16) KItem {
   int k0, keys;     // first key (row of the packed tensor) and their number
   int j0;           // its index in the sequence
   int q0, lq, lk;   // the sequence's first query (row) and lengths
-  int qb0, qb1;
+  int h0, h1;
+  int slot, slot0, parts, counter;  // as a QItem's
 };
 
 // Sizes that host and device agree on, from the call's sizes alone.
@@ -48,9 +51,10 @@ struct PackedShape {
   int q_tile;       // queries a forward unit
   int units;        // heads (or key heads) that each forward unit is run for
   int max_tiles, max_items, max_slots, split_budget;
-  int max_dq_items, max_dkv_items;
+  int max_dq_items, max_dkv_tiles, max_dkv_items, dkv_budget;
   // byte offsets in the plan
-  size_t items, dq_items, dkv_items, counters, scratch, part_o, part_lse, rows, do_norm, v_norm, total;
+  size_t items, dq_items, dkv_items, counters, dkv_counters, scratch, part_o, part_lse, part_dkv, rows, do_norm,
+      v_norm, total;
 };
 
 // Header words of the plan, one of each for the three lists: the number of
@@ -76,15 +80,19 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   s.max_items = s.max_tiles + s.split_budget;
   s.max_slots = 2 * s.split_budget;
   s.max_dq_items = training ? (int)std::min<long long>((total_q + 127) / 128 + (long long)num_seqs, total_q) : 0;
-  s.max_dkv_items = training ? (int)std::min<long long>((total_k + 127) / 128 + (long long)num_seqs, total_k) : 0;
+  s.max_dkv_tiles = training ? (int)std::min<long long>((total_k + 127) / 128 + (long long)num_seqs, total_k) : 0;
+  s.dkv_budget = training ? (296 + kv_heads - 1) / kv_heads : 0;
+  s.max_dkv_items = s.max_dkv_tiles + s.dkv_budget;
   size_t o = 256;
   s.items = o, o += pk_align((size_t)s.max_items * sizeof(QItem));
   s.dq_items = o, o += pk_align((size_t)s.max_dq_items * sizeof(QItem));
   s.dkv_items = o, o += pk_align((size_t)s.max_dkv_items * sizeof(KItem));
   s.counters = o, o += pk_align(s.few ? (size_t)s.max_tiles * s.units * 4 : 0);
+  s.dkv_counters = o, o += pk_align((size_t)s.max_dkv_tiles * kv_heads * 4);
   s.scratch = o, o += pk_align(num_seqs > kPlanSeqs ? (size_t)3 * (num_seqs + 1) * 4 : 0);
   s.part_o = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * dim * 4);
   s.part_lse = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * 4);
+  s.part_dkv = o, o += pk_align((size_t)2 * s.dkv_budget * kv_heads * 2 * kPackBlock * dim * 4);
   // training: (lse·log2 e, Δ) a query and head, ‖dO_i‖ and ‖V_j‖ (the f16 backward's)
   s.rows = o, o += pk_align(training ? (size_t)total_q * heads * 8 : 0);
   s.do_norm = o, o += pk_align(training ? (size_t)total_q * heads * 4 : 0);

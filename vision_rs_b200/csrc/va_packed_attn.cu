@@ -14,8 +14,8 @@
 //     the query heads of a key head read its keys once, over a part of the
 //     keys; two CTAs an SM.  The last CTA of a tile's parts to arrive joins
 //     them in the parts' order (single tokens, few queries).
-// Warps: 4 a tile for the softmax (a thread owns a row), 1 TMA producer, 1
-// MMA issuer.  Per 128-key step: S = Q·Kᵀ into TMEM, the row's p = 2^(s −
+// Warps: 4 a tile for the softmax (a thread owns a row), 1 a tile to issue
+// its MMAs, 1 TMA producer.  Per 128-key step: S = Q·Kᵀ into TMEM, the row's p = 2^(s −
 // reference) back into the same columns as 16-bit P, O += P·V with P as the
 // TMEM operand.  The reference only follows the row maximum when it grows by
 // more than 2^8, so O is rarely rescaled.  P is held in the inputs' 16-bit
@@ -41,6 +41,7 @@ __device__ int g_packed_status;
 
 namespace {
 
+constexpr int kHalf = 64;  // keys of a score step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.0f;  // the reference follows the maximum once it is 2^8 ahead
 constexpr float kF16Shift = 7.0f;   // f16: P is held times 2^7 (at most 2^15), so small ones keep their bits
@@ -49,10 +50,10 @@ constexpr float kF16Shift = 7.0f;   // f16: P is held times 2^7 (at most 2^15), 
 template <int DP, int TILES> struct FwdCfg {
   static constexpr int kSlotBytes = kPackBlock * DP * 2;
   static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 5);
-  static constexpr int kThreads = TILES * 128 + 64;
+  static constexpr int kThreads = TILES * 160 + 32;
   static constexpr int kCtas = TILES == 2 ? 1 : 2;  // an SM
   static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
-  static constexpr uint32_t kColS = 0, kColO = TILES * 128;  // S_m at 128·m, O_m at kColO + DP·m
+  static constexpr uint32_t kColS = 0, kColO = TILES * 128;  // tile m: scores at 128·m and 128·m + 64, O at kColO + DP·m
 };
 
 template <int DP, int TILES> struct FwdSmem {
@@ -60,7 +61,7 @@ template <int DP, int TILES> struct FwdSmem {
   uint8_t q[TILES][C::kSlotBytes];      // per 64 dims: 128 rows × 128 bytes, SW128
   uint8_t kv[C::kSlots][C::kSlotBytes];
   uint64_t q_full, kv_full[C::kSlots], kv_empty[C::kSlots];
-  uint64_t s_full[TILES], p_full[TILES], o_done[TILES], fin;
+  uint64_t s_full[TILES][2], p_full[TILES][2], o_done[TILES][2], v_ready, fin;
   uint32_t tmem_base;
   int abort;
   int last;
@@ -95,32 +96,34 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const int group = ps.few ? ps.group : 1;        // rows of a query in a tile
   const int kv_head = ps.few ? head : head / ps.group;
   const int rows = it.tokens * group;
-  // key blocks of each tile: a causal first tile ends before the second
-  int kb_end[TILES], see_end = 0;  // see_end: one past the last key that any row of the unit sees
+  // 64-key steps of each tile (a causal first tile ends before the second) and one past the last key that any row sees
+  int steps[TILES], see_end = 0;
 #pragma unroll
   for (int m = 0; m < TILES; ++m) {
     const int n = TILES == 2 ? min(kPackBlock, it.tokens - m * kPackBlock) : it.tokens;
     int end = 0;
     if (n > 0) end = ps.causal ? min(it.lk, max(0, it.see + m * kPackBlock + n)) : it.lk;
-    kb_end[m] = max(it.kb0, min(it.kb1, (end + kPackBlock - 1) / kPackBlock));
+    steps[m] = max(0, min(2 * it.kb1, (end + kHalf - 1) / kHalf) - 2 * it.kb0);
     see_end = max(see_end, end);
   }
-  const int kb_all = TILES == 2 ? max(kb_end[0], kb_end[TILES - 1]) : kb_end[0];
-  const int nkb = kb_all - it.kb0;
+  const int all_steps = max(steps[0], steps[TILES - 1]), nkb = (all_steps + 1) >> 1;
   const int dim16 = (ps.dim + 15) & ~15;
 
   if (tid == 0) {
     mbar_init(&sm.q_full, 1);
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&sm.kv_full[i], 1);
-      mbar_init(&sm.kv_empty[i], 1);
+      mbar_init(&sm.kv_empty[i], TILES);
     }
     for (int m = 0; m < TILES; ++m) {
-      mbar_init(&sm.s_full[m], 1);
-      mbar_init(&sm.p_full[m], 128);
-      mbar_init(&sm.o_done[m], 1);
+      for (int r = 0; r < 2; ++r) {
+        mbar_init(&sm.s_full[m][r], 1);
+        mbar_init(&sm.p_full[m][r], 128);
+        mbar_init(&sm.o_done[m][r], 1);
+      }
     }
-    mbar_init(&sm.fin, 1);
+    mbar_init(&sm.v_ready, 1);
+    mbar_init(&sm.fin, TILES);
     sm.abort = 0;
     fence_mbar_init();
   }
@@ -168,70 +171,116 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
     }
     __syncwarp();
-  } else if (warp == TILES * 4 + 1) {
-    // ── MMA issuer (converged warp, one elected lane issues) ──
+    // V rows past the last key that the unit sees, up to the 16-key group that the MMAs stop at: zeros
+    const int used = see_end - (it.kb0 + nkb - 1) * kPackBlock, g = 2 * nkb - 1, sv = g % C::kSlots;
+    if (nkb > 0 && (used & 15) && used < kPackBlock &&
+        mbar_wait(&sm.kv_full[sv], (g / C::kSlots) & 1, &sm.abort, &g_packed_status, 4)) {
+      for (int i = lane; i < ((used + 15) / 16 * 16 - used) * (DP / 8); i += 32) {
+        const int row = used + i / (DP / 8), c = i % (DP / 8);
+        *reinterpret_cast<uint4*>(sm.kv[sv] + (c >> 3) * kPackBlock * 128 + sw128_off(row, c & 7)) =
+            make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.v_ready);
+    }
+    __syncwarp();
+  } else if (warp > TILES * 4) {
+    // ── MMA issuer of tile m: a converged warp whose values are uniform (the instructions between two MMAs are on
+    // the critical path; operands that differ between lanes cost ~60 cycles an MMA), one elected lane issues ──
+    const int m = TILES == 2 ? __shfl_sync(0xffffffffu, warp - TILES * 4 - 1, 0) : 0;
     if (nkb > 0) {
+      auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+      const uint32_t lead = elect_lead(), tm = uniform(tmem);
+      const int n = uniform(steps[TILES == 2 ? m : 0]), all = uniform(all_steps), end = uniform(see_end - 2 * it.kb0 * kHalf);
       const uint32_t fmt = BF16 ? AB_BF16 : AB_F16;
       auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
         return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &sm.abort, &g_packed_status, where));
       };
+      constexpr int kBlk = (kPackBlock * 128) >> 4;              // 64 dims further, in descriptor units
+      constexpr int kHalfRows = (kHalf * 128) >> 4, kSlot = C::kSlotBytes >> 4;
       const uint32_t idesc_o = idesc_f32acc(kPackBlock, dim16, fmt, false, true);
-      // keys of block kb that some row of the unit sees, as the MMAs' extent
-      auto keys16 = [&](int kb) { return (min(kPackBlock, see_end - kb * kPackBlock) + 15) & ~15; };
-      auto issue_s = [&](int m, int st, int kb) {
-        const uint32_t idesc = idesc_f32acc(kPackBlock, keys16(kb), fmt, false, false);
-        const uint64_t dq = sdesc(smem_u32(sm.q[m]), 16, 1024, SW_128B), dk = sdesc(smem_u32(sm.kv[st]), 16, 1024, SW_128B);
-        for (int s = 0; s < dim16 / 16; ++s) {
-          const uint64_t off = (uint64_t)((s >> 2) * ((kPackBlock * 128) >> 4) + (s & 3) * 2);
-          mma_ss_w(tmem + C::kColS + m * 128, dq + off, dk + off, idesc, s > 0 ? 1u : 0u);
+      const uint32_t idesc_s = idesc_f32acc(kPackBlock, kHalf, fmt, false, false);
+      const uint64_t dq = sdesc(smem_u32(sm.q[m]), 16, 1024, SW_128B);
+      const uint64_t dk0 = sdesc(smem_u32(sm.kv[0]), 16, 1024, SW_128B);
+      const uint64_t dv0 = sdesc(smem_u32(sm.kv[0]), kPackBlock * 128, 1024, SW_128B);
+      const uint32_t ts = tm + C::kColS + m * 128, to = tm + C::kColO + m * DP;
+      // S of step h (64 keys of K block h / 2, in slot st) into buffer h mod 2
+      auto issue_s = [&](int h, int st) {
+        const int left = end - h * kHalf;  // keys that some row sees, as the MMAs' extent
+        const uint32_t idesc =
+            left >= kHalf ? idesc_s : idesc_f32acc(kPackBlock, (left + 15) & ~15, fmt, false, false);
+        const uint64_t dk = dk0 + (uint64_t)(st * kSlot + (h & 1) * kHalfRows);
+        const uint32_t d = ts + (h & 1) * kHalf;
+        if (dim16 == DP) {
+#pragma unroll
+          for (int s = 0; s < DP / 16; ++s) {
+            const uint64_t off = (uint64_t)((s >> 2) * kBlk + (s & 3) * 2);
+            mma_ss_p(d, dq + off, dk + off, idesc, s > 0 ? 1u : 0u, lead);
+          }
+        } else {
+          for (int s = 0; s < dim16 / 16; ++s) {
+            const uint64_t off = (uint64_t)((s >> 2) * kBlk + (s & 3) * 2);
+            mma_ss_p(d, dq + off, dk + off, idesc, s > 0 ? 1u : 0u, lead);
+          }
         }
-        mma_commit_w(&sm.s_full[m]);
+        mma_commit_p(&sm.s_full[m][h & 1], lead);
+      };
+      // Both tiles' threads wait for every K and V slot and release it, also where their own tile has no step left.
+      int sk = 0, sv = 1;          // ring slots of the K block ahead and of this step's V block, and their parities
+      uint32_t pk = 0, pv = 0;
+      auto ahead = [&](int& slot, uint32_t& par) {
+        slot += 2;
+        if (slot >= C::kSlots) slot -= C::kSlots, par ^= 1;
       };
       bool ok = wait(&sm.q_full, 0, 2) && wait(&sm.kv_full[0], 0, 3);
       tc_fence_after();
       if (ok) {
-        for (int m = 0; m < TILES; ++m)
-          if (it.kb0 < kb_end[m]) issue_s(m, 0, it.kb0);
-        mma_commit_w(&sm.kv_empty[0]);
+        for (int h = 0; h < min(2, n); ++h) issue_s(h, 0);
+        mma_commit_p(&sm.kv_empty[0], lead);
+        ahead(sk, pk);
       }
-      for (int j = 0; ok && j < nkb; ++j) {
-        const int kb = it.kb0 + j, gv = 2 * j + 1, gk = 2 * j + 2;
-        const int sv = gv % C::kSlots, sk = gk % C::kSlots;
-        if (!(ok = wait(&sm.kv_full[sv], (gv / C::kSlots) & 1, 4))) break;
-        const int used = min(kPackBlock, see_end - kb * kPackBlock), steps = (used + 15) >> 4;
-        if (used & 15) {  // V rows past the last key in its 16-key group: zeros
-          for (int i = lane; i < ((used + 15) / 16 * 16 - used) * (DP / 8); i += 32) {
-            const int r = used + i / (DP / 8), c = i % (DP / 8);
-            *reinterpret_cast<uint4*>(sm.kv[sv] + (c >> 3) * kPackBlock * 128 + sw128_off(r, c & 7)) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
+      const int last_j = (all - 1) >> 1, used_last = end - last_j * kPackBlock;  // keys of the last block
+      for (int h = 0; ok && h < all; ++h) {
+        const int r = h & 1, g = h + 2;  // g: the step whose scores take this one's buffer
+        const bool last = (h >> 1) == last_j;
+        if (r == 0) {
+          if (!(ok = wait(&sm.kv_full[sv], pv, 4))) break;
+          if (last && (used_last & 15) && used_last < kPackBlock && !(ok = wait(&sm.v_ready, 0, 11))) break;
         }
-        const uint64_t dv = sdesc(smem_u32(sm.kv[sv]), kPackBlock * 128, 1024, SW_128B);
-        bool have_k = false;
-        for (int m = 0; m < TILES; ++m) {
-          if (kb >= kb_end[m]) continue;
-          if (!(ok = wait(&sm.p_full[m], j & 1, 5))) break;
+        if (h < n) {
+          if (!(ok = wait(&sm.p_full[m][r], (h >> 1) & 1, 5))) break;
           tc_fence_after();
-          for (int s = 0; s < steps; ++s)
-            mma_ts_w(tmem + C::kColO + m * DP, tmem + C::kColS + m * 128 + s * 8, dv + (uint64_t)(s * (2048 >> 4)),
-                     idesc_o, (j > 0 || s > 0) ? 1u : 0u);
-          mma_commit_w(&sm.o_done[m]);
-          if (kb + 1 < kb_end[m]) {
-            if (!have_k && !(ok = wait(&sm.kv_full[sk], (gk / C::kSlots) & 1, 6))) break;
-            have_k = true;
-            // the next scores overwrite P's columns: P·V has to be done with them
-            if (!(ok = wait(&sm.o_done[m], j & 1, 7))) break;
-            tc_fence_after();
-            issue_s(m, sk, kb + 1);
+          const uint64_t dv = dv0 + (uint64_t)(sv * kSlot + r * kHalfRows);
+          const uint32_t tp = ts + r * kHalf;
+          const int ks = last ? min(kHalf / 16, (used_last - r * kHalf + 15) >> 4) : kHalf / 16;
+          if (ks == kHalf / 16) {
+#pragma unroll
+            for (int s = 0; s < kHalf / 16; ++s)
+              mma_ts_p(to, tp + s * 8, dv + (uint64_t)(s * (2048 >> 4)), idesc_o, (h > 0 || s > 0) ? 1u : 0u, lead);
+          } else {
+            for (int s = 0; s < ks; ++s)
+              mma_ts_p(to, tp + s * 8, dv + (uint64_t)(s * (2048 >> 4)), idesc_o, (h > 0 || s > 0) ? 1u : 0u, lead);
           }
+          mma_commit_p(&sm.o_done[m][r], lead);
         }
-        if (!ok) break;
-        mma_commit_w(&sm.kv_empty[sv]);
-        if (have_k) mma_commit_w(&sm.kv_empty[sk]);
+        if (r == 0 && g < all && !(ok = wait(&sm.kv_full[sk], pk, 6))) break;
+        if (g < n) {
+          // the next scores overwrite P's columns: P·V has to be done with them
+          if (!(ok = wait(&sm.o_done[m][r], (h >> 1) & 1, 7))) break;
+          tc_fence_after();
+          issue_s(g, sk);
+        }
+        if (r == 1 || h == all - 1) {
+          mma_commit_p(&sm.kv_empty[sv], lead);
+          ahead(sv, pv);
+        }
+        if (g < all && (r == 1 || g == all - 1)) {
+          mma_commit_p(&sm.kv_empty[sk], lead);
+          ahead(sk, pk);
+        }
       }
-      mma_commit_w(&sm.fin);  // every MMA issued here completes before the CTA tears down
+      mma_commit_p(&sm.fin, lead);  // every MMA issued here completes before the CTA tears down
       const long long c0 = clock64();
       while (!mbar_try_wait(&sm.fin, 0) && clock64() - c0 < kSpinCycles) {
       }
@@ -246,82 +295,110 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const bool mine = my_row < rows;
     // one past the last key this row sees
     const int see = !mine ? 0 : ps.causal ? min(it.lk, it.see + my_row / group + 1) : it.lk;
+    const int all_see = __reduce_min_sync(0xffffffffu, mine ? see : it.lk);  // keys below are hidden from no row here
     const float scale = a.scale;
     float ref = -INFINITY, sum = 0.0f;  // reference in log2 units
     bool ok = true;
     // warps without a row of the unit only keep the barriers going
     const bool idle = (m * kPackBlock + (warp & 3) * 32) >= rows;
-    const int n = kb_end[m] - it.kb0;
-    for (int j = 0; j < n; ++j) {
-      if (!(ok = mbar_wait(&sm.s_full[m], j & 1, &sm.abort, &g_packed_status, 8))) break;
-      if (!idle) {
-        tc_fence_after();
-        const int limit = see - (it.kb0 + j) * kPackBlock;  // columns ≥ limit are hidden
-        uint32_t u[4][32];
+    const int n = steps[m];
+    // Parts of a step's work on its 64 scores u:
+    auto fetch = [&](int h, uint32_t (&u)[2][32]) -> bool {  // starts reading them
+      if (!mbar_wait(&sm.s_full[m][h & 1], (h >> 1) & 1, &sm.abort, &g_packed_status, 8)) return false;
+      tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, u[c]);
-        tmem_ld_wait();
+      for (int c = 0; c < 2; ++c) tmem_ld32(ts + (h & 1) * kHalf + c * 32, u[c]);
+      return true;
+    };
+    auto top_of = [&](int h, uint32_t (&u)[2][32]) -> float {  // has them, hides keys, largest in log2 units
+      tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) reg_fence(u[c]);
-        if (__any_sync(0xffffffffu, limit < kPackBlock)) {
+      for (int c = 0; c < 2; ++c) reg_fence(u[c]);
+      const int limit = see - (2 * it.kb0 + h) * kHalf;  // columns ≥ limit are hidden
+      if ((2 * it.kb0 + h + 1) * kHalf > all_see) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= limit) u[c][i] = 0xff800000u;  // −∞
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int i = 0; i < 32; ++i)
+            if (c * 32 + i >= limit) u[c][i] = 0xff800000u;  // −∞
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 32; i += 2)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(u[c][i]), __uint_as_float(u[c][i + 1]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-        const bool grow = mine && (top > ref + kRescaleAt || ref == -INFINITY);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float next = fmaxf(ref, top);
-          if (j > 0) {
-            const float f = next == -INFINITY ? 1.0f : ex2(ref - next);
-            if (!(ok = mbar_wait(&sm.o_done[m], (j - 1) & 1, &sm.abort, &g_packed_status, 9))) break;
-            tc_fence_after();
-            for (int c = 0; c < dim16; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(to + c, o);
-              tmem_ld_wait();
-              reg_fence(o);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st16(to + c, o);
-            }
-            sum *= f;
-          }
-          ref = next;
-        }
-        const float base = ref == -INFINITY ? 0.0f : BF16 ? ref : ref - kF16Shift;
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < 32; i += 4)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(u[c][i]), scale, -base));
-            const float p1 = ex2(fmaf(__uint_as_float(u[c][i + 1]), scale, -base));
-            part[(i >> 1) & 3] += p0 + p1;
-            p[i >> 1] = pack2<BF16>(p0, p1);
-          }
-          tmem_st16(ts + c * 16, p);
+          const int x = (c & 1) * 2 + i;
+          mx[c] = max3(mx[c], __uint_as_float(u[c >> 1][x]), __uint_as_float(u[c >> 1][x + 1]));
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-        tmem_st_wait();
-        tc_fence_before();
+      return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+    };
+    auto follow = [&](int h, float top) -> bool {  // the reference follows, O is rescaled
+      const bool grow = mine && (top > ref + kRescaleAt || ref == -INFINITY);
+      if (!__any_sync(0xffffffffu, grow)) return true;
+      const float next = fmaxf(ref, top);
+      if (h > 0) {
+        const float f = next == -INFINITY ? 1.0f : ex2(ref - next);
+        if (!mbar_wait(&sm.o_done[m][(h & 1) ^ 1], ((h - 1) >> 1) & 1, &sm.abort, &g_packed_status, 9)) return false;
+        tc_fence_after();
+        for (int c = 0; c < dim16; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(to + c, o);
+          tmem_ld_wait();
+          reg_fence(o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          tmem_st16(to + c, o);
+        }
+        sum *= f;
       }
-      mbar_arrive(&sm.p_full[m]);
+      ref = next;
+      return true;
+    };
+    float part[4];
+    auto exps = [&](int h, const uint32_t (&u)[32], int c) {  // P of 32 keys
+      const float base = ref == -INFINITY ? 0.0f : BF16 ? ref : ref - kF16Shift;
+      uint32_t p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float p0, p1;
+        ffma2(p0, p1, __uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]), scale, scale, -base, -base);
+        p0 = ex2(p0);
+        p1 = ex2(p1);
+        fadd2(part[2 * (i & 1)], part[2 * (i & 1) + 1], p0, p1);
+        p[i] = pack2<BF16>(p0, p1);
+      }
+      tmem_st16(ts + (h & 1) * kHalf + c * 16, p);
+    };
+    auto give = [&](int h) {
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[m][h & 1]);
+    };
+    if (idle) {
+      for (int h = 0; ok && h < n; ++h)
+        if ((ok = mbar_wait(&sm.s_full[m][h & 1], (h >> 1) & 1, &sm.abort, &g_packed_status, 8)))
+          mbar_arrive(&sm.p_full[m][h & 1]);
+    } else {
+      for (int h = 0; h < n; ++h) {
+        uint32_t u[2][32];
+        if (!(ok = fetch(h, u))) break;
+        const float top = top_of(h, u);
+        if (!(ok = follow(h, top))) break;
+        part[0] = part[1] = part[2] = part[3] = 0.0f;
+        exps(h, u[0], 0);
+        exps(h, u[1], 1);
+        give(h);
+      }
     }
     // ── output ──
-    if (ok && n > 0) ok = mbar_wait(&sm.o_done[m], (n - 1) & 1, &sm.abort, &g_packed_status, 10);
+    if (ok && n > 0) ok = mbar_wait(&sm.o_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, &sm.abort, &g_packed_status, 10);
     if (ok && !idle) {
       tc_fence_after();
-      const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-      const float lse = n > 0 && ref != -INFINITY ? (ref - (BF16 ? 0.0f : kF16Shift) + log2f(sum)) * kLn2 : -INFINITY;
+      // a row without a key; one of NaN scores has no maximum either, but its sum is NaN
+      const bool none = n <= 0 || (ref == -INFINITY && sum == sum);
+      const float inv = 1.0f / sum;
+      const float lse = !none ? (ref - (BF16 ? 0.0f : kF16Shift) + log2f(sum)) * kLn2 : -INFINITY;
       const int t = my_row / group, h = ps.few ? head * group + my_row - t * group : head;
       if (it.slot < 0) {
         const long long at = (long long)(it.q0 + t) * ps.heads + h;
@@ -334,7 +411,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             reg_fence(o);
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = n > 0 ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
+          for (int i = 0; i < 16; ++i) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = pack2<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
@@ -359,10 +436,10 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           for (int i = 0; i < 16; i += 4) {
             if (!mine || c + i >= ps.dim) continue;
             float4 f;
-            f.x = n > 0 ? __uint_as_float(o[i]) * inv : 0.0f;
-            f.y = n > 0 ? __uint_as_float(o[i + 1]) * inv : 0.0f;
-            f.z = n > 0 ? __uint_as_float(o[i + 2]) * inv : 0.0f;
-            f.w = n > 0 ? __uint_as_float(o[i + 3]) * inv : 0.0f;
+            f.x = none ? 0.0f : __uint_as_float(o[i]) * inv;
+            f.y = none ? 0.0f : __uint_as_float(o[i + 1]) * inv;
+            f.z = none ? 0.0f : __uint_as_float(o[i + 2]) * inv;
+            f.w = none ? 0.0f : __uint_as_float(o[i + 3]) * inv;
             *reinterpret_cast<float4*>(out + c + i) = f;
           }
           __syncwarp();
@@ -413,7 +490,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
       }
-      if (lane == 0) a.lse[(long long)h * ps.total_q + it.q0 + t] = top == -INFINITY ? -INFINITY : ref + logf(total);
+      if (lane == 0) a.lse[(long long)h * ps.total_q + it.q0 + t] = total > 0.0f || total != total ? ref + logf(total) : -INFINITY;
     }
   }
 }

@@ -46,7 +46,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kHalf = 64;     // queries (or keys) a step
 constexpr int kStages = 4;    // ring of 64-row (Q, dO) or (K, V) pairs
-constexpr int kThreads = 320; // 2 × 4 warps of scores, 1 TMA, 1 MMA
+constexpr int kThreads = 352; // 2 × 4 warps of scores, 1 TMA, 1 to issue the scores' MMAs, 1 the gradients'
 constexpr float kPShift = 15.0f;     // f16: P is held times 2^15
 constexpr uint32_t kColAcc = 256;    // score buffers at 0 (S 64, dP 64) and 128; accumulators from here
 
@@ -58,7 +58,7 @@ template <int DP> struct BwdSmem {
   float red[8];
   uint64_t a_full, a_ready, full[kStages], empty[kStages], s_full[2], p_full[2], g_done[2], fin;
   uint32_t tmem_base;
-  int abort;
+  int abort, last;
 };
 
 struct BwdArgs {
@@ -73,6 +73,8 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b)
   if constexpr (BF16) return pack_bf16x2(a, b);
   else return pack_f16x2(a, b);
 }
+// The four warps of a score group meet; one that gives up arrives without waiting.
+__device__ __forceinline__ void group_leave(int g) { asm volatile("bar.arrive %0, 128;" ::"r"(g + 1) : "memory"); }
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
 
 // Largest power of two p with bound·p < 2^15 (1 for a bound of zero; the exponent is kept within ±60).
@@ -105,7 +107,7 @@ template <int DP> __device__ __forceinline__ uint32_t bwd_setup(BwdSmem<DP>& sm,
       mbar_init(&sm.p_full[b], 128);
       mbar_init(&sm.g_done[b], 1);
     }
-    mbar_init(&sm.fin, 1);
+    mbar_init(&sm.fin, 2);
     sm.abort = 0;
     fence_mbar_init();
   }
@@ -167,6 +169,19 @@ __device__ __forceinline__ void produce(BwdSmem<DP>& sm, const CUtensorMap* m0, 
     const long long c0 = clock64();
     while (!mbar_try_wait(&sm.a_full, 0) && clock64() - c0 < kSpinCycles) {
     }
+  }
+}
+
+// The issuing warps stay converged with uniform values (operands that differ
+// between lanes cost ~60 cycles an MMA); one elected lane issues.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_status, where));
+}
+template <typename Smem> __device__ __forceinline__ void issue_end(Smem& sm, uint32_t lead) {
+  mma_commit_p(&sm.fin, lead);  // every MMA issued here completes before the CTA tears down
+  const long long c0 = clock64();
+  while (!mbar_try_wait(&sm.fin, 0) && clock64() - c0 < kSpinCycles) {
   }
 }
 
@@ -247,9 +262,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const KItem it = reinterpret_cast<const KItem*>(a.plan + ps.dkv_items)[unit];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int dim16 = (ps.dim + 15) & ~15;
-  // steps of 64 queries: from the first that sees a key of the tile
-  const int first_q = ps.causal ? max(0, it.j0 - (it.lk - it.lq)) : 0;
-  const int hb0 = first_q / kHalf, nh = max(0, (it.lq + kHalf - 1) / kHalf - hb0), n = nh * ps.group;
+  // 64-query blocks of a head from the first that sees a key of the tile, and the unit's steps (block b0 of head g0 first)
+  const int hb0 = ps.causal ? max(0, it.j0 - (it.lk - it.lq)) / kHalf : 0, nh = max(0, (it.lq + kHalf - 1) / kHalf - hb0);
+  const int n = it.h1 - it.h0, g0 = nh > 0 ? it.h0 / nh : 0, b0 = it.h0 - g0 * nh;
   const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
 
   if (warp == 8) {
@@ -260,73 +275,90 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         tma_load_3d(sm.a[0] + b * kPackBlock * 128, &map_k, &sm.a_full, b * 64, kvh, it.k0);
         tma_load_3d(sm.a[1] + b * kPackBlock * 128, &map_v, &sm.a_full, b * 64, kvh, it.k0);
       }
-      produce<DP>(sm, &map_q, &map_do, n, [&](int h, int* head, int* row) {
-        *head = kvh * ps.group + h / nh;
-        *row = it.q0 + (hb0 + h % nh) * kHalf;
+      int g = g0, b = b0;
+      produce<DP>(sm, &map_q, &map_do, n, [&](int, int* head, int* row) {
+        *head = kvh * ps.group + g;
+        *row = it.q0 + (hb0 + b) * kHalf;
+        if (++b == nh) b = 0, ++g;
       });
     }
     __syncwarp();
   } else if (warp == 9) {
+    // ── Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ of step h into buffer h mod 2, once the products of step h − 2 are done with it ──
     if (n > 0) {
-      const uint32_t fmt = BF16 ? AB_BF16 : AB_F16;
-      auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &sm.abort, &g_packed_bwd_status, where));
-      };
-      const uint32_t id_s = idesc_f32acc(kPackBlock, kHalf, fmt, false, false);
-      const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, fmt, false, true);
+      const uint32_t lead = elect_lead(), tm = uniform(tmem);
+      const int steps = uniform(n), blocks = uniform(nh), tail = uniform(it.lq - (hb0 + nh - 1) * kHalf);
+      const uint32_t id_s = idesc_f32acc(kPackBlock, kHalf, BF16 ? AB_BF16 : AB_F16, false, false);
       const uint64_t dk = sdesc(smem_u32(sm.a[0]), 16, 1024, SW_128B), dv = sdesc(smem_u32(sm.a[1]), 16, 1024, SW_128B);
-      auto used_of = [&](int h) { return min(kHalf, it.lq - (hb0 + h % nh) * kHalf); };
-      auto issue_s = [&](int h) {  // Sᵀ = K·Qᵀ, dPᵀ = V·dOᵀ
-        const int st = h % kStages, used = used_of(h);
-        if (used & 15) {
-          zero_tail<DP>(sm.ring[st][0], used, lane);
-          zero_tail<DP>(sm.ring[st][1], used, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
+      const uint64_t dq0 = sdesc(smem_u32(sm.ring[0][0]), 16, 1024, SW_128B);
+      constexpr int kABlk = (kPackBlock * 128) >> 4, kBBlk = (kHalf * 128) >> 4, kTileStep = BwdSmem<DP>::kStep >> 4;
+      bool ok = wait_all(&sm.a_full, 0, &sm.abort, 2);
+      int b = uniform(b0);
+      for (int h = 0; ok && h < steps; ++h) {
+        const int st = h % kStages;
+        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 6))) break;
+        if (!(ok = wait_all(&sm.full[st], (h / kStages) & 1, &sm.abort, 3))) break;
+        if (++b == blocks) {  // the last block of a head: rows past the sequence's end
+          b = 0;
+          if (tail & 15) {
+            zero_tail<DP>(sm.ring[st][0], tail, lane);
+            zero_tail<DP>(sm.ring[st][1], tail, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
         }
-        const uint64_t bq = sdesc(smem_u32(sm.ring[st][0]), 16, 1024, SW_128B);
-        const uint64_t bo = sdesc(smem_u32(sm.ring[st][1]), 16, 1024, SW_128B);
-        const uint32_t ts = tmem + (h & 1) * 128;
-        for (int s = 0; s < dim16 / 16; ++s) {
-          const uint64_t oa = (uint64_t)((s >> 2) * ((kPackBlock * 128) >> 4) + (s & 3) * 2);
-          const uint64_t ob = (uint64_t)((s >> 2) * ((kHalf * 128) >> 4) + (s & 3) * 2);
-          mma_ss_w(ts, dk + oa, bq + ob, id_s, s > 0 ? 1u : 0u);
-          mma_ss_w(ts + kHalf, dv + oa, bo + ob, id_s, s > 0 ? 1u : 0u);
-        }
-        mma_commit_w(&sm.s_full[h & 1]);
-      };
-      bool ok = wait(&sm.a_full, 0, 2);
-      for (int h = 0; ok && h < min(2, n); ++h) {
-        if (!(ok = wait(&sm.full[h], 0, 3))) break;
         tc_fence_after();
-        issue_s(h);
+        const uint64_t bq = dq0 + (uint64_t)(st * 2 * kTileStep), bo = bq + kTileStep;
+        const uint32_t ts = tm + (h & 1) * 128;
+        auto one = [&](int s) {
+          const uint64_t oa = (uint64_t)((s >> 2) * kABlk + (s & 3) * 2), ob = (uint64_t)((s >> 2) * kBBlk + (s & 3) * 2);
+          mma_ss_p(ts, dk + oa, bq + ob, id_s, s > 0 ? 1u : 0u, lead);
+          mma_ss_p(ts + kHalf, dv + oa, bo + ob, id_s, s > 0 ? 1u : 0u, lead);
+        };
+        if (dim16 == DP) {
+#pragma unroll
+          for (int s = 0; s < DP / 16; ++s) one(s);
+        } else {
+          for (int s = 0; s < dim16 / 16; ++s) one(s);
+        }
+        mma_commit_p(&sm.s_full[h & 1], lead);
       }
-      for (int h = 0; ok && h < n; ++h) {
-        const int b = h & 1, st = h % kStages, steps = (used_of(h) + 15) >> 4;
-        if (!(ok = wait(&sm.p_full[b], (h >> 1) & 1, 4))) break;
+      issue_end(sm, lead);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    // ── dV += Pᵀ·dO, dK += dSᵀ·Q ──
+    if (n > 0) {
+      const uint32_t lead = elect_lead(), tm = uniform(tmem);
+      const int steps = uniform(n), blocks = uniform(nh), tail = uniform(it.lq - (hb0 + nh - 1) * kHalf);
+      const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, BF16 ? AB_BF16 : AB_F16, false, true);
+      const uint64_t dq0 = sdesc(smem_u32(sm.ring[0][0]), kHalf * 128, 1024, SW_128B);
+      constexpr int kTileStep = BwdSmem<DP>::kStep >> 4;
+      bool ok = true;
+      int b = uniform(b0);
+      for (int h = 0; h < steps; ++h) {
+        const int st = h % kStages;
+        int ks = kHalf / 16;
+        if (++b == blocks) b = 0, ks = min(ks, (tail + 15) >> 4);
+        if (!(ok = wait_all(&sm.p_full[h & 1], (h >> 1) & 1, &sm.abort, 4))) break;
         tc_fence_after();
-        const uint64_t gq = sdesc(smem_u32(sm.ring[st][0]), kHalf * 128, 1024, SW_128B);
-        const uint64_t go = sdesc(smem_u32(sm.ring[st][1]), kHalf * 128, 1024, SW_128B);
-        const uint32_t tp = tmem + b * 128;
-        for (int s = 0; s < steps; ++s) {
+        const uint64_t gq = dq0 + (uint64_t)(st * 2 * kTileStep), go = gq + kTileStep;
+        const uint32_t tp = tm + (h & 1) * 128;
+        auto one = [&](int s) {
           const uint32_t acc = (h > 0 || s > 0) ? 1u : 0u;
-          mma_ts_w(tmem + kColAcc, tp + s * 8, go + (uint64_t)(s * (2048 >> 4)), id_g, acc);
-          mma_ts_w(tmem + kColAcc + DP, tp + kHalf + s * 8, gq + (uint64_t)(s * (2048 >> 4)), id_g, acc);
+          mma_ts_p(tm + kColAcc, tp + s * 8, go + (uint64_t)(s * (2048 >> 4)), id_g, acc, lead);
+          mma_ts_p(tm + kColAcc + DP, tp + kHalf + s * 8, gq + (uint64_t)(s * (2048 >> 4)), id_g, acc, lead);
+        };
+        if (ks == kHalf / 16) {
+#pragma unroll
+          for (int s = 0; s < kHalf / 16; ++s) one(s);
+        } else {
+          for (int s = 0; s < ks; ++s) one(s);
         }
-        mma_commit_w(&sm.empty[st]);
-        mma_commit_w(&sm.g_done[b]);
-        if (h + 2 < n) {
-          const int h2 = h + 2;
-          // the next scores overwrite P's and dS's columns: the products have to be done with them
-          if (!(ok = wait(&sm.full[h2 % kStages], (h2 / kStages) & 1, 5) && wait(&sm.g_done[b], (h >> 1) & 1, 6))) break;
-          tc_fence_after();
-          issue_s(h2);
-        }
+        mma_commit_p(&sm.g_done[h & 1], lead);
+        mma_commit_p(&sm.empty[st], lead);
       }
-      mma_commit_w(&sm.fin);  // every MMA issued here completes before the CTA tears down
-      const long long c0 = clock64();
-      while (!mbar_try_wait(&sm.fin, 0) && clock64() - c0 < kSpinCycles) {
-      }
+      issue_end(sm, lead);
     }
     __syncwarp();
   } else {
@@ -364,27 +396,43 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int off = it.lk - it.lq, j = it.j0 + key;
     bool ok = true;
     // (lse, Δ) of a step's query, fetched a step ahead by the group's first 64 threads
+    int fg = g0, fb = b0;  // head and block of the step that is fetched next
+    auto advance = [&](int by) {
+      fb += by;
+      while (fb >= nh) fb -= nh, ++fg;
+    };
     auto fetch = [&](int h) -> float2 {
       float2 f = make_float2(INFINITY, 0.0f);  // past the sequence: P = 2^−∞
       if (h < n && key < kHalf) {
-        const int i = (hb0 + h % nh) * kHalf + key;
-        if (i < it.lq) f = pairs[(long long)(kvh * ps.group + h / nh) * ps.total_q + it.q0 + i];
+        const int i = (hb0 + fb) * kHalf + key;
+        if (i < it.lq) f = pairs[(long long)(kvh * ps.group + fg) * ps.total_q + it.q0 + i];
         if constexpr (!BF16) f.x -= kPShift;
       }
       return f;
     };
+    if (n > 0) advance(g);
     float2 ahead = fetch(g);
+    int block = fb;
     for (int h = g; h < n; h += 2) {
       const int k = h >> 1;
       float4* st = sm.stats[g][k & 1];
       if (key < kHalf) reinterpret_cast<float2*>(st)[key] = ahead;
       group_sync(g);
+      if (*(volatile int*)&sm.abort) {
+        ok = false;
+        break;
+      }
+      const int i0 = (hb0 + block) * kHalf;
+      advance(2);
       ahead = fetch(h + 2);
-      const int i0 = (hb0 + h % nh) * kHalf;
+      block = fb;
       // queries [lo, hi) of the step see this key
       const int lo = ps.causal ? j - off - i0 : 0, hi = it.lq - i0;
       const bool whole = hi >= kHalf && (!ps.causal || it.j0 + it.keys - 1 - off <= i0);
-      if (!(ok = mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 8))) break;
+      if (!(ok = mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 8))) {
+        group_leave(g);
+        break;
+      }
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -423,17 +471,65 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (n > 0) ok = mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 9) && ok;
     if (ok && !sm.abort) {  // group 0 stores dV, group 1 dK
       tc_fence_after();
-      const long long row = it.k0 + key;
-      uint16_t* out = g == 0 ? static_cast<uint16_t*>(a.dv) + row * a.dv_row + kvh * a.dv_head
-                             : static_cast<uint16_t*>(a.dk) + row * a.dk_row + kvh * a.dk_head;
-      const float f = g == 0 ? (BF16 ? 1.0f : 3.0517578125e-05f) : a.scale / mult;
-      for (int c = 0; c < dim16; c += 16)
-        store16<BF16>(tmem + lanes + kColAcc + g * DP, n == 0, f, mine, out, c, ps.dim);
+      const uint32_t acc = tmem + lanes + kColAcc + g * DP;
+      const float f = g == 0 ? (BF16 ? 1.0f : 3.0517578125e-05f) : 1.0f / mult;
+      if (it.slot < 0) {
+        const long long row = it.k0 + key;
+        uint16_t* out = g == 0 ? static_cast<uint16_t*>(a.dv) + row * a.dv_row + kvh * a.dv_head
+                               : static_cast<uint16_t*>(a.dk) + row * a.dk_row + kvh * a.dk_head;
+        for (int c = 0; c < dim16; c += 16)
+          store16<BF16>(acc, n == 0, g == 0 ? f : f * a.scale, mine, out, c, ps.dim);
+      } else {
+        float* out = reinterpret_cast<float*>(a.plan + ps.part_dkv) +
+                     ((((long long)it.slot * ps.kv_heads + kvh) * 2 + g) * kPackBlock + key) * ps.dim;
+        for (int c = 0; c < dim16; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(acc + c, o);
+          tmem_ld_wait();
+          reg_fence(o);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            if (mine && c + i < ps.dim)
+              *reinterpret_cast<float4*>(out + c + i) =
+                  make_float4(__uint_as_float(o[i]) * f, __uint_as_float(o[i + 1]) * f, __uint_as_float(o[i + 2]) * f,
+                              __uint_as_float(o[i + 3]) * f);
+          __syncwarp();
+        }
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 8) tmem_dealloc(tmem, 512);
+
+  if (it.slot < 0 || sm.abort) return;
+  // ── the last of a tile's parts to arrive adds them in their order ──
+  if (tid == 0) {
+    __threadfence();
+    int* cnt = reinterpret_cast<int*>(a.plan + ps.dkv_counters) + (long long)it.counter * ps.kv_heads + kvh;
+    sm.last = atomicAdd(cnt, 1) == it.parts - 1;
+    if (sm.last) *cnt = 0;  // for the next call with this plan
+    __threadfence();
+  }
+  __syncthreads();
+  if (!sm.last) return;
+  const int vecs = ps.dim / 4;
+  const long long part_step = (long long)ps.kv_heads * 2 * kPackBlock * ps.dim;
+  for (int i = tid; i < 2 * it.keys * vecs; i += kThreads) {
+    const int which = i / (it.keys * vecs), rest = i - which * it.keys * vecs, r = rest / vecs, c = (rest - r * vecs) * 4;
+    const float* src = reinterpret_cast<const float*>(a.plan + ps.part_dkv) +
+                       ((((long long)it.slot0 * ps.kv_heads + kvh) * 2 + which) * kPackBlock + r) * ps.dim + c;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < it.parts; ++k) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(src + k * part_step));
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const float f = which ? a.scale : 1.0f;
+    const long long row = it.k0 + r;
+    uint16_t* out = which ? static_cast<uint16_t*>(a.dk) + row * a.dk_row + kvh * a.dk_head
+                          : static_cast<uint16_t*>(a.dv) + row * a.dv_row + kvh * a.dv_head;
+    *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2<BF16>(sum.x * f, sum.y * f), pack2<BF16>(sum.z * f, sum.w * f));
+  }
 }
 
 // ── dQ ───────────────────────────────────────────────────────────────────────
@@ -469,59 +565,70 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     __syncwarp();
   } else if (warp == 9) {
+    // ── S = Q·Kᵀ and dP = dO·Vᵀ of step h into buffer h mod 2, once dQ is done with step h − 2's ──
     if (n > 0) {
-      const uint32_t fmt = BF16 ? AB_BF16 : AB_F16;
-      auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &sm.abort, &g_packed_bwd_status, where));
-      };
-      const uint32_t id_s = idesc_f32acc(kPackBlock, kHalf, fmt, false, false);
-      const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, fmt, false, true);
-      auto used_of = [&](int h) { return min(kHalf, see_end - h * kHalf); };
-      auto issue_s = [&](int h) {  // S = Q·Kᵀ, dP = dO·Vᵀ
-        const int st = h % kStages, used = used_of(h);
-        if (used & 15) {
-          zero_tail<DP>(sm.ring[st][0], used, lane);
+      const uint32_t lead = elect_lead(), tm = uniform(tmem);
+      const int steps = uniform(n), tail = uniform(see_end - (n - 1) * kHalf);
+      const uint32_t id_s = idesc_f32acc(kPackBlock, kHalf, BF16 ? AB_BF16 : AB_F16, false, false);
+      const uint64_t dk0 = sdesc(smem_u32(sm.ring[0][0]), 16, 1024, SW_128B);
+      constexpr int kBBlk = (kHalf * 128) >> 4, kTileStep = BwdSmem<DP>::kStep >> 4;
+      bool ok = wait_all(&sm.a_ready, 0, &sm.abort, 12);
+      for (int h = 0; ok && h < steps; ++h) {
+        const int st = h % kStages;
+        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 16))) break;
+        if (!(ok = wait_all(&sm.full[st], (h / kStages) & 1, &sm.abort, 13))) break;
+        if (h == steps - 1 && (tail & 15)) {
+          zero_tail<DP>(sm.ring[st][0], tail, lane);
           fence_proxy_async_smem();
           __syncwarp();
         }
-        const uint64_t bk = sdesc(smem_u32(sm.ring[st][0]), 16, 1024, SW_128B);
-        const uint64_t bv = sdesc(smem_u32(sm.ring[st][1]), 16, 1024, SW_128B);
-        const uint32_t ts = tmem + (h & 1) * 128;
-        for (int s = 0; s < dim16 / 16; ++s) {
-          const uint64_t ob = (uint64_t)((s >> 2) * ((kHalf * 128) >> 4) + (s & 3) * 2);
-          mma_ts_w(ts, tmem + kColQ + s * 8, bk + ob, id_s, s > 0 ? 1u : 0u);
-          mma_ts_w(ts + kHalf, tmem + kColDO + s * 8, bv + ob, id_s, s > 0 ? 1u : 0u);
-        }
-        mma_commit_w(&sm.s_full[h & 1]);
-      };
-      bool ok = wait(&sm.a_ready, 0, 12);
-      for (int h = 0; ok && h < min(2, n); ++h) {
-        if (!(ok = wait(&sm.full[h], 0, 13))) break;
         tc_fence_after();
-        issue_s(h);
-      }
-      for (int h = 0; ok && h < n; ++h) {
-        const int b = h & 1, st = h % kStages, steps = (used_of(h) + 15) >> 4;
-        if (!(ok = wait(&sm.p_full[b], (h >> 1) & 1, 14))) break;
-        tc_fence_after();
-        const uint64_t gk = sdesc(smem_u32(sm.ring[st][0]), kHalf * 128, 1024, SW_128B);
-        for (int s = 0; s < steps; ++s)
-          mma_ts_w(tmem + kColAcc, tmem + b * 128 + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g,
-                   (h > 0 || s > 0) ? 1u : 0u);
-        mma_commit_w(&sm.empty[st]);
-        mma_commit_w(&sm.g_done[b]);
-        if (h + 2 < n) {
-          const int h2 = h + 2;
-          if (!(ok = wait(&sm.full[h2 % kStages], (h2 / kStages) & 1, 15) && wait(&sm.g_done[b], (h >> 1) & 1, 16)))
-            break;
-          tc_fence_after();
-          issue_s(h2);
+        const uint64_t bk = dk0 + (uint64_t)(st * 2 * kTileStep), bv = bk + kTileStep;
+        const uint32_t ts = tm + (h & 1) * 128;
+        auto one = [&](int s) {
+          const uint64_t ob = (uint64_t)((s >> 2) * kBBlk + (s & 3) * 2);
+          mma_ts_p(ts, tm + kColQ + s * 8, bk + ob, id_s, s > 0 ? 1u : 0u, lead);
+          mma_ts_p(ts + kHalf, tm + kColDO + s * 8, bv + ob, id_s, s > 0 ? 1u : 0u, lead);
+        };
+        if (dim16 == DP) {
+#pragma unroll
+          for (int s = 0; s < DP / 16; ++s) one(s);
+        } else {
+          for (int s = 0; s < dim16 / 16; ++s) one(s);
         }
+        mma_commit_p(&sm.s_full[h & 1], lead);
       }
-      mma_commit_w(&sm.fin);
-      const long long c0 = clock64();
-      while (!mbar_try_wait(&sm.fin, 0) && clock64() - c0 < kSpinCycles) {
+      issue_end(sm, lead);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    // ── dQ += dS·K ──
+    if (n > 0) {
+      const uint32_t lead = elect_lead(), tm = uniform(tmem);
+      const int steps = uniform(n), tail = uniform(see_end - (n - 1) * kHalf);
+      const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, BF16 ? AB_BF16 : AB_F16, false, true);
+      const uint64_t dk0 = sdesc(smem_u32(sm.ring[0][0]), kHalf * 128, 1024, SW_128B);
+      constexpr int kTileStep = BwdSmem<DP>::kStep >> 4;
+      bool ok = true;
+      for (int h = 0; h < steps; ++h) {
+        const int st = h % kStages, ks = h == steps - 1 ? (tail + 15) >> 4 : kHalf / 16;
+        if (!(ok = wait_all(&sm.p_full[h & 1], (h >> 1) & 1, &sm.abort, 14))) break;
+        tc_fence_after();
+        const uint64_t gk = dk0 + (uint64_t)(st * 2 * kTileStep);
+        auto one = [&](int s) {
+          mma_ts_p(tm + kColAcc, tm + (h & 1) * 128 + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g,
+                   (h > 0 || s > 0) ? 1u : 0u, lead);
+        };
+        if (ks == kHalf / 16) {
+#pragma unroll
+          for (int s = 0; s < kHalf / 16; ++s) one(s);
+        } else {
+          for (int s = 0; s < ks; ++s) one(s);
+        }
+        mma_commit_p(&sm.g_done[h & 1], lead);
+        mma_commit_p(&sm.empty[st], lead);
       }
+      issue_end(sm, lead);
     }
     __syncwarp();
   } else {

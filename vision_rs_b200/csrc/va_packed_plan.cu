@@ -5,8 +5,8 @@
 //   list 0  forward units,  list 1  dQ units,  list 2  dK/dV units (training)
 //
 // A block counts its tiles (prefix sum over the sequences), sums their key
-// (or query) blocks, cuts the forward tiles' key ranges into parts when there
-// are few tiles (`split_budget` parts over all), and writes the units sorted
+// (or query) blocks, cuts long tiles into parts where that evens the load (at
+// most `budget` parts more than tiles), and writes the units sorted
 // by their size, longest first (a counting sort over 256 size classes), so
 // that the last blocks of the attention's grid are its shortest.  Units of a
 // class may come in any order: each writes results of its own.
@@ -20,6 +20,8 @@ namespace va {
 namespace {
 
 constexpr int kPlanThreads = 512, kClasses = 256;
+// Parts smaller than this cost more to join than they save (a forward block takes ~1 us, joining ~4 us).
+constexpr int kMinKeyBlocks = 6, kMinQuerySteps = 32;
 
 struct Seq {
   int q0, lq, k0, lk;
@@ -84,11 +86,10 @@ __device__ __forceinline__ Range key_blocks(const Seq& s, int i0, int n, int cau
   const int end = causal ? min(s.lk, max(0, i0 + n + s.lk - s.lq)) : s.lk;
   return {0, (end + kPackBlock - 1) / kPackBlock};
 }
-// Query blocks that see any of the keys from j0 on.
-__device__ __forceinline__ Range query_blocks(const Seq& s, int j0, int causal) {
-  const int n = (s.lq + kPackBlock - 1) / kPackBlock;
-  const int i0 = causal ? max(0, j0 - (s.lk - s.lq)) : 0;
-  return {min(n, i0 / kPackBlock), n};
+// Steps of 64 queries, over the heads of a group, that see any of the keys from j0 on.
+__device__ __forceinline__ Range query_steps(const Seq& s, int j0, int causal, int group) {
+  const int first = causal ? max(0, j0 - (s.lk - s.lq)) / 64 : 0;
+  return {0, max(0, (s.lq + 63) / 64 - first) * group};
 }
 
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
   if (tid == 0) first[s.num_seqs] = tiles;
   __syncthreads();
   // offsets that run backwards could name more rows than there are: keep to the lists' room
-  const int room = list == 0 ? s.max_tiles : list == 1 ? s.max_dq_items : s.max_dkv_items;
+  const int room = list == 0 ? s.max_tiles : list == 1 ? s.max_dq_items : s.max_dkv_tiles;
   if (tiles > room) {
     if (tid == 0) bad = 1;
     tiles = room;
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
     *q = load_seq(a.cu_q, a.cu_k, b, s.total_q, s.total_k, &bad);
     *i0 = (t - first[b]) * tile;
     const Range r =
-        list == 2 ? query_blocks(*q, *i0, s.causal) : key_blocks(*q, *i0, min(tile, q->lq - *i0), s.causal);
+        list == 2 ? query_steps(*q, *i0, s.causal, s.group) : key_blocks(*q, *i0, min(tile, q->lq - *i0), s.causal);
     if (t == tid) own_seq = *q, own_i0 = *i0, own_range = r;
     return r;
   };
@@ -156,8 +157,9 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
   atomicMax(&most, mine_most);
   int blocks;
   block_scan(mine, &blocks);
-  // parts of at most `chunk` blocks: Σ ceil(b / chunk) ≤ tiles + blocks / chunk ≤ tiles + split_budget
-  const int chunk = list == 0 && s.split_budget ? max((blocks + s.split_budget - 1) / s.split_budget, 2) : 1 << 30;
+  // parts of at most `chunk` blocks: Σ ceil(b / chunk) ≤ tiles + blocks / chunk ≤ tiles + budget
+  const int budget = list == 0 ? s.split_budget : list == 2 ? s.dkv_budget : 0;
+  const int chunk = budget ? max((blocks + budget - 1) / budget, list == 0 ? kMinKeyBlocks : kMinQuerySteps) : 1 << 30;
   const int top = max(1, min(most, chunk));
 
   auto parts_of = [&](const Range& r) { return max(1, (r.b1 - r.b0 + chunk - 1) / chunk); };
@@ -197,8 +199,11 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
     const int n = r.b1 - r.b0;
     int at = atomicAdd(&cursor[size_class(n, p)], p);
     if (list == 2) {
-      reinterpret_cast<KItem*>(a.plan + s.dkv_items)[at] =
-          KItem{q.k0 + i0, min(tile, q.lk - i0), i0, q.q0, q.lq, q.lk, r.b0, r.b1};
+      KItem* out = reinterpret_cast<KItem*>(a.plan + s.dkv_items);
+      for (int k = 0; k < p; ++k, ++at)
+        out[at] = KItem{q.k0 + i0, min(tile, q.lk - i0), i0, q.q0, q.lq, q.lk,
+                        (int)((long long)n * k / p), (int)((long long)n * (k + 1) / p),
+                        p > 1 ? slot0 + k : -1, slot0, p, t};
       continue;
     }
     QItem* out = reinterpret_cast<QItem*>(a.plan + (list == 0 ? s.items : s.dq_items));
@@ -207,10 +212,9 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
                       r.b0 + (int)((long long)n * k / p), r.b0 + (int)((long long)n * (k + 1) / p),
                       p > 1 ? slot0 + k : -1, slot0, p, t, 0};
   }
-  if (list == 0) {  // arrival counters of the split tiles
-    int* cnt = reinterpret_cast<int*>(a.plan + s.counters);
-    if (s.few)
-      for (int i = tid; i < tiles * s.units; i += kPlanThreads) cnt[i] = 0;
+  if (budget) {  // arrival counters of the split tiles
+    int* cnt = reinterpret_cast<int*>(a.plan + (list == 0 ? s.counters : s.dkv_counters));
+    for (int i = tid; i < tiles * (list == 0 ? s.units : s.kv_heads); i += kPlanThreads) cnt[i] = 0;
   }
   __syncthreads();
   if (tid == 0) {
