@@ -32,6 +32,8 @@
 // the summed operand past the sequence's end are zeroed (0 · NaN is NaN).
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "va_common.cuh"
 #include "va_packed.h"
 #include "va_sm100.cuh"
@@ -54,7 +56,7 @@ template <int DP> struct BwdSmem {
   static constexpr int kTile = kPackBlock * DP * 2, kStep = kHalf * DP * 2;
   uint8_t a[2][kTile];               // K and V of the keys, or Q and dO of the queries: per 64 dims 128 rows × 128 bytes
   uint8_t ring[kStages][2][kStep];   // per 64 dims 64 rows × 128 bytes
-  float4 stats[2][2][kHalf / 2];     // dK/dV: (lse, Δ) of the step's queries, per group, two steps
+  float4 stats[2][2][2][kHalf / 4];  // dK/dV: −lse·log2 e and −Δ of the step's queries, per group, two steps
   float red[8];
   uint64_t a_full, a_ready, full[kStages], empty[kStages], s_full[2], p_full[2], g_done[2], fin;
   uint32_t tmem_base;
@@ -296,7 +298,6 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       int b = uniform(b0);
       for (int h = 0; ok && h < steps; ++h) {
         const int st = h % kStages;
-        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 6))) break;
         if (!(ok = wait_all(&sm.full[st], (h / kStages) & 1, &sm.abort, 3))) break;
         if (++b == blocks) {  // the last block of a head: rows past the sequence's end
           b = 0;
@@ -307,6 +308,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             __syncwarp();
           }
         }
+        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 6))) break;
         tc_fence_after();
         const uint64_t bq = dq0 + (uint64_t)(st * 2 * kTileStep), bo = bq + kTileStep;
         const uint32_t ts = tm + (h & 1) * 128;
@@ -415,8 +417,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     int block = fb;
     for (int h = g; h < n; h += 2) {
       const int k = h >> 1;
-      float4* st = sm.stats[g][k & 1];
-      if (key < kHalf) reinterpret_cast<float2*>(st)[key] = ahead;
+      if (key < kHalf) {
+        reinterpret_cast<float*>(sm.stats[g][k & 1][0])[key] = -ahead.x;
+        reinterpret_cast<float*>(sm.stats[g][k & 1][1])[key] = -ahead.y;
+      }
       group_sync(g);
       if (*(volatile int*)&sm.abort) {
         ok = false;
@@ -434,36 +438,49 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         break;
       }
       tc_fence_after();
+      const float4 *nl = sm.stats[g][k & 1][0], *nd = sm.stats[g][k & 1][1];
+      // 16 queries at a time: their statistics are read while the scores come
+      auto scores = [&](auto masked) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], d[32];
-        tmem_ld32(ts + c * 32, s);
-        tmem_ld32(ts + kHalf + c * 32, d);
-        tmem_ld_wait();
-        reg_fence(s);
-        reg_fence(d);
-        uint32_t pp[16], pd[16];
+        for (int c = 0; c < kHalf / 16; ++c) {
+          uint32_t s[16], d[16];
+          float4 l[4], e[4];
+          tmem_ld16(ts + c * 16, s);
+          tmem_ld16(ts + kHalf + c * 16, d);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float4 q = st[(c * 32 + i) >> 1];
-          float p0 = ex2(fmaf(__uint_as_float(s[i]), scale2, -q.x));
-          float p1 = ex2(fmaf(__uint_as_float(s[i + 1]), scale2, -q.z));
-          float d0 = p0 * (__uint_as_float(d[i]) - q.y);
-          float d1 = p1 * (__uint_as_float(d[i + 1]) - q.w);
-          if (!whole) {
-            const bool v0 = c * 32 + i >= lo && c * 32 + i < hi, v1 = c * 32 + i + 1 >= lo && c * 32 + i + 1 < hi;
-            p0 = v0 ? p0 : 0.0f;
-            d0 = v0 ? d0 : 0.0f;
-            p1 = v1 ? p1 : 0.0f;
-            d1 = v1 ? d1 : 0.0f;
+          for (int i = 0; i < 4; ++i) l[i] = nl[c * 4 + i], e[i] = nd[c * 4 + i];
+          tmem_ld_wait();
+          reg_fence(s);
+          reg_fence(d);
+          uint32_t pp[8], pd[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 &lf = l[i >> 1], &ef = e[i >> 1];
+            float p0, p1, d0 = __uint_as_float(d[2 * i]), d1 = __uint_as_float(d[2 * i + 1]);
+            ffma2(p0, p1, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), scale2, scale2, i & 1 ? lf.z : lf.x,
+                  i & 1 ? lf.w : lf.y);
+            fadd2(d0, d1, i & 1 ? ef.z : ef.x, i & 1 ? ef.w : ef.y);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            fmul2(d0, d1, p0, p1);
+            if constexpr (decltype(masked)::value) {
+              const int q0 = c * 16 + 2 * i, q1 = q0 + 1;
+              const bool v0 = q0 >= lo && q0 < hi, v1 = q1 >= lo && q1 < hi;
+              p0 = v0 ? p0 : 0.0f;
+              d0 = v0 ? d0 : 0.0f;
+              p1 = v1 ? p1 : 0.0f;
+              d1 = v1 ? d1 : 0.0f;
+            }
+            if constexpr (!BF16) fmul2(d0, d1, mult_p, mult_p);
+            pp[i] = pack2<BF16>(p0, p1);
+            pd[i] = pack2<BF16>(d0, d1);
           }
-          if constexpr (!BF16) d0 *= mult_p, d1 *= mult_p;
-          pp[i >> 1] = pack2<BF16>(p0, p1);
-          pd[i >> 1] = pack2<BF16>(d0, d1);
+          tmem_st8(ts + c * 8, pp);
+          tmem_st8(ts + kHalf + c * 8, pd);
         }
-        tmem_st16(ts + c * 16, pp);
-        tmem_st16(ts + kHalf + c * 16, pd);
-      }
+      };
+      if (__all_sync(0xffffffffu, whole)) scores(std::false_type{});
+      else scores(std::true_type{});
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.p_full[g]);
@@ -575,13 +592,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       bool ok = wait_all(&sm.a_ready, 0, &sm.abort, 12);
       for (int h = 0; ok && h < steps; ++h) {
         const int st = h % kStages;
-        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 16))) break;
         if (!(ok = wait_all(&sm.full[st], (h / kStages) & 1, &sm.abort, 13))) break;
         if (h == steps - 1 && (tail & 15)) {
           zero_tail<DP>(sm.ring[st][0], tail, lane);
           fence_proxy_async_smem();
           __syncwarp();
         }
+        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 16))) break;
         tc_fence_after();
         const uint64_t bk = dk0 + (uint64_t)(st * 2 * kTileStep), bv = bk + kTileStep;
         const uint32_t ts = tm + (h & 1) * 128;
@@ -676,29 +693,34 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!(ok = mbar_wait(&sm.s_full[g], (h >> 1) & 1, &sm.abort, &g_packed_bwd_status, 18))) break;
       tc_fence_after();
       const int limit = see - h * kHalf;
-      const bool whole = __all_sync(0xffffffffu, limit >= kHalf);
+      auto scores = [&](auto masked) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], d[32];
-        tmem_ld32(ts + c * 32, s);
-        tmem_ld32(ts + kHalf + c * 32, d);
-        tmem_ld_wait();
-        reg_fence(s);
-        reg_fence(d);
-        uint32_t pd[16];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32], d[32];
+          tmem_ld32(ts + c * 32, s);
+          tmem_ld32(ts + kHalf + c * 32, d);
+          tmem_ld_wait();
+          reg_fence(s);
+          reg_fence(d);
+          uint32_t pd[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float d0 = ex2(fmaf(__uint_as_float(s[i]), scale2, -stat.x)) * (__uint_as_float(d[i]) - stat.y);
-          float d1 = ex2(fmaf(__uint_as_float(s[i + 1]), scale2, -stat.x)) * (__uint_as_float(d[i + 1]) - stat.y);
-          if (!whole) {
-            d0 = c * 32 + i < limit ? d0 : 0.0f;
-            d1 = c * 32 + i + 1 < limit ? d1 : 0.0f;
+          for (int i = 0; i < 32; i += 2) {
+            float p0, p1, d0 = __uint_as_float(d[i]), d1 = __uint_as_float(d[i + 1]);
+            ffma2(p0, p1, __uint_as_float(s[i]), __uint_as_float(s[i + 1]), scale2, scale2, -stat.x, -stat.x);
+            fadd2(d0, d1, -stat.y, -stat.y);
+            fmul2(d0, d1, ex2(p0), ex2(p1));
+            if constexpr (decltype(masked)::value) {
+              d0 = c * 32 + i < limit ? d0 : 0.0f;
+              d1 = c * 32 + i + 1 < limit ? d1 : 0.0f;
+            }
+            if constexpr (!BF16) fmul2(d0, d1, mult, mult);
+            pd[i >> 1] = pack2<BF16>(d0, d1);
           }
-          if constexpr (!BF16) d0 *= mult, d1 *= mult;
-          pd[i >> 1] = pack2<BF16>(d0, d1);
+          tmem_st16(ts + c * 16, pd);
         }
-        tmem_st16(ts + c * 16, pd);
-      }
+      };
+      if (__all_sync(0xffffffffu, limit >= kHalf)) scores(std::false_type{});
+      else scores(std::true_type{});
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.p_full[g]);

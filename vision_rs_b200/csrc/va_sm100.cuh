@@ -250,6 +250,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// 32 lanes × 32 bit, 8 consecutive columns per thread.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // Orders every later use of `r` after the preceding tcgen05.wait::ld: the
 // registers written by an asynchronous tcgen05.ld are only valid after the
 // wait, so reads must not be hoisted above it.
@@ -341,6 +347,12 @@ __device__ __forceinline__ void ffma2(float& d0, float& d1, float a0, float a1, 
 }
 __device__ __forceinline__ void fadd2(float& d0, float& d1, float a0, float a1) {
   asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.f32x2 a, a, b;\n"
+      " mov.b64 {%0, %1}, a;\n}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1));
+}
+__device__ __forceinline__ void fmul2(float& d0, float& d1, float a0, float a1) {  // d *= a
+  asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n mul.rn.f32x2 a, a, b;\n"
       " mov.b64 {%0, %1}, a;\n}"
       : "+f"(d0), "+f"(d1)
       : "f"(a0), "f"(a1));
