@@ -17,7 +17,6 @@
 // block walks its rows with the columns' sums in registers and writes one
 // partial row; a second kernel adds the partials in a fixed order, so the
 // result does not depend on scheduling (no atomics).
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -39,13 +38,6 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-
-template <typename T> struct alignas(16) Vec16 {
-  T v[16 / sizeof(T)];
-};
-template <int N> struct alignas(N) Bytes {
-  uint8_t v[N];
-};
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
   float d;
@@ -96,16 +88,25 @@ __device__ __forceinline__ void load_w(const void* w, int w_f32, int c, float (&
 #pragma unroll
     for (int j = 0; j < N; j += 4) {
       const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + c + j));
-      o[j] = f.x;
-      o[j + 1] = f.y;
-      o[j + 2] = f.z;
-      o[j + 3] = f.w;
+      o[j] = f.x, o[j + 1] = f.y, o[j + 2] = f.z, o[j + 3] = f.w;
     }
   } else {
-    const Vec16<T> v = *reinterpret_cast<const Vec16<T>*>(static_cast<const T*>(w) + c);
-#pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = to_f32(v.v[j]);
+    Bytes16<T>::get(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w) + c)), o);
   }
+}
+
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("{\n .reg .b16 lo, hi;\n cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n"
+      " mov.b32 %0, {lo, hi};\n}"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
+__device__ __forceinline__ float max_nan_abs(float a, float b) {  // max(a, |b|), NaN if either is
+  float d;
+  asm("{\n .reg .f32 t;\n abs.f32 t, %2;\n max.NaN.f32 %0, %1, t;\n}" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 __device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
@@ -115,35 +116,40 @@ constexpr int block_threads(int tpr) { return tpr == 32 ? 256 : tpr; }
 
 template <typename T, int TPR, int NV, bool F8>
 __global__ void __launch_bounds__(block_threads(TPR)) rms_norm_kernel(NormArgs a) {
-  constexpr int VEC = 16 / sizeof(T);
+  using B = Bytes16<T>;
+  constexpr int VEC = B::N;
   __shared__ float red[2][32];
   const long long row = (long long)blockIdx.x * rows_per_block(TPR) + (TPR == 32 ? threadIdx.x >> 5 : 0);
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x, nvec = a.cols / VEC;
   if (row >= a.rows) return;  // TPR = 32 only: whole warps
-  const T* x = static_cast<const T*>(a.x) + row * a.cols;
-  const T* res = a.res ? static_cast<const T*>(a.res) + row * a.cols : nullptr;
+  const long long base = row * a.cols;
+  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + base);
+  const uint4* res = reinterpret_cast<const uint4*>(static_cast<const T*>(a.res) + base);
+  const bool with_res = a.res != nullptr;
   float v[NV][VEC], ss = 0.0f;
-  Vec16<T> vx[NV], vr[NV];
+  uint4 vx[NV], vr[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = t + i * TPR;
     if (c < nvec) {
-      vx[i] = reinterpret_cast<const Vec16<T>*>(x)[c];
-      if (res) vr[i] = reinterpret_cast<const Vec16<T>*>(res)[c];
+      vx[i] = x[c];
+      if (with_res) vr[i] = res[c];
     }
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = t + i * TPR;
     if (c < nvec) {
-      Vec16<T> vh;
+      B::get(vx[i], v[i]);
+      if (with_res) {
+        float r[VEC];
+        B::get(vr[i], r);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[i][j] = to_f32(vx[i].v[j]) + (res ? to_f32(vr[i].v[j]) : 0.0f);
-        ss = fmaf(v[i][j], v[i][j], ss);
-        vh.v[j] = from_f32<T>(v[i][j]);
+        for (int j = 0; j < VEC; ++j) v[i][j] += r[j];
       }
-      if (a.h) reinterpret_cast<Vec16<T>*>(static_cast<T*>(a.h) + row * a.cols)[c] = vh;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+      if (a.h) reinterpret_cast<uint4*>(static_cast<T*>(a.h) + base)[c] = B::put(v[i]);
     }
   }
   ss = row_all<Sum, TPR>(ss, red[0]);
@@ -155,39 +161,42 @@ __global__ void __launch_bounds__(block_threads(TPR)) rms_norm_kernel(NormArgs a
     if (c < nvec) {
       float w[VEC];
       load_w<T>(a.w, a.w_f32, c * VEC, w);
-      Vec16<T> vy;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         v[i][j] = v[i][j] * r * w[j];
-        if constexpr (F8) top = max_nan(top, fabsf(v[i][j]));
-        else vy.v[j] = from_f32<T>(v[i][j]);
+        if constexpr (F8) top = max_nan_abs(top, v[i][j]);
       }
-      if constexpr (!F8) reinterpret_cast<Vec16<T>*>(static_cast<T*>(a.y) + row * a.cols)[c] = vy;
+      if constexpr (!F8) reinterpret_cast<uint4*>(static_cast<T*>(a.y) + base)[c] = B::put(v[i]);
     }
   }
   if constexpr (F8) {
-    if (a.group == a.cols) top = max_nan(row_all<Max, TPR>(top, red[1]), kSmallestAmax);
+    const bool whole = a.group == a.cols;
+    if (whole) {
+      top = max_nan(row_all<Max, TPR>(top, red[1]), kSmallestAmax);
+      if (t == 0) a.scale[row] = top / kE4M3Max;
+    }
     const int lanes = a.group / VEC;  // of one group (a power of two ≤ 32 unless the group is the row)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t + i * TPR;
       float m = top;
-      if (a.group != a.cols) {
+      if (!whole) {
         m = 0.0f;
         if (c < nvec) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(v[i][j]));
+          for (int j = 0; j < VEC; ++j) m = max_nan_abs(m, v[i][j]);
         }
         m = max_nan(warp_all<Max>(m, lanes), kSmallestAmax);
+        if (c < nvec && (t & (lanes - 1)) == 0) a.scale[row * (a.cols / a.group) + c / lanes] = m / kE4M3Max;
       }
       if (c < nvec) {
         const float inv = kE4M3Max / m;
-        Bytes<VEC> q;
+        uint32_t q[VEC / 4];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) q.v[j] = to_e4m3(v[i][j] * inv);
-        reinterpret_cast<Bytes<VEC>*>(a.q + row * a.cols)[c] = q;
-        const int g = c * VEC / a.group;
-        if (c * VEC == g * a.group) a.scale[row * (a.cols / a.group) + g] = m / kE4M3Max;
+        for (int j = 0; j < VEC; j += 4)
+          q[j / 4] = to_e4m3x4(v[i][j] * inv, v[i][j + 1] * inv, v[i][j + 2] * inv, v[i][j + 3] * inv);
+        if constexpr (VEC == 8) reinterpret_cast<uint2*>(a.q + base)[c] = make_uint2(q[0], q[1]);
+        else reinterpret_cast<uint32_t*>(a.q + base)[c] = q[0];
       }
     }
   }
@@ -251,40 +260,44 @@ struct NormBwdArgs {
 
 template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(block_threads(TPR)) rms_norm_bwd_kernel(NormBwdArgs a) {
-  constexpr int VEC = 16 / sizeof(T), RPB = rows_per_block(TPR);
+  using B = Bytes16<T>;
+  constexpr int VEC = B::N, RPB = rows_per_block(TPR);
   __shared__ float red[4][32];
   extern __shared__ float wsum[];  // TPR = 32: [8][cols], the warps' column sums
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x, nvec = a.cols / VEC;
   const int sub = TPR == 32 ? threadIdx.x >> 5 : 0;
+  const bool with_gh = a.grad_h != nullptr;
   float dw[NV][VEC] = {}, w[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (t + i * TPR < nvec) load_w<T>(a.w, a.w_f32, (t + i * TPR) * VEC, w[i]);
   int turn = 0;
   for (long long row = (long long)blockIdx.x * RPB + sub; row < a.rows; row += (long long)gridDim.x * RPB) {
-    const Vec16<T>* pdy = reinterpret_cast<const Vec16<T>*>(static_cast<const T*>(a.dy) + row * a.cols);
-    const Vec16<T>* ph = reinterpret_cast<const Vec16<T>*>(static_cast<const T*>(a.h) + row * a.cols);
-    const Vec16<T>* pg =
-        a.grad_h ? reinterpret_cast<const Vec16<T>*>(static_cast<const T*>(a.grad_h) + row * a.cols) : nullptr;
-    Vec16<T> dy[NV], h[NV], gh[NV];
+    const long long base = row * a.cols;
+    const uint4* pdy = reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + base);
+    const uint4* ph = reinterpret_cast<const uint4*>(static_cast<const T*>(a.h) + base);
+    const uint4* pg = reinterpret_cast<const uint4*>(static_cast<const T*>(a.grad_h) + base);
+    uint4 dy[NV], h[NV], gh[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t + i * TPR;
       if (c < nvec) {
         dy[i] = pdy[c];
         h[i] = ph[c];
-        if (pg) gh[i] = pg[c];
+        if (with_gh) gh[i] = pg[c];
       }
     }
     float ss = 0.0f, sg = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (t + i * TPR < nvec) {
+        float fd[VEC], fh[VEC];
+        B::get(dy[i], fd);
+        B::get(h[i], fh);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float fh = to_f32(h[i].v[j]);
-          ss = fmaf(fh, fh, ss);
-          sg = fmaf(to_f32(dy[i].v[j]) * w[i][j], fh, sg);
+          ss = fmaf(fh[j], fh[j], ss);
+          sg = fmaf(fd[j] * w[i][j], fh[j], sg);
         }
       }
     // the two buffers alternate, so a row's reduction never meets the previous row's readers
@@ -297,14 +310,17 @@ __global__ void __launch_bounds__(block_threads(TPR)) rms_norm_bwd_kernel(NormBw
     for (int i = 0; i < NV; ++i) {
       const int c = t + i * TPR;
       if (c < nvec) {
-        Vec16<T> o;
+        float fd[VEC], fh[VEC], o[VEC];
+        B::get(dy[i], fd);
+        B::get(h[i], fh);
+        if (with_gh) B::get(gh[i], o);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float fh = to_f32(h[i].v[j]), fd = to_f32(dy[i].v[j]);
-          o.v[j] = from_f32<T>(r * (fd * w[i][j] - fh * k) + (pg ? to_f32(gh[i].v[j]) : 0.0f));
-          dw[i][j] = fmaf(fd, fh * r, dw[i][j]);
+          const float g = r * (fd[j] * w[i][j] - fh[j] * k);
+          o[j] = with_gh ? o[j] + g : g;
+          dw[i][j] = fmaf(fd[j], fh[j] * r, dw[i][j]);
         }
-        reinterpret_cast<Vec16<T>*>(static_cast<T*>(a.dh) + row * a.cols)[c] = o;
+        reinterpret_cast<uint4*>(static_cast<T*>(a.dh) + base)[c] = B::put(o);
       }
     }
   }
@@ -362,22 +378,20 @@ __global__ void __launch_bounds__(256) rms_norm_bwd_any_kernel(NormBwdArgs a) {
   }
 }
 
-// dw[c] = Σ partial[p][c]: 8 rows of 32 threads, each its rows p ≡ ty (mod 8) in order, then the eight in order.
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ partial, float* __restrict__ dw,
-                                                         int n, int cols) {
-  __shared__ float s[8][32];
+// dw[c] = Σ partial[p][c]: 32 rows of 32 threads, each its rows p ≡ ty (mod 32) in order, then the 32 in order.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ partial, float* __restrict__ dw,
+                                                          int n, int cols) {
+  __shared__ float s[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
   float v = 0.0f;
   if (c < cols) {
-#pragma unroll 4
-    for (int p = ty; p < n; p += 8) v += partial[(long long)p * cols + c];
+#pragma unroll 8
+    for (int p = ty; p < n; p += 32) v += partial[(long long)p * cols + c];
   }
   s[ty][tx] = v;
   __syncthreads();
-  if (ty == 0 && c < cols) {
-    for (int k = 1; k < 8; ++k) v += s[k][tx];
-    dw[c] = v;
-  }
+  v = warp_all<Sum>(s[tx][ty]);  // column ty's 32 sums
+  if (tx == 0 && blockIdx.x * 32 + ty < cols) dw[blockIdx.x * 32 + ty] = v;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -390,7 +404,7 @@ NormShape norm_shape(long long rows, int nvec) {
   // Many rows: few threads a row, up to four vectors each (more loads in flight a thread, cheaper
   // reductions).  Few rows (under two blocks an SM): one vector a thread, the row's latency counts.
   const int most = rows <= 296 ? 1 : 4;
-  for (int tpr : {32, 128, 512, 1024})
+  for (int tpr : {32, 256, 512, 1024})
     if (nvec <= tpr * most) return {tpr, (nvec + tpr - 1) / tpr};
   return nvec <= 4096 ? NormShape{1024, (nvec + 1023) / 1024} : NormShape{0, 0};
 }
@@ -403,7 +417,7 @@ template <typename F> int with_shape(NormShape s, F&& f) {
   };
   switch (s.tpr) {
     case 32: return nv(std::integral_constant<int, 32>{});
-    case 128: return nv(std::integral_constant<int, 128>{});
+    case 256: return nv(std::integral_constant<int, 256>{});
     case 512: return nv(std::integral_constant<int, 512>{});
     default: return nv(std::integral_constant<int, 1024>{});
   }
@@ -475,7 +489,7 @@ template <typename T> int rms_norm_bwd(NormBwdArgs a, float* dw, void* ws, size_
   else if (nvec <= 1024) rc = go(rms_norm_bwd_kernel<T, 512, 2>, 512, 0);
   else rc = go(rms_norm_bwd_kernel<T, 512, 4>, 512, 0);
   if (rc) return rc;
-  column_sum_kernel<<<(a.cols + 31) / 32, 256, 0, st>>>(a.partial, dw, nb, a.cols);
+  column_sum_kernel<<<(a.cols + 31) / 32, 1024, 0, st>>>(a.partial, dw, nb, a.cols);
   return check_launch("rms_norm weight gradient");
 }
 

@@ -17,15 +17,14 @@
 // threads then walk (token, head) rows with 16-byte accesses, all q and k
 // heads of a token in the same block, so the sines cost 1/heads of a pair
 // each.  One launch serves q and k.
-#include <cuda_fp16.h>
-
 #include "va_common.cuh"
 
 namespace va {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kMaxTokensPerBlock = 4;
+constexpr int kBatch = 4;         // heads of a thread that are in flight together
+constexpr int kMaxAngles = 2048;  // of a block (16 KB)
 constexpr int kMaxRot = 512;
 
 template <typename T> struct RotCvt;
@@ -53,57 +52,126 @@ struct RotTensor {
   int heads;
 };
 
+// P elements ↔ f32 (16 bytes at once, or one by one).
+template <typename T, int P> __device__ __forceinline__ void widen(const Pack<T, P>& v, float (&f)[P]) {
+  if constexpr (sizeof(T) * P == 16) {
+    Bytes16<T>::get(*reinterpret_cast<const uint4*>(&v), f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) f[i] = RotCvt<T>::to(v.v[i]);
+  }
+}
+template <typename T, int P> __device__ __forceinline__ Pack<T, P> narrow(const float (&f)[P]) {
+  Pack<T, P> v;
+  if constexpr (sizeof(T) * P == 16) {
+    *reinterpret_cast<uint4*>(&v) = Bytes16<T>::put(f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) v.v[i] = RotCvt<T>::from(f[i]);
+  }
+  return v;
+}
+
 // P pairs (or P copied elements) per thread and row; P·sizeof(T) ≤ 16.
+// Threads: x walks a head's chunks, y the heads, z the block's tokens, so a
+// thread's (cos, sin) pairs stay in registers over its heads.  Its first
+// kBatch heads are read before the angles are computed: the loads do not
+// depend on them, and the angles' latency hides theirs.
 template <typename T, int P, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRotThreads)
 rotary_kernel(RotTensor q, RotTensor k, const void* __restrict__ positions, int pos64,
-              const double* __restrict__ inv_freq, int tokens, int tpb, int dim, int rot, float factor,
-              float sin_sign) {
-  __shared__ float2 cs[kMaxTokensPerBlock * (kMaxRot / 2)];
-  const int half = rot / 2, t0 = blockIdx.x * tpb, nt = min(tpb, tokens - t0);
-  const int tid = threadIdx.y * blockDim.x + threadIdx.x, nthreads = blockDim.x * blockDim.y;
+              const double* __restrict__ inv_freq, int tokens, int dim, int rot, float factor, float sin_sign) {
+  extern __shared__ float2 cs[];  // [tokens of the block][rot / 2]
+  using V = Pack<T, P>;
+  const int half = rot / 2, t0 = blockIdx.x * blockDim.z, t = t0 + threadIdx.z, nt = min((int)blockDim.z, tokens - t0);
+  const int tid = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + threadIdx.x;
+  const int nthreads = blockDim.x * blockDim.y * blockDim.z;
+  const int heads = t < tokens ? q.heads + k.heads : 0, nrot = half / P, nchunk = nrot + (dim - rot) / P;
+  const T *q_in = static_cast<const T*>(q.in) + t * q.in_row, *k_in = static_cast<const T*>(k.in) + t * k.in_row;
+  T *q_out = static_cast<T*>(q.out) + t * q.out_row, *k_out = static_cast<T*>(k.out) + t * k.out_row;
+  auto in_of = [&](int h) { return h < q.heads ? q_in + h * q.in_head : k_in + (h - q.heads) * k.in_head; };
+  auto out_of = [&](int h) { return h < q.heads ? q_out + h * q.out_head : k_out + (h - q.heads) * k.out_head; };
+  // the chunk's first and second vector (a copied chunk has only the first)
+  auto at = [&](int c, int& ia, int& ib) {
+    ia = c >= nrot ? rot + (c - nrot) * P : INTERLEAVED ? 2 * P * c : P * c;
+    ib = INTERLEAVED ? ia + P : ia + half;
+  };
+  auto turn = [&](V& a, V& b, const float2 (&w)[P]) {
+    float fa[P], fb[P];
+    widen<T, P>(a, fa);
+    widen<T, P>(b, fb);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      // the pair's two elements: a[i], b[i], or (interleaved) neighbours of the 2P elements (a, b)
+      float& xa = INTERLEAVED ? (2 * i < P ? fa[(2 * i) % P] : fb[(2 * i) % P]) : fa[i];
+      float& xb = INTERLEAVED ? (2 * i + 1 < P ? fa[(2 * i + 1) % P] : fb[(2 * i + 1) % P]) : fb[i];
+      const float ya = xa * w[i].x - xb * w[i].y, yb = xa * w[i].y + xb * w[i].x;
+      xa = ya;
+      xb = yb;
+    }
+    a = narrow<T, P>(fa);
+    b = narrow<T, P>(fb);
+  };
+
+  V va[kBatch], vb[kBatch];
+  const int c0 = threadIdx.x;  // < nchunk
+  int ia, ib;
+  at(c0, ia, ib);
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    const int h = threadIdx.y + i * blockDim.y;
+    if (h < heads) {
+      const T* in = in_of(h);
+      va[i] = *reinterpret_cast<const V*>(in + ia);
+      if (c0 < nrot) vb[i] = *reinterpret_cast<const V*>(in + ib);
+    }
+  }
   for (int i = tid; i < nt * half; i += nthreads) {
-    const int t = i / half, f = i - t * half;
-    const double pos = pos64 ? (double)static_cast<const long long*>(positions)[t0 + t]
-                             : (double)static_cast<const int*>(positions)[t0 + t];
+    const int ti = i / half, f = i - ti * half;
+    const double pos = pos64 ? (double)static_cast<const long long*>(positions)[t0 + ti]
+                             : (double)static_cast<const int*>(positions)[t0 + ti];
     const double turns = pos * (inv_freq[f] * 0.15915494309189533577);  // 1 / 2π
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     cs[i] = make_float2(factor * c, sin_sign * factor * s);
   }
   __syncthreads();
-
-  using V = Pack<T, P>;
-  const int heads = q.heads + k.heads, nrot = half / P, nchunk = nrot + (dim - rot) / P;
-  for (int c = threadIdx.x; c < nchunk; c += blockDim.x) {
-#pragma unroll 2
-    for (int r = threadIdx.y; r < nt * heads; r += blockDim.y) {
-      const int t = r / heads, h = r - t * heads;
-      const bool is_q = h < q.heads;
-      const RotTensor& x = is_q ? q : k;
-      const int hx = is_q ? h : h - q.heads;
-      const T* in = static_cast<const T*>(x.in) + (t0 + t) * x.in_row + hx * x.in_head;
-      T* out = static_cast<T*>(x.out) + (t0 + t) * x.out_row + hx * x.out_head;
-      if (c >= nrot) {
-        const int d = rot + (c - nrot) * P;
-        *reinterpret_cast<V*>(out + d) = *reinterpret_cast<const V*>(in + d);
-        continue;
-      }
-      const int ia = INTERLEAVED ? 2 * P * c : P * c, ib = INTERLEAVED ? ia + P : ia + half;
-      V a = *reinterpret_cast<const V*>(in + ia), b = *reinterpret_cast<const V*>(in + ib);
-      const float2* w = cs + t * half + c * P;
+  float2 w[P];
+  auto angles = [&](int c) {
+    if (c < nrot) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        // the pair's two elements: a[i], b[i], or (interleaved) neighbours of the 2P elements (a, b)
-        T& ta = INTERLEAVED ? (2 * i < P ? a.v[(2 * i) % P] : b.v[(2 * i) % P]) : a.v[i];
-        T& tb = INTERLEAVED ? (2 * i + 1 < P ? a.v[(2 * i + 1) % P] : b.v[(2 * i + 1) % P]) : b.v[i];
-        const float fa = RotCvt<T>::to(ta), fb = RotCvt<T>::to(tb);
-        const float2 z = w[i];
-        ta = RotCvt<T>::from(fa * z.x - fb * z.y);
-        tb = RotCvt<T>::from(fa * z.y + fb * z.x);
+      for (int i = 0; i < P; ++i) w[i] = cs[threadIdx.z * half + c * P + i];
+    }
+  };
+  angles(c0);
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    const int h = threadIdx.y + i * blockDim.y;
+    if (h < heads) {
+      T* out = out_of(h);
+      if (c0 < nrot) {
+        turn(va[i], vb[i], w);
+        *reinterpret_cast<V*>(out + ib) = vb[i];
+      }
+      *reinterpret_cast<V*>(out + ia) = va[i];
+    }
+  }
+  // what is left: more heads than a batch, heads of more chunks than threads
+  for (int c = c0; c < nchunk; c += blockDim.x) {
+    if (c > c0) {
+      at(c, ia, ib);
+      angles(c);
+    }
+    for (int h = threadIdx.y + (c == c0 ? kBatch * blockDim.y : 0); h < heads; h += blockDim.y) {
+      const T* in = in_of(h);
+      T* out = out_of(h);
+      V a = *reinterpret_cast<const V*>(in + ia);
+      if (c < nrot) {
+        V b = *reinterpret_cast<const V*>(in + ib);
+        turn(a, b, w);
+        *reinterpret_cast<V*>(out + ib) = b;
       }
       *reinterpret_cast<V*>(out + ia) = a;
-      *reinterpret_cast<V*>(out + ib) = b;
     }
   }
 }
@@ -138,13 +206,18 @@ int rotary(RotTensor q, RotTensor k, const void* positions, int position_bytes, 
   const RotTensor both[2] = {q, k};
   const int p = pick_pack(both, k.heads ? 2 : 1, (int)sizeof(T), dim, rot);
   const int nchunk = rot / 2 / p + (dim - rot) / p;
-  const int bx = std::min(nchunk, kRotThreads), by = kRotThreads / bx;
-  // several tokens a block once there are blocks enough for every SM (the sines of a token cost one pass anyway)
-  const int tpb = tokens >= 148 * 8 * kMaxTokensPerBlock ? kMaxTokensPerBlock : tokens >= 148 * 16 ? 2 : 1;
-  const dim3 block(bx, by), grid((tokens + tpb - 1) / tpb);
+  // A batch of heads a thread where there are tokens enough to fill the SMs with such blocks, else one; tokens fill
+  // what is left of a block (their angles fit its shared memory).
+  const int heads = q.heads + k.heads, bx = std::min(nchunk, kRotThreads);
+  const int per_thread = tokens >= 148 * 8 ? kBatch : 1;
+  const int by = std::max(1, std::min(kRotThreads / bx, (heads + per_thread - 1) / per_thread));
+  const int bz = std::max(1, std::min(std::min(kRotThreads / (bx * by), kMaxAngles / std::max(rot / 2, 1)),
+                                      std::min(64, ceil_div(tokens, 148 * 4))));
+  const dim3 block(bx, by, bz), grid(ceil_div(tokens, bz));
+  const size_t smem = (size_t)bz * (rot / 2) * sizeof(float2);
   auto go = [&](auto kernel) -> int {
-    kernel<<<grid, block, 0, st>>>(q, k, positions, position_bytes == 8, inv_freq, tokens, tpb, dim, rot, factor,
-                                   backward ? -1.0f : 1.0f);
+    kernel<<<grid, block, smem, st>>>(q, k, positions, position_bytes == 8, inv_freq, tokens, dim, rot, factor,
+                                      backward ? -1.0f : 1.0f);
     return check_launch("rotary");
   };
   switch (p) {
