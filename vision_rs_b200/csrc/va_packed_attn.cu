@@ -19,8 +19,9 @@
 // reference) back into the same columns as 16-bit P, O += P·V with P as the
 // TMEM operand.  The reference only follows the row maximum when it grows by
 // more than 2^8, so O is rarely rescaled.  P is held in the inputs' 16-bit
-// type: its rounding adds about as much error as that of the output; sums,
-// maxima and O stay f32.
+// type (rows of at most 128 keys: with its remainder as a second operand); its
+// rounding adds about as much error as that of the output.  Sums, maxima and
+// O stay f32.
 //
 // Rows of other sequences that a tile's boxes bring in: scores of keys past
 // the end are replaced, not added to; V rows past the last key that the unit sees are zeroed in
@@ -44,6 +45,9 @@ namespace {
 constexpr int kHalf = 64;  // keys of a score step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.0f;  // the reference follows the maximum once it is 2^8 ahead
+// Rows of at most this many 64-key steps hold P as two 16-bit words, value and remainder, and multiply V by both: there the
+// second product costs nothing that is measured, and the output is exact to its own rounding.
+constexpr int kFineSteps = 2;
 constexpr float kF16Shift = 7.0f;   // f16: P is held times 2^7 (at most 2^15), so small ones keep their bits
 
 // DP: head size in shared memory and TMEM (64 or 128; the TMA boxes fill what is past `dim` with zeros).
@@ -75,10 +79,6 @@ struct FwdArgs {
   float scale;  // softmax scale · log2 e
 };
 
-template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF16) return pack_bf16x2(a, b);
-  else return pack_f16x2(a, b);
-}
 
 template <int DP, int TILES, bool BF16>
 __global__ void __launch_bounds__(FwdCfg<DP, TILES>::kThreads, FwdCfg<DP, TILES>::kCtas)
@@ -226,6 +226,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         mma_commit_p(&sm.s_full[m][h & 1], lead);
       };
+      const bool fine = n <= kFineSteps;
       // Both tiles' threads wait for every K and V slot and release it, also where their own tile has no step left.
       int sk = 0, sv = 1;          // ring slots of the K block ahead and of this step's V block, and their parities
       uint32_t pk = 0, pv = 0;
@@ -254,13 +255,15 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           const uint64_t dv = dv0 + (uint64_t)(sv * kSlot + r * kHalfRows);
           const uint32_t tp = ts + r * kHalf;
           const int ks = last ? min(kHalf / 16, (used_last - r * kHalf + 15) >> 4) : kHalf / 16;
-          if (ks == kHalf / 16) {
+          if (ks == kHalf / 16 && !fine) {
 #pragma unroll
             for (int s = 0; s < kHalf / 16; ++s)
               mma_ts_p(to, tp + s * 8, dv + (uint64_t)(s * (2048 >> 4)), idesc_o, (h > 0 || s > 0) ? 1u : 0u, lead);
           } else {
             for (int s = 0; s < ks; ++s)
               mma_ts_p(to, tp + s * 8, dv + (uint64_t)(s * (2048 >> 4)), idesc_o, (h > 0 || s > 0) ? 1u : 0u, lead);
+            for (int s = 0; fine && s < ks; ++s)
+              mma_ts_p(to, tp + 32 + s * 8, dv + (uint64_t)(s * (2048 >> 4)), idesc_o, 1u, lead);
           }
           mma_commit_p(&sm.o_done[m][r], lead);
         }
@@ -355,9 +358,9 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       return true;
     };
     float part[4];
-    auto exps = [&](int h, const uint32_t (&u)[32], int c) {  // P of 32 keys
+    auto exps = [&](int h, const uint32_t (&u)[32], int c, auto fine) {  // P of 32 keys
       const float base = ref == -INFINITY ? 0.0f : BF16 ? ref : ref - kF16Shift;
-      uint32_t p[16];
+      uint32_t p[16], rest[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float p0, p1;
@@ -366,8 +369,10 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         p1 = ex2(p1);
         fadd2(part[2 * (i & 1)], part[2 * (i & 1) + 1], p0, p1);
         p[i] = pack2<BF16>(p0, p1);
+        if constexpr (decltype(fine)::value) rest[i] = pack2_rest<BF16>(p[i], p0, p1);
       }
       tmem_st16(ts + (h & 1) * kHalf + c * 16, p);
+      if constexpr (decltype(fine)::value) tmem_st16(ts + (h & 1) * kHalf + 32 + c * 16, rest);
     };
     auto give = [&](int h) {
       sum += (part[0] + part[1]) + (part[2] + part[3]);
@@ -380,16 +385,20 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if ((ok = mbar_wait(&sm.s_full[m][h & 1], (h >> 1) & 1, &sm.abort, &g_packed_status, 8)))
           mbar_arrive(&sm.p_full[m][h & 1]);
     } else {
-      for (int h = 0; h < n; ++h) {
-        uint32_t u[2][32];
-        if (!(ok = fetch(h, u))) break;
-        const float top = top_of(h, u);
-        if (!(ok = follow(h, top))) break;
-        part[0] = part[1] = part[2] = part[3] = 0.0f;
-        exps(h, u[0], 0);
-        exps(h, u[1], 1);
-        give(h);
-      }
+      auto steps_of = [&](auto fine) {
+        for (int h = 0; h < n; ++h) {
+          uint32_t u[2][32];
+          if (!(ok = fetch(h, u))) break;
+          const float top = top_of(h, u);
+          if (!(ok = follow(h, top))) break;
+          part[0] = part[1] = part[2] = part[3] = 0.0f;
+          exps(h, u[0], 0, fine);
+          exps(h, u[1], 1, fine);
+          give(h);
+        }
+      };
+      if (n <= kFineSteps) steps_of(std::true_type{});
+      else steps_of(std::false_type{});
     }
     // ── output ──
     if (ok && n > 0) ok = mbar_wait(&sm.o_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, &sm.abort, &g_packed_status, 10);

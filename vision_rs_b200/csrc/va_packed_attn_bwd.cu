@@ -8,13 +8,14 @@
 // launches, no atomics, so the results do not depend on scheduling:
 //
 //   row kernel   (lse·log2 e, Δ) of every query and head
-//   dK/dV kernel a CTA per (128 keys, key head) walks the group's heads and
-//                their queries in steps of 64: Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ in
-//                TMEM, Pᵀ and dSᵀ back into the same columns in 16 bits, then
-//                dV += Pᵀ·dO, dK += dSᵀ·Q with the TMEM operand
 //   dQ kernel    a CTA per (128 queries, head) walks the keys in steps of 64:
 //                S = Q·Kᵀ, dP = dO·Vᵀ with Q and dO as TMEM operands, dS in
 //                TMEM, dQ += dS·K
+//   dK/dV kernel a CTA per (128 keys, key head) walks the group's heads and
+//                their queries in steps of 64: Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ in
+//                TMEM, Pᵀ and dSᵀ back into the same columns in 16 bits, then
+//                dV += Pᵀ·dO, dK += dSᵀ·Q with the TMEM operand; long ranges are
+//                split over CTAs and joined by the last, in order
 //
 // S and dP are computed twice (7 products instead of 5); the one-kernel form
 // would add f32 dQ partials to memory from every key tile, in an order that
@@ -49,6 +50,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kHalf = 64;     // queries (or keys) a step
 constexpr int kStages = 4;    // ring of 64-row (Q, dO) or (K, V) pairs
 constexpr int kThreads = 352; // 2 × 4 warps of scores, 1 TMA, 1 to issue the scores' MMAs, 1 the gradients'
+// Sequences of at most this many 64-row steps hold P and dS as two 16-bit words, value and remainder, and multiply by both:
+// there the second products cost nothing that is measured, and the gradients are exact to their own rounding.
+constexpr int kFineSteps = 2;
 constexpr float kPShift = 15.0f;     // f16: P is held times 2^15
 constexpr uint32_t kColAcc = 256;    // score buffers at 0 (S 64, dP 64) and 128; accumulators from here
 
@@ -58,6 +62,7 @@ template <int DP> struct BwdSmem {
   uint8_t ring[kStages][2][kStep];   // per 64 dims 64 rows × 128 bytes
   float4 stats[2][2][2][kHalf / 4];  // dK/dV: −lse·log2 e and −Δ of the step's queries, per group, two steps
   float red[8];
+  float row_part[2][kPackBlock];     // dQ: Σ P·dP over a group's keys
   uint64_t a_full, a_ready, full[kStages], empty[kStages], s_full[2], p_full[2], g_done[2], fin;
   uint32_t tmem_base;
   int abort, last;
@@ -71,10 +76,6 @@ struct BwdArgs {
   float scale;
 };
 
-template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF16) return pack_bf16x2(a, b);
-  else return pack_f16x2(a, b);
-}
 // The four warps of a score group meet; one that gives up arrives without waiting.
 __device__ __forceinline__ void group_leave(int g) { asm volatile("bar.arrive %0, 128;" ::"r"(g + 1) : "memory"); }
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
@@ -267,6 +268,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   // 64-query blocks of a head from the first that sees a key of the tile, and the unit's steps (block b0 of head g0 first)
   const int hb0 = ps.causal ? max(0, it.j0 - (it.lk - it.lq)) / kHalf : 0, nh = max(0, (it.lq + kHalf - 1) / kHalf - hb0);
   const int n = it.h1 - it.h0, g0 = nh > 0 ? it.h0 / nh : 0, b0 = it.h0 - g0 * nh;
+  const bool fine = it.lq <= kFineSteps * kHalf;
   const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
 
   if (warp == 8) {
@@ -331,6 +333,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   } else if (warp == 10) {
     // ── dV += Pᵀ·dO, dK += dSᵀ·Q ──
     if (n > 0) {
+      const bool uniform_fine = uniform(fine);
       const uint32_t lead = elect_lead(), tm = uniform(tmem);
       const int steps = uniform(n), blocks = uniform(nh), tail = uniform(it.lq - (hb0 + nh - 1) * kHalf);
       const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, BF16 ? AB_BF16 : AB_F16, false, true);
@@ -351,11 +354,15 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           mma_ts_p(tm + kColAcc, tp + s * 8, go + (uint64_t)(s * (2048 >> 4)), id_g, acc, lead);
           mma_ts_p(tm + kColAcc + DP, tp + kHalf + s * 8, gq + (uint64_t)(s * (2048 >> 4)), id_g, acc, lead);
         };
-        if (ks == kHalf / 16) {
+        if (ks == kHalf / 16 && !uniform_fine) {
 #pragma unroll
           for (int s = 0; s < kHalf / 16; ++s) one(s);
         } else {
           for (int s = 0; s < ks; ++s) one(s);
+          for (int s = 0; uniform_fine && s < ks; ++s) {
+            mma_ts_p(tm + kColAcc, tp + 32 + s * 8, go + (uint64_t)(s * (2048 >> 4)), id_g, 1u, lead);
+            mma_ts_p(tm + kColAcc + DP, tp + kHalf + 32 + s * 8, gq + (uint64_t)(s * (2048 >> 4)), id_g, 1u, lead);
+          }
         }
         mma_commit_p(&sm.g_done[h & 1], lead);
         mma_commit_p(&sm.empty[st], lead);
@@ -440,47 +447,91 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       tc_fence_after();
       const float4 *nl = sm.stats[g][k & 1][0], *nd = sm.stats[g][k & 1][1];
       // 16 queries at a time: their statistics are read while the scores come
+      struct Chunk {
+        uint32_t s[16], d[16];
+      };
+      struct Stats {
+        float4 l[4], e[4];
+      };
+      auto fetch16 = [&](int c, Chunk& x) {
+        tmem_ld16(ts + c * 16, x.s);
+        tmem_ld16(ts + kHalf + c * 16, x.d);
+      };
+      auto stats16 = [&](int c) {
+        Stats x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.l[i] = nl[c * 4 + i], x.e[i] = nd[c * 4 + i];
+        return x;
+      };
+      auto scores16 = [&](int c, const Chunk& x, const Stats& y, auto masked, auto with_rest) {
+        uint32_t pp[8], pd[8], rp[8], rd[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 &lf = y.l[i >> 1], &ef = y.e[i >> 1];
+          float p0, p1, d0 = __uint_as_float(x.d[2 * i]), d1 = __uint_as_float(x.d[2 * i + 1]);
+          ffma2(p0, p1, __uint_as_float(x.s[2 * i]), __uint_as_float(x.s[2 * i + 1]), scale2, scale2,
+                i & 1 ? lf.z : lf.x, i & 1 ? lf.w : lf.y);
+          fadd2(d0, d1, i & 1 ? ef.z : ef.x, i & 1 ? ef.w : ef.y);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          fmul2(d0, d1, p0, p1);
+          if constexpr (decltype(masked)::value) {
+            const int q0 = c * 16 + 2 * i, q1 = q0 + 1;
+            const bool v0 = q0 >= lo && q0 < hi, v1 = q1 >= lo && q1 < hi;
+            p0 = v0 ? p0 : 0.0f;
+            d0 = v0 ? d0 : 0.0f;
+            p1 = v1 ? p1 : 0.0f;
+            d1 = v1 ? d1 : 0.0f;
+          }
+          if constexpr (!BF16) fmul2(d0, d1, mult_p, mult_p);
+          pp[i] = pack2<BF16>(p0, p1);
+          pd[i] = pack2<BF16>(d0, d1);
+          if constexpr (decltype(with_rest)::value) {
+            rp[i] = pack2_rest<BF16>(pp[i], p0, p1);
+            rd[i] = pack2_rest<BF16>(pd[i], d0, d1);
+          }
+        }
+        tmem_st8(ts + c * 8, pp);
+        tmem_st8(ts + kHalf + c * 8, pd);
+        if constexpr (decltype(with_rest)::value) {
+          tmem_st8(ts + 32 + c * 8, rp);
+          tmem_st8(ts + kHalf + 32 + c * 8, rd);
+        }
+      };
+      auto arrived = [&](Chunk& x) {
+        reg_fence(x.s);
+        reg_fence(x.d);
+      };
       auto scores = [&](auto masked) {
 #pragma unroll
         for (int c = 0; c < kHalf / 16; ++c) {
-          uint32_t s[16], d[16];
-          float4 l[4], e[4];
-          tmem_ld16(ts + c * 16, s);
-          tmem_ld16(ts + kHalf + c * 16, d);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) l[i] = nl[c * 4 + i], e[i] = nd[c * 4 + i];
+          Chunk x;
+          fetch16(c, x);
+          const Stats y = stats16(c);
           tmem_ld_wait();
-          reg_fence(s);
-          reg_fence(d);
-          uint32_t pp[8], pd[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 &lf = l[i >> 1], &ef = e[i >> 1];
-            float p0, p1, d0 = __uint_as_float(d[2 * i]), d1 = __uint_as_float(d[2 * i + 1]);
-            ffma2(p0, p1, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), scale2, scale2, i & 1 ? lf.z : lf.x,
-                  i & 1 ? lf.w : lf.y);
-            fadd2(d0, d1, i & 1 ? ef.z : ef.x, i & 1 ? ef.w : ef.y);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
-            fmul2(d0, d1, p0, p1);
-            if constexpr (decltype(masked)::value) {
-              const int q0 = c * 16 + 2 * i, q1 = q0 + 1;
-              const bool v0 = q0 >= lo && q0 < hi, v1 = q1 >= lo && q1 < hi;
-              p0 = v0 ? p0 : 0.0f;
-              d0 = v0 ? d0 : 0.0f;
-              p1 = v1 ? p1 : 0.0f;
-              d1 = v1 ? d1 : 0.0f;
-            }
-            if constexpr (!BF16) fmul2(d0, d1, mult_p, mult_p);
-            pp[i] = pack2<BF16>(p0, p1);
-            pd[i] = pack2<BF16>(d0, d1);
-          }
-          tmem_st8(ts + c * 8, pp);
-          tmem_st8(ts + kHalf + c * 8, pd);
+          arrived(x);
+          scores16(c, x, y, masked, std::false_type{});
         }
       };
-      if (__all_sync(0xffffffffu, whole)) scores(std::false_type{});
-      else scores(std::true_type{});
+      if (fine) {  // the remainders of chunk c take the columns of scores c / 2 + 2: those are read first
+        Chunk even, odd;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          Chunk x, &later = c ? odd : even;
+          fetch16(c, x);
+          fetch16(c + 2, later);
+          tmem_ld_wait();
+          arrived(x);
+          arrived(later);
+          scores16(c, x, stats16(c), std::true_type{}, std::true_type{});
+        }
+        scores16(2, even, stats16(2), std::true_type{}, std::true_type{});
+        scores16(3, odd, stats16(3), std::true_type{}, std::true_type{});
+      } else if (__all_sync(0xffffffffu, whole)) {
+        scores(std::false_type{});
+      } else {
+        scores(std::true_type{});
+      }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.p_full[g]);
@@ -636,11 +687,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           mma_ts_p(tm + kColAcc, tm + (h & 1) * 128 + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g,
                    (h > 0 || s > 0) ? 1u : 0u, lead);
         };
-        if (ks == kHalf / 16) {
+        if (ks == kHalf / 16 && steps > kFineSteps) {
 #pragma unroll
           for (int s = 0; s < kHalf / 16; ++s) one(s);
         } else {
           for (int s = 0; s < ks; ++s) one(s);
+          for (int s = 0; steps <= kFineSteps && s < ks; ++s)
+            mma_ts_p(tm + kColAcc, tm + (h & 1) * 128 + kHalf + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g, 1u, lead);
         }
         mma_commit_p(&sm.g_done[h & 1], lead);
         mma_commit_p(&sm.empty[st], lead);
@@ -689,11 +742,14 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         mbar_arrive(&sm.a_ready);
       }
     }
-    for (int h = g; ok && h < n; h += 2) {
-      if (!(ok = mbar_wait(&sm.s_full[g], (h >> 1) & 1, &sm.abort, &g_packed_bwd_status, 18))) break;
-      tc_fence_after();
-      const int limit = see - h * kHalf;
-      auto scores = [&](auto masked) {
+    if (ok && n > 0 && n <= kFineSteps) {
+      // Rows that see at most 128 keys: all their scores are in the two buffers, so Δ_i = Σ_j P_ij dP_ij is summed from
+      // them.  dO·O carries the rounding of the stored O, which matters here (O is an average of few values): it
+      // would add as much error to dQ and dK as the rounding of dS.  The dK/dV kernel reads the better Δ too.
+      float t = 0.0f;
+      if (g < n && (ok = mbar_wait(&sm.s_full[g], 0, &sm.abort, &g_packed_bwd_status, 20))) {
+        tc_fence_after();
+        const int limit = see - g * kHalf;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t s[32], d[32];
@@ -702,7 +758,37 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tmem_ld_wait();
           reg_fence(s);
           reg_fence(d);
-          uint32_t pd[16];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float p = ex2(fmaf(__uint_as_float(s[i]), scale2, -stat.x)) * __uint_as_float(d[i]);
+            t += c * 32 + i < limit ? p : 0.0f;
+          }
+        }
+      }
+      sm.row_part[g][row] = t;
+      if (ok) {
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        ok = !*(volatile int*)&sm.abort;
+      } else {
+        asm volatile("bar.arrive 3, 256;" ::: "memory");
+      }
+      stat.y = sm.row_part[0][row] + sm.row_part[1][row];
+      if (mine && ok && g == 0) reinterpret_cast<float2*>(a.plan + ps.rows)[at].y = stat.y;
+    }
+    for (int h = g; ok && h < n; h += 2) {
+      if (!(ok = mbar_wait(&sm.s_full[g], (h >> 1) & 1, &sm.abort, &g_packed_bwd_status, 18))) break;
+      tc_fence_after();
+      const int limit = see - h * kHalf;
+      auto scores = [&](auto masked, auto fine) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32], d[32];
+          tmem_ld32(ts + c * 32, s);
+          tmem_ld32(ts + kHalf + c * 32, d);
+          tmem_ld_wait();
+          reg_fence(s);
+          reg_fence(d);
+          uint32_t pd[16], rest[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float p0, p1, d0 = __uint_as_float(d[i]), d1 = __uint_as_float(d[i + 1]);
@@ -715,12 +801,15 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
             if constexpr (!BF16) fmul2(d0, d1, mult, mult);
             pd[i >> 1] = pack2<BF16>(d0, d1);
+            if constexpr (decltype(fine)::value) rest[i >> 1] = pack2_rest<BF16>(pd[i >> 1], d0, d1);
           }
           tmem_st16(ts + c * 16, pd);
+          if constexpr (decltype(fine)::value) tmem_st16(ts + kHalf + c * 16, rest);
         }
       };
-      if (__all_sync(0xffffffffu, limit >= kHalf)) scores(std::false_type{});
-      else scores(std::true_type{});
+      if (n <= kFineSteps) scores(std::true_type{}, std::true_type{});
+      else if (__all_sync(0xffffffffu, limit >= kHalf)) scores(std::false_type{}, std::false_type{});
+      else scores(std::true_type{}, std::false_type{});
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.p_full[g]);
@@ -757,13 +846,13 @@ template <int DP, bool BF16> int launch_bwd(const BwdMaps& m, const BwdArgs& a, 
     return rc;
   const long long g1 = (long long)a.s.max_dkv_items * a.s.kv_heads, g2 = (long long)a.s.max_dq_items * a.s.heads;
   VA_CHECK_ARG(g1 < (1LL << 31) && g2 < (1LL << 31), "packed attention backward: too many units");
-  if (g1 > 0) {
-    packed_dkv_kernel<DP, BF16><<<(unsigned)g1, kThreads, smem, st>>>(m.q_step, m.do_step, m.k_tile, m.v_tile, a);
-    if (int rc = check_launch("packed attention dK/dV")) return rc;
-  }
   if (g2 > 0) {
     packed_dq_kernel<DP, BF16><<<(unsigned)g2, kThreads, smem, st>>>(m.q_tile, m.do_tile, m.k_step, m.v_step, a);
     if (int rc = check_launch("packed attention dQ")) return rc;
+  }
+  if (g1 > 0) {
+    packed_dkv_kernel<DP, BF16><<<(unsigned)g1, kThreads, smem, st>>>(m.q_step, m.do_step, m.k_tile, m.v_tile, a);
+    if (int rc = check_launch("packed attention dK/dV")) return rc;
   }
   return VA_OK;
 }

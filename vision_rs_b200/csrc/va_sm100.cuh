@@ -316,6 +316,20 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
+// Two f32 values as two 16-bit words and what those leave out, as two more.
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) return pack_bf16x2(a, b);
+  else return pack_f16x2(a, b);
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack2_rest(uint32_t w, float a, float b) {
+  if constexpr (BF16) {
+    return pack_bf16x2(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pack_f16x2(a - f.x, b - f.y);
+  }
+}
+
 // 2^x on the FMA pipe, to share the exponential work with the MUFU unit.
 // Cody–Waite range reduction x = n + f (n integer, |f| ≤ 1/2; the rounding
 // uses the 1.5·2^23 magic-number addition), then a degree-4 polynomial for
