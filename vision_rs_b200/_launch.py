@@ -12,6 +12,7 @@ import torch
 from . import _lib
 
 raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t of torch's current stream
+_current_device = torch._C._cuda_getDevice
 _entries: dict = {}
 
 
@@ -26,7 +27,7 @@ def entry(name: str):
 def run(name: str, index: int, *args) -> None:
     """Calls ``name(*args, stream)`` on torch's current stream of device ``index``; raises on a non-zero status."""
     fn = _entries.get(name) or entry(name)
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = fn(*args, raw_stream(index))
     else:
         with torch.cuda.device(index):

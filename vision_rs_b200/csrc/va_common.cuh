@@ -32,6 +32,30 @@ inline int check_launch(const char* what) {
   return VA_OK;
 }
 
+// Launches a kernel that may be set up while the previous one of the stream
+// still runs its last blocks (programmatic dependent launch).  Such a kernel
+// calls wait_for_previous() before its first access to global memory, which
+// returns once all earlier work of the stream is complete and visible; the
+// previous kernel may call let_next_start() at any time.
+template <typename... P, typename... A>
+int launch_behind(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  count_launch();
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(VA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  }
+  return VA_OK;
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // One-time set-up that must run once on every device, such as
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize), which applies to the
 // current device only.  run(f) calls f() with the calling thread's current

@@ -13,6 +13,9 @@
 namespace va {
 
 constexpr int kPackBlock = 128;   // keys (and rows of a tile) a step
+// A tile is cut into parts of at least so many key blocks (forward) or query steps (dK/dV): smaller ones cost more to join
+// than they save (a forward block takes ~1 us, joining ~4 us).
+constexpr int kMinKeyBlocks = 6, kMinQuerySteps = 32;
 constexpr int kMaxSeqs = 1 << 20;
 constexpr int kPlanSeqs = 2048;   // sequences whose tile counts fit the plan kernel's shared memory
 
@@ -76,12 +79,20 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   s.q_tile = s.few ? kPackBlock / s.group : 2 * kPackBlock;
   s.units = s.few ? kv_heads : heads;
   s.max_tiles = (int)std::min<long long>((total_q + s.q_tile - 1) / s.q_tile + (long long)num_seqs, total_q);
-  s.split_budget = s.few ? (592 + s.units - 1) / s.units : 0;
+  // Parts over the number of tiles: enough for four units an SM slot, and no more than the longest possible tiles allow
+  // (none where no tile can pass the smallest part).
+  auto budget = [](int most, long long tiles, long long longest, int smallest) {
+    return longest <= smallest ? 0 : (int)std::min<long long>(most, (tiles * longest + smallest - 1) / smallest);
+  };
+  s.split_budget =
+      s.few ? budget((592 + s.units - 1) / s.units, s.max_tiles, ((long long)total_k + 127) / 128, kMinKeyBlocks) : 0;
   s.max_items = s.max_tiles + s.split_budget;
   s.max_slots = 2 * s.split_budget;
   s.max_dq_items = training ? (int)std::min<long long>((total_q + 127) / 128 + (long long)num_seqs, total_q) : 0;
   s.max_dkv_tiles = training ? (int)std::min<long long>((total_k + 127) / 128 + (long long)num_seqs, total_k) : 0;
-  s.dkv_budget = training ? (296 + kv_heads - 1) / kv_heads : 0;
+  s.dkv_budget = training ? budget((296 + kv_heads - 1) / kv_heads, s.max_dkv_tiles,
+                                   ((long long)total_q + 63) / 64 * s.group, kMinQuerySteps)
+                          : 0;
   s.max_dkv_items = s.max_dkv_tiles + s.dkv_budget;
   size_t o = 256;
   s.items = o, o += pk_align((size_t)s.max_items * sizeof(QItem));

@@ -89,6 +89,8 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   FwdSmem<DP, TILES>& sm = *reinterpret_cast<FwdSmem<DP, TILES>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PackedShape& ps = a.s;
+  let_next_start();
+  wait_for_previous();
   const int unit = blockIdx.x / ps.units, head = blockIdx.x - unit * ps.units;
   if (unit >= reinterpret_cast<const int*>(a.plan)[kHdrItems]) return;
   const QItem it = reinterpret_cast<const QItem*>(a.plan + ps.items)[unit];
@@ -551,8 +553,7 @@ int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
     return rc;
   const long long grid = (long long)a.s.max_items * a.s.units;
   VA_CHECK_ARG(grid < (1LL << 31), "packed attention: too many units");
-  kernel<<<(unsigned)grid, C::kThreads, smem, st>>>(mq, mk, mv, a);
-  return check_launch("packed attention");
+  return launch_behind("packed attention", kernel, (unsigned)grid, C::kThreads, smem, st, mq, mk, mv, a);
 }
 
 template <bool BF16>

@@ -212,6 +212,8 @@ packed_rows_kernel(const uint16_t* __restrict__ out, const uint16_t* __restrict_
                    long long do_head, const uint16_t* __restrict__ v, long long v_row, long long v_head,
                    const float* __restrict__ lse, float2* __restrict__ pairs, float* __restrict__ do_norm,
                    float* __restrict__ v_norm, int total_q, int total_k, int heads, int kv_heads, int dim) {
+  let_next_start();
+  wait_for_previous();
   const long long r = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), nq = (long long)total_q * heads;
   const int c = (threadIdx.x & 15) * 8;
   float dot = 0.0f, sq = 0.0f;
@@ -260,6 +262,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PackedShape& ps = a.s;
+  let_next_start();
+  wait_for_previous();
   const int unit = blockIdx.x / ps.kv_heads, kvh = blockIdx.x - unit * ps.kv_heads;
   if (unit >= reinterpret_cast<const int*>(a.plan)[kHdrDkv]) return;
   const KItem it = reinterpret_cast<const KItem*>(a.plan + ps.dkv_items)[unit];
@@ -608,6 +612,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PackedShape& ps = a.s;
+  let_next_start();
+  wait_for_previous();
   const int unit = blockIdx.x / ps.heads, head = blockIdx.x - unit * ps.heads, kvh = head / ps.group;
   if (unit >= reinterpret_cast<const int*>(a.plan)[kHdrDq]) return;
   const QItem it = reinterpret_cast<const QItem*>(a.plan + ps.dq_items)[unit];
@@ -847,12 +853,14 @@ template <int DP, bool BF16> int launch_bwd(const BwdMaps& m, const BwdArgs& a, 
   const long long g1 = (long long)a.s.max_dkv_items * a.s.kv_heads, g2 = (long long)a.s.max_dq_items * a.s.heads;
   VA_CHECK_ARG(g1 < (1LL << 31) && g2 < (1LL << 31), "packed attention backward: too many units");
   if (g2 > 0) {
-    packed_dq_kernel<DP, BF16><<<(unsigned)g2, kThreads, smem, st>>>(m.q_tile, m.do_tile, m.k_step, m.v_step, a);
-    if (int rc = check_launch("packed attention dQ")) return rc;
+    if (int rc = launch_behind("packed attention dQ", packed_dq_kernel<DP, BF16>, (unsigned)g2, kThreads, smem, st,
+                               m.q_tile, m.do_tile, m.k_step, m.v_step, a))
+      return rc;
   }
   if (g1 > 0) {
-    packed_dkv_kernel<DP, BF16><<<(unsigned)g1, kThreads, smem, st>>>(m.q_step, m.do_step, m.k_tile, m.v_tile, a);
-    if (int rc = check_launch("packed attention dK/dV")) return rc;
+    if (int rc = launch_behind("packed attention dK/dV", packed_dkv_kernel<DP, BF16>, (unsigned)g1, kThreads, smem, st,
+                               m.q_step, m.do_step, m.k_tile, m.v_tile, a))
+      return rc;
   }
   return VA_OK;
 }
@@ -903,12 +911,13 @@ int packed_bwd(const void* d_out, const void* q, const void* k, const void* v, c
   const long long rows = (long long)total_q * heads + (BF16 ? 0 : (long long)total_k * kv_heads);
   VA_CHECK_ARG((rows + 15) / 16 < (1LL << 31), "packed attention backward: too many rows");
   if (rows > 0) {
-    packed_rows_kernel<BF16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(
-        static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(d_out), strides[6], strides[7],
-        static_cast<const uint16_t*>(v), strides[4], strides[5], lse, reinterpret_cast<float2*>(a.plan + a.s.rows),
-        reinterpret_cast<float*>(a.plan + a.s.do_norm), reinterpret_cast<float*>(a.plan + a.s.v_norm), total_q, total_k,
-        heads, kv_heads, dim);
-    if (int rc = check_launch("packed attention backward rows")) return rc;
+    if (int rc = launch_behind("packed attention backward rows", packed_rows_kernel<BF16>, (unsigned)((rows + 15) / 16),
+                               256, 0, st, static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(d_out),
+                               strides[6], strides[7], static_cast<const uint16_t*>(v), strides[4], strides[5], lse,
+                               reinterpret_cast<float2*>(a.plan + a.s.rows),
+                               reinterpret_cast<float*>(a.plan + a.s.do_norm),
+                               reinterpret_cast<float*>(a.plan + a.s.v_norm), total_q, total_k, heads, kv_heads, dim))
+      return rc;
   }
   return dim <= 64 ? launch_bwd<64, BF16>(m, a, st) : launch_bwd<128, BF16>(m, a, st);
 }

@@ -20,8 +20,7 @@ namespace va {
 namespace {
 
 constexpr int kPlanThreads = 512, kClasses = 256;
-// Parts smaller than this cost more to join than they save (a forward block takes ~1 us, joining ~4 us).
-constexpr int kMinKeyBlocks = 6, kMinQuerySteps = 32;
+
 
 struct Seq {
   int q0, lq, k0, lk;
@@ -96,6 +95,8 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
   __shared__ int hist[kClasses], cursor[kClasses];
   __shared__ int bad, most, first_smem[kPlanSeqs + 1];
   const PackedShape& s = a.s;
+  let_next_start();
+  wait_for_previous();
   const int list = blockIdx.x, tid = threadIdx.x;
   int* hdr = reinterpret_cast<int*>(a.plan);
   // tiles before each sequence
@@ -260,8 +261,7 @@ int va_packed_plan_build(const int32_t* cu_q, const int32_t* cu_k, int num_seqs,
     return set_error(VA_ERR_WORKSPACE, "packed plan: %zu < %zu bytes", plan_bytes, a.s.total);
   if (reinterpret_cast<uintptr_t>(plan) & 255)
     return set_error(VA_ERR_ALIGN, "packed plan: the buffer needs 256-byte alignment");
-  packed_plan_kernel<<<training ? 3 : 1, kPlanThreads, 0, (cudaStream_t)stream>>>(a);
-  return check_launch("packed plan");
+  return launch_behind("packed plan", packed_plan_kernel, training ? 3 : 1, kPlanThreads, 0, (cudaStream_t)stream, a);
 }
 
 int va_packed_plan_status(const void* plan, int training, int* bad_offsets, va_stream_t stream) {

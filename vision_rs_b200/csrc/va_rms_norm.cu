@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) rms_norm_bwd_kernel(NormBw
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x, nvec = a.cols / VEC;
   const int sub = TPR == 32 ? threadIdx.x >> 5 : 0;
   const bool with_gh = a.grad_h != nullptr;
+  let_next_start();
   float dw[NV][VEC] = {}, w[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -382,6 +383,7 @@ __global__ void __launch_bounds__(256) rms_norm_bwd_any_kernel(NormBwdArgs a) {
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ partial, float* __restrict__ dw,
                                                           int n, int cols) {
   __shared__ float s[32][33];
+  wait_for_previous();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
   float v = 0.0f;
   if (c < cols) {
@@ -489,8 +491,8 @@ template <typename T> int rms_norm_bwd(NormBwdArgs a, float* dw, void* ws, size_
   else if (nvec <= 1024) rc = go(rms_norm_bwd_kernel<T, 512, 2>, 512, 0);
   else rc = go(rms_norm_bwd_kernel<T, 512, 4>, 512, 0);
   if (rc) return rc;
-  column_sum_kernel<<<(a.cols + 31) / 32, 1024, 0, st>>>(a.partial, dw, nb, a.cols);
-  return check_launch("rms_norm weight gradient");
+  return launch_behind("rms_norm weight gradient", column_sum_kernel, (a.cols + 31) / 32, 1024, 0, st, a.partial, dw, nb,
+                       a.cols);
 }
 
 }  // namespace
