@@ -547,13 +547,16 @@ VA_API int va_rms_norm_bwd_f32(const float *dy, const float *h, const void *w, i
  * [num_seqs + 1] on the device, the rows where each sequence's queries and
  * keys begin (cu[0] = 0, cu[num_seqs] = total).  It fills the plan (256-byte
  * aligned, va_packed_plan_bytes) on the stream, without a copy to the host;
+ * used_k (optional, int32 [num_seqs], not with `training`): how many of the
+ * rows between cu_k[b] and cu_k[b + 1] hold keys, for a cache with room to grow.
  * later calls with the same sizes read it, layer after layer, and keep their
  * partial results in it: calls that share a plan must not overlap.
  * va_packed_plan_status reads whether offsets were out of order or range (they
  * are clamped; synchronises). */
 VA_API size_t va_packed_plan_bytes(int num_seqs, int total_q, int total_k, int num_heads, int num_kv_heads,
                                    int head_dim, int causal, int training);
-VA_API int va_packed_plan_build(const int32_t *cu_q, const int32_t *cu_k, int num_seqs, int total_q, int total_k,
+VA_API int va_packed_plan_build(const int32_t *cu_q, const int32_t *cu_k, const int32_t *used_k, int num_seqs,
+                                int total_q, int total_k,
                                 int num_heads, int num_kv_heads, int head_dim, int causal, int training,
                                 void *plan, size_t plan_bytes, va_stream_t stream);
 VA_API int va_packed_plan_status(const void *plan, int training, int *bad_offsets, va_stream_t stream);

@@ -173,6 +173,31 @@ def test_cache_of_more_than_2_31_elements(cuda):
     _check(o, lse, q, kv[far:], kv[far:], [3], [n], D ** -0.5, True)
 
 
+@pytest.mark.parametrize("lq", [[1, 1, 1, 1], [3, 0, 300, 40]])
+def test_cache_with_room_to_grow(cuda, lq):
+    """Key rows past the used length hold anything (NaN here) and are never seen."""
+    from vision_rs_b200 import packed
+    room, used, H, Hk, D = [200, 64, 1000, 300], [130, 0, 1000, 77], 8, 2, 64
+    q, k, v = _qkv(cuda, torch.bfloat16, lq, used, H, Hk, D)
+    kc = torch.full((sum(room), Hk, D), float("nan"), dtype=torch.bfloat16, device=cuda)
+    vc, at, a = kc.clone(), 0, 0
+    for r, u in zip(room, used):
+        kc[at:at + u], vc[at:at + u] = k[a:a + u], v[a:a + u]
+        at, a = at + r, a + u
+    plan = packed.PackedPlan(packed.cu_seqlens(lq), packed.cu_seqlens(room), sum(lq), sum(room), H, Hk, D, causal=True,
+                             used_k=torch.tensor(used, dtype=torch.int32, device=cuda))
+    o, lse = packed.packed_attention_forward(q, kc, vc, plan)
+    plan.check()
+    _check(o, lse, q, k, v, lq, used, D ** -0.5, True)
+    over = packed.PackedPlan(packed.cu_seqlens(lq), packed.cu_seqlens(room), sum(lq), sum(room), H, Hk, D, causal=True,
+                             used_k=torch.tensor([201, 0, 5, 5], dtype=torch.int32, device=cuda))
+    with pytest.raises(ValueError):
+        over.check()
+    with pytest.raises(ValueError):
+        packed.PackedPlan(packed.cu_seqlens(lq), packed.cu_seqlens(room), sum(lq), sum(room), H, Hk, D, training=True,
+                          used_k=torch.tensor(used, dtype=torch.int32, device=cuda))
+
+
 def test_offsets_out_of_order_are_reported(cuda):
     from vision_rs_b200 import packed
     q, k, v = _qkv(cuda, torch.bfloat16, [64], [64], 2, 1, 64)
@@ -220,5 +245,5 @@ def test_refusals(cuda):
     assert e.value.code == 4
     lib = _lib.lib()
     st = torch.cuda.current_stream().cuda_stream
-    assert lib.va_packed_plan_build(cu.data_ptr(), cu.data_ptr(), *plan.sizes, plan.buf.data_ptr(), 16, st) == 6
-    assert lib.va_packed_plan_build(cu.data_ptr(), cu.data_ptr(), *plan.sizes, None, 0, st) == 6
+    assert lib.va_packed_plan_build(cu.data_ptr(), cu.data_ptr(), None, *plan.sizes, plan.buf.data_ptr(), 16, st) == 6
+    assert lib.va_packed_plan_build(cu.data_ptr(), cu.data_ptr(), None, *plan.sizes, None, 0, st) == 6

@@ -97,7 +97,7 @@ SIGNATURES: dict[str, tuple] = {
     "va_rms_norm_bwd_workspace_bytes": (SZ, [LL, I]),
     **{f"va_rms_norm_bwd_{t}": (I, [P, P, P, I, P, P, P, LL, I, F, P, SZ, S]) for t in ("bf16", "f16", "f32")},
     "va_packed_plan_bytes": (SZ, [I, I, I, I, I, I, I, I]),
-    "va_packed_plan_build": (I, [P, P, I, I, I, I, I, I, I, I, P, SZ, S]),
+    "va_packed_plan_build": (I, [P, P, P, I, I, I, I, I, I, I, I, P, SZ, S]),
     "va_packed_plan_status": (I, [P, I, C.POINTER(C.c_int), S]),
     **{f"va_packed_attention_fwd_{t}": (I, [P, P, P, P, P, I64P, I, I, I, I, I, I, I, I, F, P, SZ, S])
        for t in ("bf16", "f16")},

@@ -26,14 +26,23 @@ struct Seq {
   int q0, lq, k0, lk;
 };
 
-__device__ __forceinline__ Seq load_seq(const int* cu_q, const int* cu_k, int b, int total_q, int total_k, int* bad) {
+__device__ __forceinline__ Seq load_seq(const int* cu_q, const int* cu_k, const int* used_k, int b, int total_q,
+                                       int total_k, int* bad) {
   const int a0 = cu_q[b], a1 = cu_q[b + 1], c0 = cu_k[b], c1 = cu_k[b + 1];
   Seq s;
   s.q0 = min(max(a0, 0), total_q);
   s.lq = max(min(max(a1, 0), total_q) - s.q0, 0);
   s.k0 = min(max(c0, 0), total_k);
   s.lk = max(min(max(c1, 0), total_k) - s.k0, 0);
-  if (s.q0 != a0 || s.lq != a1 - a0 || s.k0 != c0 || s.lk != c1 - c0 || (b == 0 && (a0 != 0 || c0 != 0))) *bad = 1;
+  if (used_k) {  // keys in use of the rows reserved
+    const int n = min(max(used_k[b], 0), s.lk);
+    if (n != used_k[b]) *bad = 1;
+    if (s.k0 != c0 || s.lk != c1 - c0) *bad = 1;
+    s.lk = n;
+  } else if (s.lk != c1 - c0) {
+    *bad = 1;
+  }
+  if (s.q0 != a0 || s.lq != a1 - a0 || s.k0 != c0 || (b == 0 && (a0 != 0 || c0 != 0))) *bad = 1;
   return s;
 }
 
@@ -61,7 +70,7 @@ __device__ int block_scan(int v, int* total) {
 }
 
 struct PlanArgs {
-  const int *cu_q, *cu_k;
+  const int *cu_q, *cu_k, *used_k;
   uint8_t* plan;
   PackedShape s;
 };
@@ -113,7 +122,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
     const int b = b0 + tid;
     int n = 0;
     if (b < s.num_seqs) {
-      const Seq q = load_seq(a.cu_q, a.cu_k, b, s.total_q, s.total_k, &bad);
+      const Seq q = load_seq(a.cu_q, a.cu_k, a.used_k, b, s.total_q, s.total_k, &bad);
       n = ((list == 2 ? q.lk : q.lq) + tile - 1) / tile;
     }
     int sum;
@@ -139,7 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
       return own_range;
     }
     const int b = seq_of_tile(first, s.num_seqs, t);
-    *q = load_seq(a.cu_q, a.cu_k, b, s.total_q, s.total_k, &bad);
+    *q = load_seq(a.cu_q, a.cu_k, a.used_k, b, s.total_q, s.total_k, &bad);
     *i0 = (t - first[b]) * tile;
     const Range r =
         list == 2 ? query_steps(*q, *i0, s.causal, s.group) : key_blocks(*q, *i0, min(tile, q->lq - *i0), s.causal);
@@ -250,12 +259,13 @@ size_t va_packed_plan_bytes(int num_seqs, int total_q, int total_k, int num_head
   return packed_shape(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim, causal != 0, training != 0).total;
 }
 
-int va_packed_plan_build(const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int total_q, int total_k,
+int va_packed_plan_build(const int32_t* cu_q, const int32_t* cu_k, const int32_t* used_k, int num_seqs, int total_q, int total_k,
                          int num_heads, int num_kv_heads, int head_dim, int causal, int training, void* plan,
                          size_t plan_bytes, va_stream_t stream) {
   if (int rc = packed_check(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim)) return rc;
   VA_CHECK_ARG(cu_q && cu_k, "packed plan: null offsets");
-  PlanArgs a{cu_q, cu_k, static_cast<uint8_t*>(plan),
+  VA_CHECK_ARG(!(used_k && training), "packed plan: reserved rows have no gradient, train without used_k");
+  PlanArgs a{cu_q, cu_k, used_k, static_cast<uint8_t*>(plan),
              packed_shape(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim, causal != 0, training != 0)};
   if (!plan || plan_bytes < a.s.total)
     return set_error(VA_ERR_WORKSPACE, "packed plan: %zu < %zu bytes", plan_bytes, a.s.total);

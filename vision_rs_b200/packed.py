@@ -46,15 +46,17 @@ def _plan_bytes(*sizes) -> int:
 class PackedPlan:
     """Work lists of packed-sequence attention for one batch's sequences and
     one head layout (with the kernels' partial results: calls that share a
-    plan must not overlap on the GPU).  ``cu_q`` and ``cu_k`` stay on the
-    device and are read on ``stream``; ``check()`` raises if they were not
+    plan must not overlap on the GPU).  With ``used_k`` (int32 ``[n]`` on the
+    device) only that many of a sequence's key rows hold keys: a cache with
+    room to grow.  The offsets stay on the device and are read on ``stream``; ``check()`` raises if they were not
     ascending offsets from 0 to the totals."""
 
     def __init__(self, cu_q, cu_k, total_q: int, total_k: int, num_heads: int, num_kv_heads: int, head_dim: int,
-                 causal: bool = False, training: bool = False, stream=None):
+                 causal: bool = False, training: bool = False, used_k=None, stream=None):
         if stream is not None:
             with _launch.on(stream):
-                return self.__init__(cu_q, cu_k, total_q, total_k, num_heads, num_kv_heads, head_dim, causal, training)
+                return self.__init__(cu_q, cu_k, total_q, total_k, num_heads, num_kv_heads, head_dim, causal, training,
+                                     used_k)
         index = cu_q.get_device()
         for t in (cu_q, cu_k):
             if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != index or index < 0 \
@@ -63,13 +65,17 @@ class PackedPlan:
         n = cu_q.shape[0] - 1
         if n < 1 or cu_k.shape[0] != n + 1:
             raise ValueError("cu_q and cu_k must have the same sequences, one at least")
+        if used_k is not None and (used_k.dtype is not torch.int32 or used_k.get_device() != index
+                                   or used_k.shape != (n,) or not used_k.is_contiguous() or training):
+            raise ValueError("used_k must be a contiguous int32 [sequences] tensor beside cu_k, and not for training")
         self.sizes = sizes = (n, total_q, total_k, num_heads, num_kv_heads, head_dim, int(causal), int(training))
         self.nbytes = need = _plan_bytes(*sizes)
         self.index = index
         self.buf = cu_q.new_empty(need, dtype=torch.uint8)
         self.ptr = self.buf.data_ptr()
         self.stream = _launch.raw_stream(index)
-        _launch.run("va_packed_plan_build", index, cu_q.data_ptr(), cu_k.data_ptr(), *sizes, self.ptr, need)
+        _launch.run("va_packed_plan_build", index, cu_q.data_ptr(), cu_k.data_ptr(),
+                    None if used_k is None else used_k.data_ptr(), *sizes, self.ptr, need)
 
     def check(self, stream=None):
         """Raises if the offsets were out of order or range (synchronises)."""
