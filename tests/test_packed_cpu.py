@@ -88,7 +88,7 @@ def test_plan_sizes_and_refusals():
     # keys that fit the smallest part even as one sequence are never split: no room for partial results
     assert size(64, 64, 6 * 128, 32, 8, 128, 1, 0) < 1 << 17 < size(64, 64, 64 * 700, 32, 8, 128, 1, 0)
     for bad in ((0, 5, 5, 2, 1, 64), (2, -1, 5, 2, 1, 64), (2, 5, -1, 2, 1, 64), (2, 5, 5, 3, 2, 64), (2, 5, 5, 0, 1, 64),
-                (2, 5, 5, 2, 1, 12), (2, 5, 5, 2, 1, 0), (2, 5, 5, 2, 1, 136), (2, 5, 5, 129, 1, 64), (2, 1 << 31 - 1, 5, 2, 1, 64)):
+                (2, 5, 5, 2, 1, 12), (2, 5, 5, 2, 1, 0), (2, 5, 5, 2, 1, 136), (2, 5, 5, 129, 1, 64), (2, (1 << 30) + 1, 5, 2, 1, 64)):
         assert size(*bad, 0, 0) == 0 and lib.va_get_last_error_string()
     st = (C.c_int64 * 14)(*[64] * 14)
     fwd = lambda **k: lib.va_packed_attention_fwd_bf16(
