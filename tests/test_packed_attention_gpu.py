@@ -132,6 +132,35 @@ def test_other_sequences_stay_out(cuda, lq, lk):
         assert torch.equal(o2[keep], o[keep]) and torch.equal(lse2[:, keep], lse[:, keep])
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("lq,lk,H,Hk,D", [([300], [300], 2, 2, 64), ([700, 800, 900], [700, 800, 900], 8, 4, 128),
+                                          ([40], [1500], 4, 1, 64), ([9, 300], [9, 400], 2, 1, 80)])
+def test_later_keys_may_hold_anything(cuda, dt, lq, lk, H, Hk, D):
+    """Causal: NaN or infinity in a key or value of each sequence reaches the rows that see it and no earlier one."""
+    from vision_rs_b200 import packed
+    q, k, v = _qkv(cuda, dt, lq, lk, H, Hk, D, seed=1)
+    plan = _plan(lq, lk, H, Hk, D, True)
+    o, lse = packed.packed_attention_forward(q, k, v, plan)
+    for bad in (float("nan"), float("inf")):
+        for which in "kv":
+            k2, v2, sees, at = k.clone(), v.clone(), [], 0
+            for a, b in zip(lq, lk):
+                j = b - min(a, 37) + 3 if a > 3 else b - 1  # a key that the last rows see
+                (k2 if which == "k" else v2)[at + j, :, 5] = bad
+                sees += [i >= j - (b - a) for i in range(a)]
+                at += b
+            sees = torch.tensor(sees)
+            o2, lse2 = packed.packed_attention_forward(q, k2, v2, plan)
+            assert torch.equal(o2[~sees], o[~sees]) and torch.equal(lse2[:, ~sees], lse[:, ~sees])
+            if which == "v":
+                rest = [c for c in range(D) if c != 5]
+                assert torch.equal(lse2, lse) and torch.equal(o2[..., rest], o[..., rest])
+                got = o2[sees][..., 5]
+                assert (got.isnan() if bad != bad else got == bad).all()
+            elif bad != bad:
+                assert o2[sees].isnan().all() and lse2[:, sees].isnan().all()
+
+
 def test_plan_is_shared_and_results_repeat(cuda):
     """Layer after layer over one plan, on another stream too; the same bits each time."""
     from vision_rs_b200 import packed

@@ -23,10 +23,12 @@
 // rounding adds about as much error as that of the output.  Sums, maxima and
 // O stay f32.
 //
-// Rows of other sequences that a tile's boxes bring in: scores of keys past
-// the end are replaced, not added to; V rows past the last key that the unit sees are zeroed in
-// shared memory (0 · NaN would be NaN), and the MMAs stop at the last 16-key
-// group in use.
+// What a row does not see stays out of it, whatever it holds (another
+// sequence's rows in a box, unused rows of a cache, later keys): scores of such
+// keys are replaced, not added to, and as 0 · NaN would be NaN, a warp of its
+// own checks the V blocks that hold them: rows past the unit's last key become
+// zeros, values that are not finite are left out of the product and given back
+// to the rows that do see them.  The MMAs stop at the last 16-key group in use.
 #include <cudaTypedefs.h>
 
 #include <type_traits>
@@ -48,13 +50,14 @@ constexpr float kRescaleAt = 8.0f;  // the reference follows the maximum once it
 // Rows of at most this many 64-key steps hold P as two 16-bit words, value and remainder, and multiply V by both: there the
 // second product costs nothing that is measured, and the output is exact to its own rounding.
 constexpr int kFineSteps = 2;
+constexpr int kMaxChecked = 3;        // V blocks with keys that some row of a unit does not see: at most 256 rows' diagonal
 constexpr float kF16Shift = 7.0f;   // f16: P is held times 2^7 (at most 2^15), so small ones keep their bits
 
 // DP: head size in shared memory and TMEM (64 or 128; the TMA boxes fill what is past `dim` with zeros).
 template <int DP, int TILES> struct FwdCfg {
   static constexpr int kSlotBytes = kPackBlock * DP * 2;
   static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 5);
-  static constexpr int kThreads = TILES * 160 + 32;
+  static constexpr int kThreads = TILES == 2 ? 384 : 192;
   static constexpr int kCtas = TILES == 2 ? 1 : 2;  // an SM
   static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
   static constexpr uint32_t kColS = 0, kColO = TILES * 128;  // tile m: scores at 128·m and 128·m + 64, O at kColO + DP·m
@@ -65,15 +68,18 @@ template <int DP, int TILES> struct FwdSmem {
   uint8_t q[TILES][C::kSlotBytes];      // per 64 dims: 128 rows × 128 bytes, SW128
   uint8_t kv[C::kSlots][C::kSlotBytes];
   uint64_t q_full, kv_full[C::kSlots], kv_empty[C::kSlots];
-  uint64_t s_full[TILES][2], p_full[TILES][2], o_done[TILES][2], v_ready, fin;
+  uint64_t s_full[TILES][2], p_full[TILES][2], o_done[TILES][2], v_sent[kMaxChecked], v_ready[kMaxChecked], fin;
   uint32_t tmem_base;
   int abort;
   int last;
+  int loose;  // a checked V block held something that is not finite
 };
 
 struct FwdArgs {
   const uint8_t* plan;
   PackedShape s;
+  const uint16_t* v;
+  long long v_row, v_head;  // strides in elements
   void* out;
   float* lse;
   float scale;  // softmax scale · log2 e
@@ -110,6 +116,13 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   }
   const int all_steps = max(steps[0], steps[TILES - 1]), nkb = (all_steps + 1) >> 1;
   const int dim16 = (ps.dim + 15) & ~15;
+  // V blocks that are looked at before they are multiplied: those with keys hidden from some row (weight 0, but 0 · NaN
+  // is NaN), and a last one that ends inside a 16-key group of the MMAs
+  const int hidden = ps.causal ? min(see_end, max(0, it.see + 1)) : see_end;  // first key that a row does not see
+  const int used_last = see_end - (it.kb0 + nkb - 1) * kPackBlock;            // keys of the last block
+  const int checked = hidden < see_end ? max(it.kb0, hidden / kPackBlock)
+                      : (used_last & 15) && used_last < kPackBlock ? it.kb0 + nkb - 1
+                                                                   : it.kb0 + nkb;
 
   if (tid == 0) {
     mbar_init(&sm.q_full, 1);
@@ -124,7 +137,8 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         mbar_init(&sm.o_done[m][r], 1);
       }
     }
-    mbar_init(&sm.v_ready, 1);
+    for (int i = 0; i < kMaxChecked; ++i) mbar_init(&sm.v_sent[i], 1), mbar_init(&sm.v_ready[i], 1);
+    sm.loose = 0;
     mbar_init(&sm.fin, TILES);
     sm.abort = 0;
     fence_mbar_init();
@@ -138,28 +152,88 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
 
+  // ── V check (a whole warp): zeroes rows past the last key in its 16-key group, and what is not finite in blocks with
+  // hidden keys (rows that see such a value get it back when the output is written) ──
+  auto check_v = [&](int kb) -> bool {
+    const int g = 2 * (kb - it.kb0) + 1, sv = g % C::kSlots, used = min(kPackBlock, see_end - kb * kPackBlock);
+    if (!__all_sync(0xffffffffu, mbar_wait(&sm.kv_full[sv], (g / C::kSlots) & 1, &sm.abort, &g_packed_status, 4)))
+      return false;
+    auto cell = [&](int row, int c) {
+      return reinterpret_cast<uint4*>(sm.kv[sv] + (c >> 3) * kPackBlock * 128 + sw128_off(row, c & 7));
+    };
+    for (int i = lane; i < ((used + 15) / 16 * 16 - used) * (DP / 8); i += 32)
+      *cell(used + i / (DP / 8), i % (DP / 8)) = make_uint4(0, 0, 0, 0);
+    if (hidden < see_end) {
+      constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+      // an exponent of ones carries into its half's top bit
+      auto flags = [&](uint32_t w) { return (w & kExp) + kOne; };
+      uint32_t any = 0;  // all cells are read without a branch between them; the rare second pass mends
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        const uint4* base = reinterpret_cast<const uint4*>(sm.kv[sv] + c * kPackBlock * 128);
+        const int cells = used * 8;  // 16-byte cells of the block's rows, in whatever order the swizzle has them
+#pragma unroll 8
+        for (int i = lane; i < cells; i += 32) {
+          const uint4 x = base[i];
+          any |= flags(x.x) | flags(x.y) | flags(x.z) | flags(x.w);
+        }
+      }
+      bool found = false;
+      if (__any_sync(0xffffffffu, (any & 0x80008000u) != 0)) {
+        for (int i = lane; i < used * (DP / 8); i += 32) {
+          uint4* p = cell(i / (DP / 8), i % (DP / 8));
+          const uint4 x = *p;
+          auto keep = [&](uint32_t w) {  // without the halves whose top bit is flagged
+            const uint32_t t = (flags(w) & 0x80008000u) >> 15;
+            found |= t != 0;
+            return w & ~(t * 0xffffu);
+          };
+          *p = make_uint4(keep(x.x), keep(x.y), keep(x.z), keep(x.w));
+        }
+      }
+      if (found) *(volatile int*)&sm.loose = 1;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.v_ready[kb - checked]);
+    return true;
+  };
+
   if (warp == TILES * 4) {
-    // ── TMA producer: Q, then K and V blocks alternately through the slot ring ──
-    if (lane == 0 && nkb > 0) {
+    // ── TMA producer: Q, then K and V blocks alternately through the slot ring.  A unit of one tile has its V blocks
+    // checked here (a warp more would cost its softmax registers; what it holds up is at most the last two blocks) ──
+    if (nkb > 0) {
       constexpr int NB = DP / 64;
       const uint32_t q_bytes = (uint32_t)(ps.few ? (kPackBlock / group) * group : kPackBlock) * 128 * NB;
-      mbar_arrive_expect_tx(&sm.q_full, q_bytes * TILES);
-      for (int m = 0; m < TILES; ++m)
-        for (int b = 0; b < NB; ++b)
-          tma_load_3d(sm.q[m] + b * kPackBlock * 128, &map_q, &sm.q_full, b * 64, ps.few ? head * group : head,
-                      it.q0 + m * kPackBlock);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sm.q_full, q_bytes * TILES);
+        for (int m = 0; m < TILES; ++m)
+          for (int b = 0; b < NB; ++b)
+            tma_load_3d(sm.q[m] + b * kPackBlock * 128, &map_q, &sm.q_full, b * 64, ps.few ? head * group : head,
+                        it.q0 + m * kPackBlock);
+      }
       bool ok = true;
       int issued = 0;
       for (int g = 0; g < 2 * nkb; ++g) {
-        const int st = g % C::kSlots, row = it.k0 + (it.kb0 + (g >> 1)) * kPackBlock;
+        const int st = g % C::kSlots, kb = it.kb0 + (g >> 1);
         if (g >= C::kSlots &&
-            !(ok = mbar_wait(&sm.kv_empty[st], (g / C::kSlots - 1) & 1, &sm.abort, &g_packed_status, 1)))
+            !(ok = __all_sync(0xffffffffu, mbar_wait(&sm.kv_empty[st], (g / C::kSlots - 1) & 1, &sm.abort,
+                                                     &g_packed_status, 1))))
           break;
-        mbar_arrive_expect_tx(&sm.kv_full[st], C::kSlotBytes);
-        for (int b = 0; b < NB; ++b)
-          tma_load_3d(sm.kv[st] + b * kPackBlock * 128, (g & 1) ? &map_v : &map_k, &sm.kv_full[st], b * 64, kv_head,
-                      row);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sm.kv_full[st], C::kSlotBytes);
+          for (int b = 0; b < NB; ++b)
+            tma_load_3d(sm.kv[st] + b * kPackBlock * 128, (g & 1) ? &map_v : &map_k, &sm.kv_full[st], b * 64, kv_head,
+                        it.k0 + kb * kPackBlock);
+        }
         ++issued;
+        if ((g & 1) && kb >= checked) {
+          if constexpr (TILES == 1) {
+            if (!(ok = check_v(kb))) break;
+          } else if (lane == 0) {
+            mbar_arrive(&sm.v_sent[kb - checked]);
+          }
+        }
       }
       if (!ok) {  // loads issued here land (bounded) before the CTA can exit
         for (int g = max(0, issued - C::kSlots); g < issued; ++g) {
@@ -173,19 +247,12 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
     }
     __syncwarp();
-    // V rows past the last key that the unit sees, up to the 16-key group that the MMAs stop at: zeros
-    const int used = see_end - (it.kb0 + nkb - 1) * kPackBlock, g = 2 * nkb - 1, sv = g % C::kSlots;
-    if (nkb > 0 && (used & 15) && used < kPackBlock &&
-        mbar_wait(&sm.kv_full[sv], (g / C::kSlots) & 1, &sm.abort, &g_packed_status, 4)) {
-      for (int i = lane; i < ((used + 15) / 16 * 16 - used) * (DP / 8); i += 32) {
-        const int row = used + i / (DP / 8), c = i % (DP / 8);
-        *reinterpret_cast<uint4*>(sm.kv[sv] + (c >> 3) * kPackBlock * 128 + sw128_off(row, c & 7)) =
-            make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.v_ready);
-    }
+  } else if (TILES == 2 && warp == TILES * 5 + 1) {
+    // (the slot's barrier is in the phase of a block's load only once the load is sent)
+    for (int kb = checked; kb < it.kb0 + nkb; ++kb)
+      if (!__all_sync(0xffffffffu, mbar_wait(&sm.v_sent[kb - checked], 0, &sm.abort, &g_packed_status, 12)) ||
+          !check_v(kb))
+        break;
     __syncwarp();
   } else if (warp > TILES * 4) {
     // ── MMA issuer of tile m: a converged warp whose values are uniform (the instructions between two MMAs are on
@@ -243,20 +310,20 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         mma_commit_p(&sm.kv_empty[0], lead);
         ahead(sk, pk);
       }
-      const int last_j = (all - 1) >> 1, used_last = end - last_j * kPackBlock;  // keys of the last block
+      const int last_j = (all - 1) >> 1, in_last = uniform(used_last), check_j = uniform(checked - it.kb0);
       for (int h = 0; ok && h < all; ++h) {
         const int r = h & 1, g = h + 2;  // g: the step whose scores take this one's buffer
         const bool last = (h >> 1) == last_j;
         if (r == 0) {
           if (!(ok = wait(&sm.kv_full[sv], pv, 4))) break;
-          if (last && (used_last & 15) && used_last < kPackBlock && !(ok = wait(&sm.v_ready, 0, 11))) break;
+          if ((h >> 1) >= check_j && !(ok = wait(&sm.v_ready[(h >> 1) - check_j], 0, 11))) break;
         }
         if (h < n) {
           if (!(ok = wait(&sm.p_full[m][r], (h >> 1) & 1, 5))) break;
           tc_fence_after();
           const uint64_t dv = dv0 + (uint64_t)(sv * kSlot + r * kHalfRows);
           const uint32_t tp = ts + r * kHalf;
-          const int ks = last ? min(kHalf / 16, (used_last - r * kHalf + 15) >> 4) : kHalf / 16;
+          const int ks = last ? min(kHalf / 16, (in_last - r * kHalf + 15) >> 4) : kHalf / 16;
           if (ks == kHalf / 16 && !fine) {
 #pragma unroll
             for (int s = 0; s < kHalf / 16; ++s)
@@ -340,7 +407,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     auto follow = [&](int h, float top) -> bool {  // the reference follows, O is rescaled
       const bool grow = mine && (top > ref + kRescaleAt || ref == -INFINITY);
       if (!__any_sync(0xffffffffu, grow)) return true;
-      const float next = fmaxf(ref, top);
+      const float next = grow ? fmaxf(ref, top) : ref;  // a row's result does not depend on its warp's other rows
       if (h > 0) {
         const float f = next == -INFINITY ? 1.0f : ex2(ref - next);
         if (!mbar_wait(&sm.o_done[m][(h & 1) ^ 1], ((h - 1) >> 1) & 1, &sm.abort, &g_packed_status, 9)) return false;
@@ -411,6 +478,17 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const float inv = 1.0f / sum;
       const float lse = !none ? (ref - (BF16 ? 0.0f : kF16Shift) + log2f(sum)) * kLn2 : -INFINITY;
       const int t = my_row / group, h = ps.few ? head * group + my_row - t * group : head;
+      // Values that are not finite were left out of the product: a row that sees one has it in the output whatever its weight.
+      const bool loose = n > 0 && checked < it.kb0 + nkb && *(volatile int*)&sm.loose;
+      auto add_loose = [&](uint32_t (&o)[16], int c) {
+        for (int j = checked * kPackBlock; j < min(see, it.kb1 * kPackBlock); ++j) {
+          const uint16_t* vj = a.v + (it.k0 + j) * a.v_row + kv_head * a.v_head + c;
+          for (int i = 0; i < 16 && c + i < ps.dim; ++i) {
+            const float x = BF16 ? __uint_as_float((uint32_t)vj[i] << 16) : __half2float(__ushort_as_half(vj[i]));
+            if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+          }
+        }
+      };
       if (it.slot < 0) {
         const long long at = (long long)(it.q0 + t) * ps.heads + h;
         uint16_t* out = static_cast<uint16_t*>(a.out) + at * ps.dim;
@@ -423,6 +501,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+          if (loose && mine) add_loose(o, c);
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = pack2<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
@@ -444,15 +523,12 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             reg_fence(o);
           }
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            if (!mine || c + i >= ps.dim) continue;
-            float4 f;
-            f.x = none ? 0.0f : __uint_as_float(o[i]) * inv;
-            f.y = none ? 0.0f : __uint_as_float(o[i + 1]) * inv;
-            f.z = none ? 0.0f : __uint_as_float(o[i + 2]) * inv;
-            f.w = none ? 0.0f : __uint_as_float(o[i + 3]) * inv;
-            *reinterpret_cast<float4*>(out + c + i) = f;
-          }
+          for (int i = 0; i < 16; ++i) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+          if (loose && mine) add_loose(o, c);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            if (mine && c + i < ps.dim)
+              *reinterpret_cast<uint4*>(out + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           __syncwarp();
         }
         if (mine) reinterpret_cast<float*>(const_cast<uint8_t*>(a.plan) + ps.part_lse)[at] = lse;
@@ -565,8 +641,8 @@ int packed_fwd(const void* q, const void* k, const void* v, void* out, float* ls
   if (total_q == 0) return VA_OK;
   VA_CHECK_ARG(q && out && lse && strides && (total_k == 0 || (k && v)), "packed attention: null pointer");
   FwdArgs a{static_cast<const uint8_t*>(plan),
-            packed_shape(num_seqs, total_q, total_k, heads, kv_heads, dim, causal != 0, training != 0), out, lse,
-            scale * kLog2e};
+            packed_shape(num_seqs, total_q, total_k, heads, kv_heads, dim, causal != 0, training != 0),
+            static_cast<const uint16_t*>(v), strides[4], strides[5], out, lse, scale * kLog2e};
   if (!plan || plan_bytes < a.s.total)
     return set_error(VA_ERR_WORKSPACE, "packed attention: plan of %zu < %zu bytes", plan_bytes, a.s.total);
   if ((reinterpret_cast<uintptr_t>(plan) & 255) || (reinterpret_cast<uintptr_t>(out) & 15))
