@@ -51,6 +51,7 @@ struct PackedShape {
   // unit (few = 0), or (query, head of the group) pairs, one tile a unit
   // with its keys split over units (few = 1).
   int few;
+  int tile_rows;    // few: rows of a tile that hold anything, 128 or 32
   int q_tile;       // queries a forward unit
   int units;        // heads (or key heads) that each forward unit is run for
   int max_tiles, max_items, max_slots, split_budget;
@@ -76,7 +77,9 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   // average, or when units of 256 queries would leave SMs idle.
   const long long big = ((long long)total_q / 256 + num_seqs) * heads;
   s.few = (long long)total_q * s.group <= 128LL * num_seqs || big < 148 ? 1 : 0;
-  s.q_tile = s.few ? kPackBlock / s.group : 2 * kPackBlock;
+  // Single tokens and the like: 32 rows a tile leave shared memory for a third K or V block on its way.
+  s.tile_rows = s.few && s.group <= 32 && (long long)total_q * s.group <= 32LL * num_seqs ? 32 : kPackBlock;
+  s.q_tile = s.few ? s.tile_rows / s.group : 2 * kPackBlock;
   s.units = s.few ? kv_heads : heads;
   s.max_tiles = (int)std::min<long long>((total_q + s.q_tile - 1) / s.q_tile + (long long)num_seqs, total_q);
   // Parts over the number of tiles: enough for four units an SM slot, and no more than the longest possible tiles allow
@@ -101,8 +104,8 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   s.counters = o, o += pk_align(s.few ? (size_t)s.max_tiles * s.units * 4 : 0);
   s.dkv_counters = o, o += pk_align((size_t)s.max_dkv_tiles * kv_heads * 4);
   s.scratch = o, o += pk_align(num_seqs > kPlanSeqs ? (size_t)3 * (num_seqs + 1) * 4 : 0);
-  s.part_o = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * dim * 4);
-  s.part_lse = o, o += pk_align((size_t)s.max_slots * s.units * kPackBlock * 4);
+  s.part_o = o, o += pk_align((size_t)s.max_slots * s.units * s.tile_rows * dim * 4);
+  s.part_lse = o, o += pk_align((size_t)s.max_slots * s.units * s.tile_rows * 4);
   s.part_dkv = o, o += pk_align((size_t)2 * s.dkv_budget * kv_heads * 2 * kPackBlock * dim * 4);
   // training: (lse·log2 e, Δ) a query and head, ‖dO_i‖ and ‖V_j‖ (the f16 backward's)
   s.rows = o, o += pk_align(training ? (size_t)total_q * heads * 8 : 0);

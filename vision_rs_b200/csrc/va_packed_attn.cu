@@ -54,18 +54,20 @@ constexpr int kMaxChecked = 3;        // V blocks with keys that some row of a u
 constexpr float kF16Shift = 7.0f;   // f16: P is held times 2^7 (at most 2^15), so small ones keep their bits
 
 // DP: head size in shared memory and TMEM (64 or 128; the TMA boxes fill what is past `dim` with zeros).
-template <int DP, int TILES> struct FwdCfg {
+// ROWS: rows of a tile that hold anything (32 or 128; the MMAs always take 128, the others' results go nowhere).
+template <int DP, int TILES, int ROWS> struct FwdCfg {
   static constexpr int kSlotBytes = kPackBlock * DP * 2;
-  static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 5);
+  static constexpr int kQBytes = ROWS * DP * 2;
+  static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 5) + (ROWS == 32 ? 1 : 0);
   static constexpr int kThreads = TILES == 2 ? 384 : 192;
   static constexpr int kCtas = TILES == 2 ? 1 : 2;  // an SM
   static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
   static constexpr uint32_t kColS = 0, kColO = TILES * 128;  // tile m: scores at 128·m and 128·m + 64, O at kColO + DP·m
 };
 
-template <int DP, int TILES> struct FwdSmem {
-  using C = FwdCfg<DP, TILES>;
-  uint8_t q[TILES][C::kSlotBytes];      // per 64 dims: 128 rows × 128 bytes, SW128
+template <int DP, int TILES, int ROWS> struct FwdSmem {
+  using C = FwdCfg<DP, TILES, ROWS>;
+  uint8_t q[TILES][C::kQBytes];         // per 64 dims: ROWS rows × 128 bytes, SW128 (the MMAs read on into kv)
   uint8_t kv[C::kSlots][C::kSlotBytes];
   uint64_t q_full, kv_full[C::kSlots], kv_empty[C::kSlots];
   uint64_t s_full[TILES][2], p_full[TILES][2], o_done[TILES][2], v_sent[kMaxChecked], v_ready[kMaxChecked], fin;
@@ -86,13 +88,14 @@ struct FwdArgs {
 };
 
 
-template <int DP, int TILES, bool BF16>
-__global__ void __launch_bounds__(FwdCfg<DP, TILES>::kThreads, FwdCfg<DP, TILES>::kCtas)
+template <int DP, int TILES, bool BF16, int ROWS>
+__global__ void __launch_bounds__(FwdCfg<DP, TILES, ROWS>::kThreads, FwdCfg<DP, TILES, ROWS>::kCtas)
 packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, FwdArgs a) {
-  using C = FwdCfg<DP, TILES>;
+  using C = FwdCfg<DP, TILES, ROWS>;
   extern __shared__ uint8_t smem_raw[];
-  FwdSmem<DP, TILES>& sm = *reinterpret_cast<FwdSmem<DP, TILES>*>(
+  using Smem = FwdSmem<DP, TILES, ROWS>;
+  Smem& sm = *reinterpret_cast<Smem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PackedShape& ps = a.s;
   let_next_start();
@@ -204,12 +207,12 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     // checked here (a warp more would cost its softmax registers; what it holds up is at most the last two blocks) ──
     if (nkb > 0) {
       constexpr int NB = DP / 64;
-      const uint32_t q_bytes = (uint32_t)(ps.few ? (kPackBlock / group) * group : kPackBlock) * 128 * NB;
+      const uint32_t q_bytes = (uint32_t)(ps.few ? ps.q_tile * group : kPackBlock) * 128 * NB;
       if (lane == 0) {
         mbar_arrive_expect_tx(&sm.q_full, q_bytes * TILES);
         for (int m = 0; m < TILES; ++m)
           for (int b = 0; b < NB; ++b)
-            tma_load_3d(sm.q[m] + b * kPackBlock * 128, &map_q, &sm.q_full, b * 64, ps.few ? head * group : head,
+            tma_load_3d(sm.q[m] + b * ROWS * 128, &map_q, &sm.q_full, b * 64, ps.few ? head * group : head,
                         it.q0 + m * kPackBlock);
       }
       bool ok = true;
@@ -267,6 +270,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &sm.abort, &g_packed_status, where));
       };
       constexpr int kBlk = (kPackBlock * 128) >> 4;              // 64 dims further, in descriptor units
+      constexpr int kQBlk = (ROWS * 128) >> 4;
       constexpr int kHalfRows = (kHalf * 128) >> 4, kSlot = C::kSlotBytes >> 4;
       const uint32_t idesc_o = idesc_f32acc(kPackBlock, dim16, fmt, false, true);
       const uint32_t idesc_s = idesc_f32acc(kPackBlock, kHalf, fmt, false, false);
@@ -284,13 +288,13 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (dim16 == DP) {
 #pragma unroll
           for (int s = 0; s < DP / 16; ++s) {
-            const uint64_t off = (uint64_t)((s >> 2) * kBlk + (s & 3) * 2);
-            mma_ss_p(d, dq + off, dk + off, idesc, s > 0 ? 1u : 0u, lead);
+            mma_ss_p(d, dq + (uint64_t)((s >> 2) * kQBlk + (s & 3) * 2), dk + (uint64_t)((s >> 2) * kBlk + (s & 3) * 2),
+                     idesc, s > 0 ? 1u : 0u, lead);
           }
         } else {
           for (int s = 0; s < dim16 / 16; ++s) {
-            const uint64_t off = (uint64_t)((s >> 2) * kBlk + (s & 3) * 2);
-            mma_ss_p(d, dq + off, dk + off, idesc, s > 0 ? 1u : 0u, lead);
+            mma_ss_p(d, dq + (uint64_t)((s >> 2) * kQBlk + (s & 3) * 2), dk + (uint64_t)((s >> 2) * kBlk + (s & 3) * 2),
+                     idesc, s > 0 ? 1u : 0u, lead);
           }
         }
         mma_commit_p(&sm.s_full[m][h & 1], lead);
@@ -513,7 +517,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         if (mine) a.lse[(long long)h * ps.total_q + it.q0 + t] = lse;
       } else {
-        const long long at = ((long long)it.slot * ps.units + head) * kPackBlock + row;
+        const long long at = ((long long)it.slot * ps.units + head) * ROWS + row;
         float* out = reinterpret_cast<float*>(const_cast<uint8_t*>(a.plan) + ps.part_o) + at * ps.dim;
         for (int c = 0; c < dim16; c += 16) {
           uint32_t o[16];
@@ -553,7 +557,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (!sm.last) return;
     const float* plse = reinterpret_cast<const float*>(a.plan + ps.part_lse);
     const float* po = reinterpret_cast<const float*>(a.plan + ps.part_o);
-    const long long base = ((long long)it.slot0 * ps.units + head) * kPackBlock, step = (long long)ps.units * kPackBlock;
+    const long long base = ((long long)it.slot0 * ps.units + head) * ROWS, step = (long long)ps.units * ROWS;
     for (int r = warp; r < rows; r += C::kThreads / 32) {
       float top = -INFINITY;
       for (int k = lane; k < it.parts; k += 32) top = fmaxf(top, __ldcg(plse + base + k * step + r));
@@ -616,11 +620,11 @@ int packed_map(CUtensorMap* m, const void* base, bool bf16, int rows, int heads,
 
 namespace {
 
-template <int DP, int TILES, bool BF16>
+template <int DP, int TILES, bool BF16, int ROWS>
 int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdArgs& a, cudaStream_t st) {
-  using C = FwdCfg<DP, TILES>;
-  auto kernel = packed_attn_kernel<DP, TILES, BF16>;
-  constexpr int smem = (int)sizeof(FwdSmem<DP, TILES>) + 1024;
+  using C = FwdCfg<DP, TILES, ROWS>;
+  auto kernel = packed_attn_kernel<DP, TILES, BF16, ROWS>;
+  constexpr int smem = (int)sizeof(FwdSmem<DP, TILES, ROWS>) + 1024;
   static PerDeviceOnce once;
   if (int rc = once.run([&]() -> int {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -658,8 +662,11 @@ int packed_fwd(const void* q, const void* k, const void* v, void* out, float* ls
   } else {
     mk = mv = mq;  // no unit has a key block: never read
   }
-  if (dim <= 64) return s.few ? launch_fwd<64, 1, BF16>(mq, mk, mv, a, st) : launch_fwd<64, 2, BF16>(mq, mk, mv, a, st);
-  return s.few ? launch_fwd<128, 1, BF16>(mq, mk, mv, a, st) : launch_fwd<128, 2, BF16>(mq, mk, mv, a, st);
+  auto go = [&](auto dp) -> int {
+    if (!s.few) return launch_fwd<dp, 2, BF16, 128>(mq, mk, mv, a, st);
+    return s.tile_rows == 32 ? launch_fwd<dp, 1, BF16, 32>(mq, mk, mv, a, st) : launch_fwd<dp, 1, BF16, 128>(mq, mk, mv, a, st);
+  };
+  return dim <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
 
 }  // namespace

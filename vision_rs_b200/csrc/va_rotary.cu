@@ -23,7 +23,7 @@ namespace va {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kBatch = 4;         // heads of a thread that are in flight together
+constexpr int kBatch = 6;         // heads of a thread that are in flight together
 constexpr int kMaxAngles = 2048;  // of a block (16 KB)
 constexpr int kMaxRot = 512;
 
