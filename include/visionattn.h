@@ -537,7 +537,8 @@ VA_API int va_rms_norm_bwd_f32(const float *dy, const float *h, const void *w, i
  * over the keys of query i's own sequence, query head h reading key head
  * h / (num_heads/num_kv_heads); causal: query i of lq sees key j of lk when
  * j ≤ i + lk − lq (the last query sees every key).  A query that sees no key gets
- * O = 0 and lse = −∞.  q [total_q, num_heads, head_dim], k and v
+ * O = 0 and lse = −∞; keys and values that it does not see may hold anything, NaN
+ * included.  q [total_q, num_heads, head_dim], k and v
  * [total_k, num_kv_heads, head_dim], 16-bit types, rows and heads strided
  * (strides, host, elements: q row, q head, k row, k head, v row, v head;
  * 16-byte multiples, base 16-byte aligned, a head's dimensions contiguous),
@@ -574,7 +575,9 @@ VA_API int va_packed_attention_fwd_f16(const void *q, const void *k, const void 
  * share a key head) from grad_out and the forward's out and lse; the plan must
  * be built with `training`.  strides: as the forward's six, then grad_out row,
  * head, grad_q row, head, grad_k row, head, grad_v row, head.  Rows of keys
- * and queries that see nothing get zeros.  No atomics: the same bits each time. */
+ * and queries that see nothing get zeros.  The bits do not depend on scheduling.
+ * Another sequence's rows may hold anything; within a sequence a value that is
+ * not finite may reach gradients of rows up to 127 positions before it. */
 VA_API int va_packed_attention_bwd_bf16(const va_bf16 *grad_out, const va_bf16 *q, const va_bf16 *k, const va_bf16 *v,
                                         const va_bf16 *out, const float *lse, va_bf16 *grad_q, va_bf16 *grad_k, va_bf16 *grad_v,
                                         const int64_t *strides, int num_seqs, int total_q, int total_k,
