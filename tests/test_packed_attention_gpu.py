@@ -231,7 +231,7 @@ def test_offsets_out_of_order_are_reported(cuda):
     from vision_rs_b200 import packed
     q, k, v = _qkv(cuda, torch.bfloat16, [64], [64], 2, 1, 64)
     good = packed.cu_seqlens([20, 44])
-    for cu in ([0, 50, 20], [0, 20, 9999], [-5, 20, 64], [3, 20, 64]):
+    for cu in ([0, 50, 20], [0, 20, 9999], [-5, 20, 64], [3, 20, 64], [0, 20, 60]):
         plan = packed.PackedPlan(torch.tensor(cu, dtype=torch.int32, device=cuda), good, 64, 64, 2, 1, 64)
         packed.packed_attention_forward(q, k, v, plan)  # clamped: stays inside the tensors
         torch.cuda.synchronize()

@@ -66,6 +66,40 @@ def test_token_by_token_is_the_whole_prompt(cuda, eight_bits):
     assert rel_l2(got.float().cpu(), o.view(n, steps, -1)) < (0.08 if eight_bits else 0.02)
 
 
+def test_training_step_in_a_cuda_graph(cuda):
+    """Plan, forward and backward captured once and replayed on new data, new lengths included: the same bits as eager."""
+    from vision_rs_b200 import packed, rmsnorm, rotary
+    H, D, T = 4, 64, 500
+    gen = torch.Generator().manual_seed(2)
+    new = lambda: torch.randn(T, 3 * H, D, generator=gen).to(cuda, torch.bfloat16)
+    qkv, gout, cu = new(), new()[:, :H], packed.cu_seqlens([200, 300])
+    pos, inv, w = torch.arange(T, device=cuda), rotary.rotary_frequencies(D), torch.ones(H * D, device=cuda)
+
+    def step():
+        q, k, v = qkv.split(H, dim=1)
+        q, k = rotary.rotary_forward(q, k, pos, inv)
+        plan = packed.PackedPlan(cu, cu, T, T, H, H, D, causal=True, training=True)
+        out, lse = packed.packed_attention_forward(q, k, v, plan)
+        grads = packed.packed_attention_backward(gout, q, k, v, out, lse, plan)
+        y, h = rmsnorm.rms_norm_forward(out.view(T, -1), w)
+        return (out, lse, *grads, y, *rmsnorm.rms_norm_backward(y, h, w))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for lengths in ([200, 300], [499, 1], [37, 463]):
+        qkv.copy_(new())
+        cu.copy_(packed.cu_seqlens(lengths))
+        graph.replay()
+        got = [t.clone() for t in outs]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
 def test_example_runs(cuda, capsys):
     import packed_attention_layer
     packed_attention_layer.main()

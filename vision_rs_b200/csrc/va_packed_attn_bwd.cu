@@ -20,9 +20,10 @@
 // S and dP are computed twice (7 products instead of 5); the one-kernel form
 // would add f32 dQ partials to memory from every key tile, in an order that
 // changes from run to run, or write and read all of them.  Two score buffers
-// and two softmax groups alternate, so the MMAs of one step run under the
-// exponentials of the other.  Steps are 64 wide because dV, dK (256 columns)
-// and two buffers of S and dP (4 × 64) fill the 512 TMEM columns at 128 dims.
+// (three at 64 dims) and as many groups of warps alternate, so the MMAs of one
+// step run under the exponentials of another.  Steps are 64 wide because dV,
+// dK (256 columns) and two buffers of S and dP (4 × 64) fill the 512 TMEM
+// columns at 128 dims.
 //
 // P and dS are 16-bit operands.  f16 has few exponents, so there P carries
 // 2^15 and dS a power of two chosen for its row (key or query) such that the
@@ -48,22 +49,33 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kHalf = 64;     // queries (or keys) a step
-constexpr int kStages = 4;    // ring of 64-row (Q, dO) or (K, V) pairs
-constexpr int kThreads = 352; // 2 × 4 warps of scores, 1 TMA, 1 to issue the scores' MMAs, 1 the gradients'
 // Sequences of at most this many 64-row steps hold P and dS as two 16-bit words, value and remainder, and multiply by both:
 // there the second products cost nothing that is measured, and the gradients are exact to their own rounding.
 constexpr int kFineSteps = 2;
 constexpr float kPShift = 15.0f;     // f16: P is held times 2^15
-constexpr uint32_t kColAcc = 256;    // score buffers at 0 (S 64, dP 64) and 128; accumulators from here
+
+// Groups of four warps that take the score steps in turn, each with a buffer of S and dP (64 + 64 columns) of its own: as
+// many as fit the 512 TMEM columns beside the accumulators (and Q and dO).  At 64 dims, where the exponentials and not the
+// MMAs set the pace, the third hides the others' latencies.
+template <int DP> struct BwdCfg {
+  static constexpr int kGroups = DP == 64 ? 3 : 2;
+  static constexpr int kSoft = kGroups * 128;         // threads of the score groups
+  static constexpr int kWarps = kGroups * 4;          // their warps; then 1 TMA, 1 issues the scores' MMAs, 1 the gradients'
+  static constexpr int kThreads = kSoft + 96;
+  static constexpr int kStages = DP == 64 ? 6 : 4;    // ring of 64-row (Q, dO) or (K, V) pairs
+  static constexpr uint32_t kColAcc = kGroups * 128;  // score buffer b at 128·b (S, then dP); accumulators from here
+};
 
 template <int DP> struct BwdSmem {
+  using C = BwdCfg<DP>;
   static constexpr int kTile = kPackBlock * DP * 2, kStep = kHalf * DP * 2;
   uint8_t a[2][kTile];               // K and V of the keys, or Q and dO of the queries: per 64 dims 128 rows × 128 bytes
-  uint8_t ring[kStages][2][kStep];   // per 64 dims 64 rows × 128 bytes
-  float4 stats[2][2][2][kHalf / 4];  // dK/dV: −lse·log2 e and −Δ of the step's queries, per group, two steps
-  float red[8];
+  uint8_t ring[C::kStages][2][kStep];   // per 64 dims 64 rows × 128 bytes
+  float4 stats[C::kGroups][2][2][kHalf / 4];  // dK/dV: −lse·log2 e and −Δ of the step's queries, per group, two steps
+  float red[C::kWarps];
   float row_part[2][kPackBlock];     // dQ: Σ P·dP over a group's keys
-  uint64_t a_full, a_ready, full[kStages], empty[kStages], s_full[2], p_full[2], g_done[2], fin;
+  uint64_t a_full, a_ready, full[C::kStages], empty[C::kStages];
+  uint64_t s_full[C::kGroups], p_full[C::kGroups], g_done[C::kGroups], fin;
   uint32_t tmem_base;
   int abort, last;
 };
@@ -78,6 +90,9 @@ struct BwdArgs {
 
 // The four warps of a score group meet; one that gives up arrives without waiting.
 __device__ __forceinline__ void group_leave(int g) { asm volatile("bar.arrive %0, 128;" ::"r"(g + 1) : "memory"); }
+// All score groups.
+template <int N> __device__ __forceinline__ void scores_sync() { asm volatile("bar.sync 4, %0;" ::"n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void scores_leave() { asm volatile("bar.arrive 4, %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
 
 // Largest power of two p with bound·p < 2^15 (1 for a bound of zero; the exponent is kept within ±60).
@@ -101,11 +116,11 @@ template <int DP> __device__ __forceinline__ uint32_t bwd_setup(BwdSmem<DP>& sm,
   if (tid == 0) {
     mbar_init(&sm.a_full, 1);
     mbar_init(&sm.a_ready, 256);
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < BwdCfg<DP>::kStages; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < BwdCfg<DP>::kGroups; ++b) {
       mbar_init(&sm.s_full[b], 1);
       mbar_init(&sm.p_full[b], 128);
       mbar_init(&sm.g_done[b], 1);
@@ -114,7 +129,7 @@ template <int DP> __device__ __forceinline__ uint32_t bwd_setup(BwdSmem<DP>& sm,
     sm.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == BwdCfg<DP>::kWarps) {
     tmem_alloc(&sm.tmem_base, 512);
     tmem_relinquish();
   }
@@ -147,7 +162,7 @@ __device__ __forceinline__ void store16(uint32_t taddr, bool zero, float f, bool
 // Producer: the ring's steps, each two 64-row tiles.  at(h, &head, &row) says where step h begins.
 template <int DP, typename At>
 __device__ __forceinline__ void produce(BwdSmem<DP>& sm, const CUtensorMap* m0, const CUtensorMap* m1, int n, At at) {
-  constexpr int NB = DP / 64;
+  constexpr int NB = DP / 64, kStages = BwdCfg<DP>::kStages;
   bool ok = true;
   int issued = 0;
   for (int h = 0; h < n; ++h) {
@@ -256,11 +271,14 @@ packed_rows_kernel(const uint16_t* __restrict__ out, const uint16_t* __restrict_
 
 // ── dK and dV ────────────────────────────────────────────────────────────────
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
 packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, BwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using C = BwdCfg<DP>;
+  constexpr int kStages = C::kStages;
+  constexpr uint32_t kColAcc = C::kColAcc;
   const PackedShape& ps = a.s;
   let_next_start();
   wait_for_previous();
@@ -275,7 +293,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const bool fine = it.lq <= kFineSteps * kHalf;
   const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
 
-  if (warp == 8) {
+  if (warp == C::kWarps) {
     if (lane == 0 && n > 0) {
       constexpr int NB = DP / 64;
       mbar_arrive_expect_tx(&sm.a_full, 2 * BwdSmem<DP>::kTile);
@@ -291,8 +309,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       });
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ── Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ of step h into buffer h mod 2, once the products of step h − 2 are done with it ──
+  } else if (warp == C::kWarps + 1) {
+    // ── Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ of step h into buffer h mod groups, once the products of its last step are done ──
     if (n > 0) {
       const uint32_t lead = elect_lead(), tm = uniform(tmem);
       const int steps = uniform(n), blocks = uniform(nh), tail = uniform(it.lq - (hb0 + nh - 1) * kHalf);
@@ -300,6 +318,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint64_t dk = sdesc(smem_u32(sm.a[0]), 16, 1024, SW_128B), dv = sdesc(smem_u32(sm.a[1]), 16, 1024, SW_128B);
       const uint64_t dq0 = sdesc(smem_u32(sm.ring[0][0]), 16, 1024, SW_128B);
       constexpr int kABlk = (kPackBlock * 128) >> 4, kBBlk = (kHalf * 128) >> 4, kTileStep = BwdSmem<DP>::kStep >> 4;
+      int buf = 0;       // score buffer of the step
+      uint32_t par = 0;  // parity of its use
+      auto next_buffer = [&] {
+        if (++buf == C::kGroups) buf = 0, par ^= 1;
+      };
       bool ok = wait_all(&sm.a_full, 0, &sm.abort, 2);
       int b = uniform(b0);
       for (int h = 0; ok && h < steps; ++h) {
@@ -314,10 +337,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             __syncwarp();
           }
         }
-        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 6))) break;
+        if (h >= C::kGroups && !(ok = wait_all(&sm.g_done[buf], par ^ 1, &sm.abort, 6))) break;
         tc_fence_after();
         const uint64_t bq = dq0 + (uint64_t)(st * 2 * kTileStep), bo = bq + kTileStep;
-        const uint32_t ts = tm + (h & 1) * 128;
+        const uint32_t ts = tm + buf * 128;
         auto one = [&](int s) {
           const uint64_t oa = (uint64_t)((s >> 2) * kABlk + (s & 3) * 2), ob = (uint64_t)((s >> 2) * kBBlk + (s & 3) * 2);
           mma_ss_p(ts, dk + oa, bq + ob, id_s, s > 0 ? 1u : 0u, lead);
@@ -329,12 +352,13 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         } else {
           for (int s = 0; s < dim16 / 16; ++s) one(s);
         }
-        mma_commit_p(&sm.s_full[h & 1], lead);
+        mma_commit_p(&sm.s_full[buf], lead);
+        next_buffer();
       }
       issue_end(sm, lead);
     }
     __syncwarp();
-  } else if (warp == 10) {
+  } else if (warp == C::kWarps + 2) {
     // ── dV += Pᵀ·dO, dK += dSᵀ·Q ──
     if (n > 0) {
       const bool uniform_fine = uniform(fine);
@@ -343,16 +367,21 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, BF16 ? AB_BF16 : AB_F16, false, true);
       const uint64_t dq0 = sdesc(smem_u32(sm.ring[0][0]), kHalf * 128, 1024, SW_128B);
       constexpr int kTileStep = BwdSmem<DP>::kStep >> 4;
+      int buf = 0;       // score buffer of the step
+      uint32_t par = 0;  // parity of its use
+      auto next_buffer = [&] {
+        if (++buf == C::kGroups) buf = 0, par ^= 1;
+      };
       bool ok = true;
       int b = uniform(b0);
       for (int h = 0; h < steps; ++h) {
         const int st = h % kStages;
         int ks = kHalf / 16;
         if (++b == blocks) b = 0, ks = min(ks, (tail + 15) >> 4);
-        if (!(ok = wait_all(&sm.p_full[h & 1], (h >> 1) & 1, &sm.abort, 4))) break;
+        if (!(ok = wait_all(&sm.p_full[buf], par, &sm.abort, 4))) break;
         tc_fence_after();
         const uint64_t gq = dq0 + (uint64_t)(st * 2 * kTileStep), go = gq + kTileStep;
-        const uint32_t tp = tm + (h & 1) * 128;
+        const uint32_t tp = tm + buf * 128;
         auto one = [&](int s) {
           const uint32_t acc = (h > 0 || s > 0) ? 1u : 0u;
           mma_ts_p(tm + kColAcc, tp + s * 8, go + (uint64_t)(s * (2048 >> 4)), id_g, acc, lead);
@@ -368,14 +397,15 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             mma_ts_p(tm + kColAcc + DP, tp + kHalf + 32 + s * 8, gq + (uint64_t)(s * (2048 >> 4)), id_g, 1u, lead);
           }
         }
-        mma_commit_p(&sm.g_done[h & 1], lead);
+        mma_commit_p(&sm.g_done[buf], lead);
         mma_commit_p(&sm.empty[st], lead);
+        next_buffer();
       }
       issue_end(sm, lead);
     }
     __syncwarp();
   } else {
-    // ── scores: group g takes steps h ≡ g (mod 2), thread = key ──
+    // ── scores: group g takes steps h ≡ g (mod groups), thread = key ──
     const int g = warp >> 2, key = tid - g * 128;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + g * 128;
@@ -386,7 +416,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if constexpr (!BF16) {  // |dS_ij| ≤ max_i ‖dO_i‖ · ‖V_j‖ + max_i |Δ_i|
       const float* norms = reinterpret_cast<const float*>(a.plan + ps.do_norm);
       float top_n = 0.0f, top_d = 0.0f;
-      for (int i = tid; i < nh * kHalf * ps.group; i += 256) {
+      for (int i = tid; i < nh * kHalf * ps.group; i += C::kSoft) {
         const int gh = i / (nh * kHalf), q = hb0 * kHalf + i - gh * nh * kHalf;
         if (q >= it.lq) continue;
         const long long at = (long long)(kvh * ps.group + gh) * ps.total_q + it.q0 + q;
@@ -398,10 +428,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         top_d = fmaxf(top_d, __shfl_xor_sync(0xffffffffu, top_d, o));
       }
       float* red = reinterpret_cast<float*>(sm.stats);
-      if (lane == 0) red[warp] = top_n, red[8 + warp] = top_d;
-      asm volatile("bar.sync 3, 256;" ::: "memory");
-      for (int i = 0; i < 8; ++i) top_n = fmaxf(top_n, red[i]), top_d = fmaxf(top_d, red[8 + i]);
-      asm volatile("bar.sync 3, 256;" ::: "memory");
+      if (lane == 0) red[warp] = top_n, red[C::kWarps + warp] = top_d;
+      scores_sync<C::kSoft>();
+      for (int i = 0; i < C::kWarps; ++i) top_n = fmaxf(top_n, red[i]), top_d = fmaxf(top_d, red[C::kWarps + i]);
+      scores_sync<C::kSoft>();
       const float vn = mine ? reinterpret_cast<const float*>(a.plan + ps.v_norm)[(long long)kvh * ps.total_k + it.k0 + key] : 0.0f;
       mult = pow2_below(top_n * vn + top_d);
     }
@@ -426,8 +456,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (n > 0) advance(g);
     float2 ahead = fetch(g);
     int block = fb;
-    for (int h = g; h < n; h += 2) {
-      const int k = h >> 1;
+    for (int h = g, k = 0; h < n; h += C::kGroups, ++k) {
       if (key < kHalf) {
         reinterpret_cast<float*>(sm.stats[g][k & 1][0])[key] = -ahead.x;
         reinterpret_cast<float*>(sm.stats[g][k & 1][1])[key] = -ahead.y;
@@ -438,8 +467,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         break;
       }
       const int i0 = (hb0 + block) * kHalf;
-      advance(2);
-      ahead = fetch(h + 2);
+      advance(C::kGroups);
+      ahead = fetch(h + C::kGroups);
       block = fb;
       // queries [lo, hi) of the step see this key
       const int lo = ps.causal ? j - off - i0 : 0, hi = it.lq - i0;
@@ -541,7 +570,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_arrive(&sm.p_full[g]);
     }
     if (n > 0) ok = mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 9) && ok;
-    if (ok && !sm.abort) {  // group 0 stores dV, group 1 dK
+    if (ok && !sm.abort && g < 2) {  // group 0 stores dV, group 1 dK
       tc_fence_after();
       const uint32_t acc = tmem + lanes + kColAcc + g * DP;
       const float f = g == 0 ? (BF16 ? 1.0f : 3.0517578125e-05f) : 1.0f / mult;
@@ -572,7 +601,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == C::kWarps) tmem_dealloc(tmem, 512);
 
   if (it.slot < 0 || sm.abort) return;
   // ── the last of a tile's parts to arrive adds them in their order ──
@@ -587,7 +616,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (!sm.last) return;
   const int vecs = ps.dim / 4;
   const long long part_step = (long long)ps.kv_heads * 2 * kPackBlock * ps.dim;
-  for (int i = tid; i < 2 * it.keys * vecs; i += kThreads) {
+  for (int i = tid; i < 2 * it.keys * vecs; i += C::kThreads) {
     const int which = i / (it.keys * vecs), rest = i - which * it.keys * vecs, r = rest / vecs, c = (rest - r * vecs) * 4;
     const float* src = reinterpret_cast<const float*>(a.plan + ps.part_dkv) +
                        ((((long long)it.slot0 * ps.kv_heads + kvh) * 2 + which) * kPackBlock + r) * ps.dim + c;
@@ -606,11 +635,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
 // ── dQ ───────────────────────────────────────────────────────────────────────
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
 packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, BwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using C = BwdCfg<DP>;
+  constexpr int kStages = C::kStages;
+  constexpr uint32_t kColAcc = C::kColAcc;
   const PackedShape& ps = a.s;
   let_next_start();
   wait_for_previous();
@@ -624,7 +656,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   constexpr uint32_t kColQ = kColAcc + DP, kColDO = kColQ + DP / 2;
   const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
 
-  if (warp == 8) {
+  if (warp == C::kWarps) {
     if (lane == 0 && n > 0) {
       constexpr int NB = DP / 64;
       mbar_arrive_expect_tx(&sm.a_full, 2 * BwdSmem<DP>::kTile);
@@ -638,14 +670,19 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       });
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ── S = Q·Kᵀ and dP = dO·Vᵀ of step h into buffer h mod 2, once dQ is done with step h − 2's ──
+  } else if (warp == C::kWarps + 1) {
+    // ── S = Q·Kᵀ and dP = dO·Vᵀ of step h into buffer h mod groups, once dQ is done with its last step's ──
     if (n > 0) {
       const uint32_t lead = elect_lead(), tm = uniform(tmem);
       const int steps = uniform(n), tail = uniform(see_end - (n - 1) * kHalf);
       const uint32_t id_s = idesc_f32acc(kPackBlock, kHalf, BF16 ? AB_BF16 : AB_F16, false, false);
       const uint64_t dk0 = sdesc(smem_u32(sm.ring[0][0]), 16, 1024, SW_128B);
       constexpr int kBBlk = (kHalf * 128) >> 4, kTileStep = BwdSmem<DP>::kStep >> 4;
+      int buf = 0;       // score buffer of the step
+      uint32_t par = 0;  // parity of its use
+      auto next_buffer = [&] {
+        if (++buf == C::kGroups) buf = 0, par ^= 1;
+      };
       bool ok = wait_all(&sm.a_ready, 0, &sm.abort, 12);
       for (int h = 0; ok && h < steps; ++h) {
         const int st = h % kStages;
@@ -655,10 +692,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (h >= 2 && !(ok = wait_all(&sm.g_done[h & 1], ((h >> 1) - 1) & 1, &sm.abort, 16))) break;
+        if (h >= C::kGroups && !(ok = wait_all(&sm.g_done[buf], par ^ 1, &sm.abort, 16))) break;
         tc_fence_after();
         const uint64_t bk = dk0 + (uint64_t)(st * 2 * kTileStep), bv = bk + kTileStep;
-        const uint32_t ts = tm + (h & 1) * 128;
+        const uint32_t ts = tm + buf * 128;
         auto one = [&](int s) {
           const uint64_t ob = (uint64_t)((s >> 2) * kBBlk + (s & 3) * 2);
           mma_ts_p(ts, tm + kColQ + s * 8, bk + ob, id_s, s > 0 ? 1u : 0u, lead);
@@ -670,12 +707,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         } else {
           for (int s = 0; s < dim16 / 16; ++s) one(s);
         }
-        mma_commit_p(&sm.s_full[h & 1], lead);
+        mma_commit_p(&sm.s_full[buf], lead);
+        next_buffer();
       }
       issue_end(sm, lead);
     }
     __syncwarp();
-  } else if (warp == 10) {
+  } else if (warp == C::kWarps + 2) {
     // ── dQ += dS·K ──
     if (n > 0) {
       const uint32_t lead = elect_lead(), tm = uniform(tmem);
@@ -683,14 +721,19 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const uint32_t id_g = idesc_f32acc(kPackBlock, dim16, BF16 ? AB_BF16 : AB_F16, false, true);
       const uint64_t dk0 = sdesc(smem_u32(sm.ring[0][0]), kHalf * 128, 1024, SW_128B);
       constexpr int kTileStep = BwdSmem<DP>::kStep >> 4;
+      int buf = 0;       // score buffer of the step
+      uint32_t par = 0;  // parity of its use
+      auto next_buffer = [&] {
+        if (++buf == C::kGroups) buf = 0, par ^= 1;
+      };
       bool ok = true;
       for (int h = 0; h < steps; ++h) {
         const int st = h % kStages, ks = h == steps - 1 ? (tail + 15) >> 4 : kHalf / 16;
-        if (!(ok = wait_all(&sm.p_full[h & 1], (h >> 1) & 1, &sm.abort, 14))) break;
+        if (!(ok = wait_all(&sm.p_full[buf], par, &sm.abort, 14))) break;
         tc_fence_after();
         const uint64_t gk = dk0 + (uint64_t)(st * 2 * kTileStep);
         auto one = [&](int s) {
-          mma_ts_p(tm + kColAcc, tm + (h & 1) * 128 + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g,
+          mma_ts_p(tm + kColAcc, tm + buf * 128 + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g,
                    (h > 0 || s > 0) ? 1u : 0u, lead);
         };
         if (ks == kHalf / 16 && steps > kFineSteps) {
@@ -699,10 +742,11 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         } else {
           for (int s = 0; s < ks; ++s) one(s);
           for (int s = 0; steps <= kFineSteps && s < ks; ++s)
-            mma_ts_p(tm + kColAcc, tm + (h & 1) * 128 + kHalf + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g, 1u, lead);
+            mma_ts_p(tm + kColAcc, tm + buf * 128 + kHalf + s * 8, gk + (uint64_t)(s * (2048 >> 4)), id_g, 1u, lead);
         }
-        mma_commit_p(&sm.g_done[h & 1], lead);
+        mma_commit_p(&sm.g_done[buf], lead);
         mma_commit_p(&sm.empty[st], lead);
+        next_buffer();
       }
       issue_end(sm, lead);
     }
@@ -720,16 +764,16 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if constexpr (!BF16) {  // |dS_ij| ≤ ‖dO_i‖ · max_j ‖V_j‖ + |Δ_i|
       const float* vn = reinterpret_cast<const float*>(a.plan + ps.v_norm) + (long long)kvh * ps.total_k + it.k0;
       float top = 0.0f;
-      for (int i = tid; i < see_end; i += 256) top = fmaxf(top, vn[i]);
+      for (int i = tid; i < see_end; i += C::kSoft) top = fmaxf(top, vn[i]);
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (lane == 0) sm.red[warp] = top;
-      asm volatile("bar.sync 3, 256;" ::: "memory");
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, sm.red[i]);
+      scores_sync<C::kSoft>();
+      for (int i = 0; i < C::kWarps; ++i) top = fmaxf(top, sm.red[i]);
       if (mine) mult = pow2_below(reinterpret_cast<const float*>(a.plan + ps.do_norm)[at] * top + fabsf(stat.y));
     }
     const float scale2 = a.scale * kLog2e;
     bool ok = true;
-    if (n > 0) {
+    if (n > 0 && g < 2) {
       // group 0 moves Q, group 1 dO from shared memory to TMEM: a thread its row
       ok = mbar_wait(&sm.a_full, 0, &sm.abort, &g_packed_bwd_status, 17);
       if (ok) {
@@ -748,12 +792,12 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         mbar_arrive(&sm.a_ready);
       }
     }
-    if (ok && n > 0 && n <= kFineSteps) {
+    if (n > 0 && n <= kFineSteps) {
       // Rows that see at most 128 keys: all their scores are in the two buffers, so Δ_i = Σ_j P_ij dP_ij is summed from
       // them.  dO·O carries the rounding of the stored O, which matters here (O is an average of few values): it
       // would add as much error to dQ and dK as the rounding of dS.  The dK/dV kernel reads the better Δ too.
       float t = 0.0f;
-      if (g < n && (ok = mbar_wait(&sm.s_full[g], 0, &sm.abort, &g_packed_bwd_status, 20))) {
+      if (ok && g < n && (ok = mbar_wait(&sm.s_full[g], 0, &sm.abort, &g_packed_bwd_status, 20))) {
         tc_fence_after();
         const int limit = see - g * kHalf;
 #pragma unroll
@@ -771,18 +815,18 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         }
       }
-      sm.row_part[g][row] = t;
+      if (g < 2) sm.row_part[g][row] = t;
       if (ok) {
-        asm volatile("bar.sync 3, 256;" ::: "memory");
+        scores_sync<C::kSoft>();
         ok = !*(volatile int*)&sm.abort;
       } else {
-        asm volatile("bar.arrive 3, 256;" ::: "memory");
+        scores_leave<C::kSoft>();
       }
       stat.y = sm.row_part[0][row] + sm.row_part[1][row];
       if (mine && ok && g == 0) reinterpret_cast<float2*>(a.plan + ps.rows)[at].y = stat.y;
     }
-    for (int h = g; ok && h < n; h += 2) {
-      if (!(ok = mbar_wait(&sm.s_full[g], (h >> 1) & 1, &sm.abort, &g_packed_bwd_status, 18))) break;
+    for (int h = g, k = 0; ok && h < n; h += C::kGroups, ++k) {
+      if (!(ok = mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 18))) break;
       tc_fence_after();
       const int limit = see - h * kHalf;
       auto scores = [&](auto masked, auto fine) {
@@ -824,13 +868,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (ok && !sm.abort) {  // each group stores half of the 16-column chunks
       tc_fence_after();
       uint16_t* out = static_cast<uint16_t*>(a.dq) + (it.q0 + row) * a.dq_row + head * a.dq_head;
-      for (int c = g * 16; c < dim16; c += 32)
+      for (int c = g * 16; c < dim16; c += C::kGroups * 16)
         store16<BF16>(tmem + lanes + kColAcc, n == 0, a.scale / mult, mine, out, c, ps.dim);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == C::kWarps) tmem_dealloc(tmem, 512);
 }
 
 template <typename K> int set_smem(K kernel, int smem) {
@@ -853,12 +897,12 @@ template <int DP, bool BF16> int launch_bwd(const BwdMaps& m, const BwdArgs& a, 
   const long long g1 = (long long)a.s.max_dkv_items * a.s.kv_heads, g2 = (long long)a.s.max_dq_items * a.s.heads;
   VA_CHECK_ARG(g1 < (1LL << 31) && g2 < (1LL << 31), "packed attention backward: too many units");
   if (g2 > 0) {
-    if (int rc = launch_behind("packed attention dQ", packed_dq_kernel<DP, BF16>, (unsigned)g2, kThreads, smem, st,
+    if (int rc = launch_behind("packed attention dQ", packed_dq_kernel<DP, BF16>, (unsigned)g2, BwdCfg<DP>::kThreads, smem, st,
                                m.q_tile, m.do_tile, m.k_step, m.v_step, a))
       return rc;
   }
   if (g1 > 0) {
-    if (int rc = launch_behind("packed attention dK/dV", packed_dkv_kernel<DP, BF16>, (unsigned)g1, kThreads, smem, st,
+    if (int rc = launch_behind("packed attention dK/dV", packed_dkv_kernel<DP, BF16>, (unsigned)g1, BwdCfg<DP>::kThreads, smem, st,
                                m.q_step, m.do_step, m.k_tile, m.v_tile, a))
       return rc;
   }

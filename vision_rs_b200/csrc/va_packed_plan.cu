@@ -26,8 +26,8 @@ struct Seq {
   int q0, lq, k0, lk;
 };
 
-__device__ __forceinline__ Seq load_seq(const int* cu_q, const int* cu_k, const int* used_k, int b, int total_q,
-                                       int total_k, int* bad) {
+__device__ __forceinline__ Seq load_seq(const int* cu_q, const int* cu_k, const int* used_k, int num_seqs, int b,
+                                       int total_q, int total_k, int* bad) {
   const int a0 = cu_q[b], a1 = cu_q[b + 1], c0 = cu_k[b], c1 = cu_k[b + 1];
   Seq s;
   s.q0 = min(max(a0, 0), total_q);
@@ -43,6 +43,7 @@ __device__ __forceinline__ Seq load_seq(const int* cu_q, const int* cu_k, const 
     *bad = 1;
   }
   if (s.q0 != a0 || s.lq != a1 - a0 || s.k0 != c0 || (b == 0 && (a0 != 0 || c0 != 0))) *bad = 1;
+  if (b == num_seqs - 1 && (a1 != total_q || c1 != total_k)) *bad = 1;  // rows of no sequence would stay unwritten
   return s;
 }
 
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
     const int b = b0 + tid;
     int n = 0;
     if (b < s.num_seqs) {
-      const Seq q = load_seq(a.cu_q, a.cu_k, a.used_k, b, s.total_q, s.total_k, &bad);
+      const Seq q = load_seq(a.cu_q, a.cu_k, a.used_k, s.num_seqs, b, s.total_q, s.total_k, &bad);
       n = ((list == 2 ? q.lk : q.lq) + tile - 1) / tile;
     }
     int sum;
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
       return own_range;
     }
     const int b = seq_of_tile(first, s.num_seqs, t);
-    *q = load_seq(a.cu_q, a.cu_k, a.used_k, b, s.total_q, s.total_k, &bad);
+    *q = load_seq(a.cu_q, a.cu_k, a.used_k, s.num_seqs, b, s.total_q, s.total_k, &bad);
     *i0 = (t - first[b]) * tile;
     const Range r =
         list == 2 ? query_steps(*q, *i0, s.causal, s.group) : key_blocks(*q, *i0, min(tile, q->lq - *i0), s.causal);
