@@ -71,6 +71,16 @@ template <typename OP, int TPR> __device__ __forceinline__ float row_all(float v
   return v;
 }
 
+// 8 bits: y/s needs no r (y = h·w·r, s = max|y|/448), so the row's h·w is scaled by 448 / max|h·w| directly: two
+// roundings an element less, each of which can tip a value over to the next of the 8-bit grid.
+struct Quant {
+  float amax, mul;  // max|y|, and what h·w is multiplied by
+};
+__device__ __forceinline__ Quant quant_of(float top, float r) {  // top: max|h·w|
+  const float y = top * r, amax = max_nan(y, kSmallestAmax);
+  return {amax, y >= kSmallestAmax ? kE4M3Max / top : r * (kE4M3Max / amax)};
+}
+
 struct NormArgs {
   const void *x, *res, *w;
   void *h, *y;
@@ -163,34 +173,38 @@ __global__ void __launch_bounds__(block_threads(TPR)) rms_norm_kernel(NormArgs a
       load_w<T>(a.w, a.w_f32, c * VEC, w);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        v[i][j] = v[i][j] * r * w[j];
-        if constexpr (F8) top = max_nan_abs(top, v[i][j]);
+        if constexpr (F8) {
+          v[i][j] *= w[j];
+          top = max_nan_abs(top, v[i][j]);
+        } else {
+          v[i][j] = v[i][j] * r * w[j];
+        }
       }
       if constexpr (!F8) reinterpret_cast<uint4*>(static_cast<T*>(a.y) + base)[c] = B::put(v[i]);
     }
   }
   if constexpr (F8) {
     const bool whole = a.group == a.cols;
+    Quant z{};
     if (whole) {
-      top = max_nan(row_all<Max, TPR>(top, red[1]), kSmallestAmax);
-      if (t == 0) a.scale[row] = top / kE4M3Max;
+      z = quant_of(row_all<Max, TPR>(top, red[1]), r);
+      if (t == 0) a.scale[row] = z.amax / kE4M3Max;
     }
     const int lanes = a.group / VEC;  // of one group (a power of two ≤ 32 unless the group is the row)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t + i * TPR;
-      float m = top;
       if (!whole) {
-        m = 0.0f;
+        float m = 0.0f;
         if (c < nvec) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) m = max_nan_abs(m, v[i][j]);
         }
-        m = max_nan(warp_all<Max>(m, lanes), kSmallestAmax);
-        if (c < nvec && (t & (lanes - 1)) == 0) a.scale[row * (a.cols / a.group) + c / lanes] = m / kE4M3Max;
+        z = quant_of(warp_all<Max>(m, lanes), r);
+        if (c < nvec && (t & (lanes - 1)) == 0) a.scale[row * (a.cols / a.group) + c / lanes] = z.amax / kE4M3Max;
       }
       if (c < nvec) {
-        const float inv = kE4M3Max / m;
+        const float inv = z.mul;
         uint32_t q[VEC / 4];
 #pragma unroll
         for (int j = 0; j < VEC; j += 4)
@@ -221,22 +235,20 @@ __global__ void __launch_bounds__(256) rms_norm_any_kernel(NormArgs a) {
   const float r = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
   if constexpr (F8) {
     const bool whole = a.group == a.cols;
-    float top = 0.0f;
     if (whole) {
-      for (int c = threadIdx.x; c < a.cols; c += 256) top = max_nan(top, fabsf(at(c) * r * weight(c)));
-      top = max_nan(row_all<Max, 256>(top, red[1]), kSmallestAmax);
-      if (threadIdx.x == 0) a.scale[row] = top / kE4M3Max;
-      for (int c = threadIdx.x; c < a.cols; c += 256)
-        a.q[base + c] = to_e4m3(at(c) * r * weight(c) * (kE4M3Max / top));
+      float top = 0.0f;
+      for (int c = threadIdx.x; c < a.cols; c += 256) top = max_nan_abs(top, at(c) * weight(c));
+      const Quant z = quant_of(row_all<Max, 256>(top, red[1]), r);
+      if (threadIdx.x == 0) a.scale[row] = z.amax / kE4M3Max;
+      for (int c = threadIdx.x; c < a.cols; c += 256) a.q[base + c] = to_e4m3(at(c) * weight(c) * z.mul);
     } else {
       const int ng = a.cols / a.group, lane = threadIdx.x & 31;
       for (int g = threadIdx.x >> 5; g < ng; g += 8) {  // a warp for each group
         float m = 0.0f;
-        for (int c = lane; c < a.group; c += 32) m = max_nan(m, fabsf(at(g * a.group + c) * r * weight(g * a.group + c)));
-        m = max_nan(warp_all<Max>(m), kSmallestAmax);
-        if (lane == 0) a.scale[row * ng + g] = m / kE4M3Max;
-        for (int c = g * a.group + lane; c < (g + 1) * a.group; c += 32)
-          a.q[base + c] = to_e4m3(at(c) * r * weight(c) * (kE4M3Max / m));
+        for (int c = lane; c < a.group; c += 32) m = max_nan_abs(m, at(g * a.group + c) * weight(g * a.group + c));
+        const Quant z = quant_of(warp_all<Max>(m), r);
+        if (lane == 0) a.scale[row * ng + g] = z.amax / kE4M3Max;
+        for (int c = g * a.group + lane; c < (g + 1) * a.group; c += 32) a.q[base + c] = to_e4m3(at(c) * weight(c) * z.mul);
       }
     }
   }
