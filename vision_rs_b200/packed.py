@@ -88,9 +88,8 @@ class PackedPlan:
             raise ValueError("cu_q or cu_k are not ascending offsets from 0 to the number of tokens")
 
     def _use(self):
-        """The buffer must outlive a call on another stream than the plan's own."""
-        if _launch.raw_stream(self.index) != self.stream:
-            self.buf.record_stream(torch.cuda.current_stream(self.index))
+        """For a call on another stream than the plan's own: the buffer must outlive it."""
+        self.buf.record_stream(torch.cuda.current_stream(self.index))
 
 
 def _heads(t, name, dtype, index, shape):
@@ -122,13 +121,16 @@ def packed_attention_forward(q, k, v, plan: PackedPlan, scale: float | None = No
         raise ValueError("q must be bf16 or f16")
     _, tq, tk, h, hk, d, _, _ = sizes
     sq, sk = (tq, h, d), (tk, hk, d)
-    strides = _Strides6(*_heads(q, "q", dtype, index, sq), *_heads(k, "k", dtype, index, sk),
-                        *_heads(v, "v", dtype, index, sk))
-    out = q.new_empty(sq) if out is None else _dense(out, "out", sq, dtype, index)
+    q_row, q_head = _heads(q, "q", dtype, index, sq)
+    k_row, k_head = _heads(k, "k", dtype, index, sk)
+    v_row, v_head = _heads(v, "v", dtype, index, sk)
+    out = q.new_empty_strided(sq, (h * d, d, 1)) if out is None else _dense(out, "out", sq, dtype, index)
     lse = q.new_empty((h, tq), dtype=torch.float32) if lse is None else _dense(lse, "lse", (h, tq), torch.float32, index)
-    plan._use()
-    _launch.run(name, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), strides, *sizes,
-                d ** -0.5 if scale is None else scale, plan.ptr, plan.nbytes)
+    if _launch.raw_stream(index) != plan.stream:
+        plan._use()
+    _launch.run(name, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                _Strides6(q_row, q_head, k_row, k_head, v_row, v_head), *sizes, d ** -0.5 if scale is None else scale,
+                plan.ptr, plan.nbytes)
     return out, lse
 
 
@@ -155,7 +157,8 @@ def packed_attention_backward(grad_out, q, k, v, out, lse, plan: PackedPlan, sca
                          *_heads(v, "v", dtype, index, sk), *_heads(grad_out, "grad_out", dtype, index, sq),
                          *_heads(gq, "grad_q", dtype, index, sq), *_heads(gk, "grad_k", dtype, index, sk),
                          *_heads(gv, "grad_v", dtype, index, sk))
-    plan._use()
+    if _launch.raw_stream(index) != plan.stream:
+        plan._use()
     _launch.run(name, index, grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                 lse.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), strides, *sizes,
                 d ** -0.5 if scale is None else scale, plan.ptr, plan.nbytes)

@@ -17,10 +17,10 @@ _FWD, _F8, _BWD = ({t: f"va_rms_norm_{kind}_{s}" for t, s in _SFX.items()} for k
 
 def _rows(t):
     """(device index, rows, cols) of the tensor that the others are held to."""
-    index = t.get_device()
-    if index < 0 or t.dtype not in _SFX or not t.is_contiguous() or t.dim() == 0:
+    index, shape = t.get_device(), t.shape
+    if index < 0 or t.dtype not in _SFX or not shape or not t.is_contiguous():
         raise ValueError("rows must be contiguous CUDA tensors of bf16, f16 or f32")
-    cols = t.shape[-1]
+    cols = shape[-1]
     return index, (t.numel() // cols if cols else 0), cols
 
 
@@ -75,9 +75,8 @@ def rms_norm_forward_f8(x, w, residual=None, eps: float = 1e-6, group: int = 0, 
         raise ValueError(f"{cols} columns do not split into groups of {group}")
     pw, w32 = _weight(w, x, index, cols)
     pr, ph, h = _sum(x, residual, out_h, index)
-    shape = x.shape
-    q = x.new_empty(shape, dtype=torch.float8_e4m3fn)
-    scale = x.new_empty(shape[:-1] + (cols // group if group else 1,), dtype=torch.float32)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty((*x.shape[:-1], cols // group if group else 1), dtype=torch.float32)
     _launch.run(_F8[x.dtype], index, x.data_ptr(), pr, pw, w32, ph, q.data_ptr(), scale.data_ptr(), rows, cols, group,
                 eps)
     return q, scale, h

@@ -45,61 +45,59 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, stretch: float = 1.0
     return inv.to(device)
 
 
-def _heads(t, name, dtype, index):
-    if t.dtype is not dtype or t.get_device() != index or t.dim() != 3:
-        raise ValueError(f"{name} must be a CUDA [tokens, heads, head_dim] tensor of q's type and device")
-    if t.stride(2) != 1 and t.shape[2] > 1:
-        raise ValueError(f"{name}: a head's dimensions must be contiguous")
-
-
 def _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, stream):
     if stream is not None:
         with _launch.on(stream):
             return _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, None)
     dtype, index = q.dtype, q.get_device()
     name = _ENTRY.get(dtype)
-    if name is None or index < 0:
-        raise ValueError("q must be a CUDA tensor of bf16, f16 or f32")
-    _heads(q, "q", dtype, index)
-    tokens, hq, dim = shape = q.shape
-    hk = 0
+    if name is None or index < 0 or q.dim() != 3:
+        raise ValueError("q must be a CUDA [tokens, heads, head_dim] tensor of bf16, f16 or f32")
+    shape = tokens, heads, dim = q.shape
+    q_row, q_head, one = q.stride()
+    pk = pko = ko = None
+    kv_heads = k_row = k_head = ko_row = ko_head = 0
     if k is not None:
-        _heads(k, "k", dtype, index)
-        tk, hk, dk = k.shape
-        if tk != tokens or dk != dim:
+        if k.dtype is not dtype or k.get_device() != index or k.dim() != 3:
+            raise ValueError("k must be a [tokens, heads, head_dim] tensor of q's type and device")
+        k_tokens, kv_heads, k_dim = k_shape = k.shape
+        k_row, k_head, k_one = k.stride()
+        if k_tokens != tokens or k_dim != dim:
             raise ValueError("q and k must have the same tokens and head_dim")
-    if positions.get_device() != index or positions.dtype not in _POSITION or positions.shape != (tokens,) \
+        one = one if k_one == 1 else k_one
+        pk = k.data_ptr()
+    position_bytes = _POSITION.get(positions.dtype)
+    if position_bytes is None or positions.get_device() != index or positions.shape != (tokens,) \
             or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous CUDA int32 or int64 [tokens] tensor")
-    if inv_freq.get_device() != index or inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 \
+    if inv_freq.dtype is not torch.float64 or inv_freq.get_device() != index or inv_freq.dim() != 1 \
             or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous CUDA float64 [rot_dim/2] tensor")
-    rot = 2 * inv_freq.shape[0]
+    rot = 2 * inv_freq.numel()
     if rot > dim:
         raise ValueError(f"{rot} rotated dimensions in heads of {dim}")
     if out is None:
-        qo = q.new_empty(shape)
-        ko = None if k is None else k.new_empty(k.shape)
+        qo = torch.empty_like(q)  # dense
+        if k is not None:
+            ko = torch.empty_like(k)
     else:
         qo, ko = out
-        if (k is None) != (ko is None):
+        if (k is None) != (ko is None) or qo.shape != shape or (ko is not None and ko.shape != k_shape):
             raise ValueError("outputs must have the inputs' shapes")
-        for o, x in ((qo, q), (ko, k)):
-            if o is not None:
-                _heads(o, "an output", dtype, index)
-                if o.shape != x.shape:
-                    raise ValueError("outputs must have the inputs' shapes")
-    a, b, _ = q.stride()
-    e, f, _ = qo.stride()
-    if k is None:
-        strides, pk, pko = _Strides(a, b, 0, 0, e, f, 0, 0), None, None
-    else:
-        c, d, _ = k.stride()
-        g, h, _ = ko.stride()
-        strides, pk, pko = _Strides(a, b, c, d, e, f, g, h), k.data_ptr(), ko.data_ptr()
-    _launch.run(name, index, q.data_ptr(), pk, qo.data_ptr(), pko, strides, positions.data_ptr(),
-                _POSITION[positions.dtype], inv_freq.data_ptr(), tokens, hq, hk, dim, rot, int(interleaved), backward,
-                factor)
+        for o in (qo, ko):
+            if o is not None and (o.dtype is not dtype or o.get_device() != index):
+                raise ValueError("outputs must have the inputs' type and device")
+    qo_row, qo_head, o_one = qo.stride()
+    one = one if o_one == 1 else o_one
+    if ko is not None:
+        ko_row, ko_head, o_one = ko.stride()
+        one = one if o_one == 1 else o_one
+        pko = ko.data_ptr()
+    if one != 1 and dim > 1:
+        raise ValueError("a head's dimensions must be contiguous")
+    _launch.run(name, index, q.data_ptr(), pk, qo.data_ptr(), pko,
+                _Strides(q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head), positions.data_ptr(),
+                position_bytes, inv_freq.data_ptr(), tokens, heads, kv_heads, dim, rot, interleaved, backward, factor)
     return qo, ko
 
 
