@@ -82,8 +82,9 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   s.q_tile = s.few ? s.tile_rows / s.group : 2 * kPackBlock;
   s.units = s.few ? kv_heads : heads;
   s.max_tiles = (int)std::min<long long>((total_q + s.q_tile - 1) / s.q_tile + (long long)num_seqs, total_q);
-  // Parts over the number of tiles: enough for four units an SM slot, and no more than the longest possible tiles allow
-  // (none where no tile can pass the smallest part).
+  // Parts over the number of tiles: about two units for each place a CTA has on the GPU (forward), one an SM (dK/dV, whose
+  // parts are larger to join: 507 us for a causal step of 10 k tokens against 516 with half as many more and 520 with
+  // twice), and no more than the longest possible tiles allow (none where no tile can pass the smallest part).
   auto budget = [](int most, long long tiles, long long longest, int smallest) {
     return longest <= smallest ? 0 : (int)std::min<long long>(most, (tiles * longest + smallest - 1) / smallest);
   };
@@ -93,7 +94,7 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   s.max_slots = 2 * s.split_budget;
   s.max_dq_items = training ? (int)std::min<long long>((total_q + 127) / 128 + (long long)num_seqs, total_q) : 0;
   s.max_dkv_tiles = training ? (int)std::min<long long>((total_k + 127) / 128 + (long long)num_seqs, total_k) : 0;
-  s.dkv_budget = training ? budget((296 + kv_heads - 1) / kv_heads, s.max_dkv_tiles,
+  s.dkv_budget = training ? budget((148 + kv_heads - 1) / kv_heads, s.max_dkv_tiles,
                                    ((long long)total_q + 63) / 64 * s.group, kMinQuerySteps)
                           : 0;
   s.max_dkv_items = s.max_dkv_tiles + s.dkv_budget;

@@ -571,6 +571,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       uint16_t* out = static_cast<uint16_t*>(a.out) + ((long long)(it.q0 + t) * ps.heads + h) * ps.dim;
       for (int c = lane * 4; c < ps.dim; c += 128) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int k = 0; k < it.parts; ++k) {
           const float w = exp2f((__ldcg(plse + base + k * step + r) - ref) * kLog2e) * inv;
           const float4 f = __ldcg(reinterpret_cast<const float4*>(po + (base + k * step + r) * ps.dim + c));

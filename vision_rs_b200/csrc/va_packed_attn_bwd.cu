@@ -220,52 +220,55 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
   }
 }
 
-// 16 lanes a (token, head) row.  Rows below nq: Δ of a query; the rest (f16): ‖V_j‖.
+// 16 lanes a row, four rows in flight.  blockIdx.y below heads: Δ of a query head's tokens; the rest (f16): ‖V_j‖ of a key head's.
+constexpr int kRowsBlock = 64;
 template <bool BF16>
 __global__ void __launch_bounds__(256)
 packed_rows_kernel(const uint16_t* __restrict__ out, const uint16_t* __restrict__ d_out, long long do_row,
                    long long do_head, const uint16_t* __restrict__ v, long long v_row, long long v_head,
                    const float* __restrict__ lse, float2* __restrict__ pairs, float* __restrict__ do_norm,
-                   float* __restrict__ v_norm, int total_q, int total_k, int heads, int kv_heads, int dim) {
+                   float* __restrict__ v_norm, int total_q, int total_k, int heads, int dim) {
   let_next_start();
   wait_for_previous();
-  const long long r = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), nq = (long long)total_q * heads;
-  const int c = (threadIdx.x & 15) * 8;
-  float dot = 0.0f, sq = 0.0f;
-  const bool is_q = r < nq, in = r < nq + (BF16 ? 0 : (long long)total_k * kv_heads);
-  int t = 0, h = 0;
-  if (in) {
-    const int hn = is_q ? heads : kv_heads;
-    const long long rr = is_q ? r : r - nq;
-    t = (int)(rr / hn), h = (int)(rr - (long long)t * hn);
-    if (c < dim) {
-      float a[8], b[8];
-      if (is_q) {
-        unpack8<BF16>(*reinterpret_cast<const uint4*>(out + r * dim + c), a);
-        unpack8<BF16>(*reinterpret_cast<const uint4*>(d_out + t * do_row + h * do_head + c), b);
+  const bool is_q = (int)blockIdx.y < heads;
+  const int h = is_q ? blockIdx.y : blockIdx.y - heads, total = is_q ? total_q : total_k;
+  const int t0 = blockIdx.x * kRowsBlock + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
+  if ((int)blockIdx.x * kRowsBlock >= total) return;
+  uint4 ua[4], ub[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dot = fmaf(a[i], b[i], dot);
-      } else {
-        unpack8<BF16>(*reinterpret_cast<const uint4*>(v + t * v_row + h * v_head + c), b);
-      }
-      if constexpr (!BF16) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sq = fmaf(b[i], b[i], sq);
-      }
+  for (int u = 0; u < 4; ++u) {
+    const long long t = t0 + u * 16;
+    ua[u] = ub[u] = make_uint4(0, 0, 0, 0);
+    if (t < total && c < dim) {
+      if (is_q) ua[u] = *reinterpret_cast<const uint4*>(out + (t * heads + h) * dim + c);
+      ub[u] = *reinterpret_cast<const uint4*>(is_q ? d_out + t * do_row + h * do_head + c : v + t * v_row + h * v_head + c);
     }
   }
 #pragma unroll
-  for (int o = 8; o; o >>= 1) {
-    dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if constexpr (!BF16) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-  }
-  if (!in || (threadIdx.x & 15)) return;
-  if (is_q) {
-    const long long at = (long long)h * total_q + t;
-    pairs[at] = make_float2(lse[at] * kLog2e, dot);
-    if constexpr (!BF16) do_norm[at] = sqrtf(sq);
-  } else if constexpr (!BF16) {
-    v_norm[(long long)h * total_k + t] = sqrtf(sq);
+  for (int u = 0; u < 4; ++u) {
+    const int t = t0 + u * 16;
+    float a[8], b[8], dot = 0.0f, sq = 0.0f;
+    unpack8<BF16>(ua[u], a);
+    unpack8<BF16>(ub[u], b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      dot = fmaf(a[i], b[i], dot);
+      if constexpr (!BF16) sq = fmaf(b[i], b[i], sq);
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) {
+      dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if constexpr (!BF16) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    }
+    if (t < total && (threadIdx.x & 15) == 0) {
+      const long long at = (long long)h * total + t;
+      if (is_q) {
+        pairs[at] = make_float2(lse[at] * kLog2e, dot);
+        if constexpr (!BF16) do_norm[at] = sqrtf(sq);
+      } else if constexpr (!BF16) {
+        v_norm[at] = sqrtf(sq);
+      }
+    }
   }
 }
 
@@ -616,20 +619,38 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (!sm.last) return;
   const int vecs = ps.dim / 4;
   const long long part_step = (long long)ps.kv_heads * 2 * kPackBlock * ps.dim;
-  for (int i = tid; i < 2 * it.keys * vecs; i += C::kThreads) {
-    const int which = i / (it.keys * vecs), rest = i - which * it.keys * vecs, r = rest / vecs, c = (rest - r * vecs) * 4;
-    const float* src = reinterpret_cast<const float*>(a.plan + ps.part_dkv) +
-                       ((((long long)it.slot0 * ps.kv_heads + kvh) * 2 + which) * kPackBlock + r) * ps.dim + c;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < it.parts; ++k) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(src + k * part_step));
-      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  const int all = 2 * it.keys * vecs;
+  constexpr int kTogether = 4;  // vectors of a thread that are in flight together
+  for (int i0 = tid; i0 < all; i0 += kTogether * C::kThreads) {
+    float4 sum[kTogether];
+    const float* src[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int i = min(i0 + u * C::kThreads, all - 1), which = i / (it.keys * vecs), rest = i - which * it.keys * vecs;
+      const int r = rest / vecs, c = (rest - r * vecs) * 4;
+      src[u] = reinterpret_cast<const float*>(a.plan + ps.part_dkv) +
+               ((((long long)it.slot0 * ps.kv_heads + kvh) * 2 + which) * kPackBlock + r) * ps.dim + c;
+      sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const float f = which ? a.scale : 1.0f;
-    const long long row = it.k0 + r;
-    uint16_t* out = which ? static_cast<uint16_t*>(a.dk) + row * a.dk_row + kvh * a.dk_head
-                          : static_cast<uint16_t*>(a.dv) + row * a.dv_row + kvh * a.dv_head;
-    *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2<BF16>(sum.x * f, sum.y * f), pack2<BF16>(sum.z * f, sum.w * f));
+    for (int k = 0; k < it.parts; ++k) {
+      float4 v[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) v[u] = __ldcg(reinterpret_cast<const float4*>(src[u] + k * part_step));
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) sum[u].x += v[u].x, sum[u].y += v[u].y, sum[u].z += v[u].z, sum[u].w += v[u].w;
+    }
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int i = i0 + u * C::kThreads;
+      if (i >= all) continue;
+      const int which = i / (it.keys * vecs), rest = i - which * it.keys * vecs, r = rest / vecs, c = (rest - r * vecs) * 4;
+      const float f = which ? a.scale : 1.0f;
+      const long long row = it.k0 + r;
+      uint16_t* out = which ? static_cast<uint16_t*>(a.dk) + row * a.dk_row + kvh * a.dk_head
+                            : static_cast<uint16_t*>(a.dv) + row * a.dv_row + kvh * a.dv_head;
+      *reinterpret_cast<uint2*>(out + c) =
+          make_uint2(pack2<BF16>(sum[u].x * f, sum[u].y * f), pack2<BF16>(sum[u].z * f, sum[u].w * f));
+    }
   }
 }
 
@@ -952,16 +973,18 @@ int packed_bwd(const void* d_out, const void* q, const void* k, const void* v, c
     if (int rc = packed_map(step ? &m.k_step : &m.k_tile, mk, BF16, nk, hk, dim, sk[0], sk[1], 1, rows, "k")) return rc;
     if (int rc = packed_map(step ? &m.v_step : &m.v_tile, mv, BF16, nk, hk, dim, sv[0], sv[1], 1, rows, "v")) return rc;
   }
-  const long long rows = (long long)total_q * heads + (BF16 ? 0 : (long long)total_k * kv_heads);
-  VA_CHECK_ARG((rows + 15) / 16 < (1LL << 31), "packed attention backward: too many rows");
-  if (rows > 0) {
-    if (int rc = launch_behind("packed attention backward rows", packed_rows_kernel<BF16>, (unsigned)((rows + 15) / 16),
-                               256, 0, st, static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(d_out),
-                               strides[6], strides[7], static_cast<const uint16_t*>(v), strides[4], strides[5], lse,
-                               reinterpret_cast<float2*>(a.plan + a.s.rows),
-                               reinterpret_cast<float*>(a.plan + a.s.do_norm),
-                               reinterpret_cast<float*>(a.plan + a.s.v_norm), total_q, total_k, heads, kv_heads, dim))
-      return rc;
+  {
+    // queries' heads, and for f16 the key heads
+    const int tokens = BF16 ? total_q : std::max(total_q, total_k), y = (total_q ? heads : 0) + (BF16 ? 0 : kv_heads);
+    if (tokens > 0)
+      if (int rc = launch_behind("packed attention backward rows", packed_rows_kernel<BF16>,
+                                 dim3((tokens + kRowsBlock - 1) / kRowsBlock, y), 256, 0, st,
+                                 static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(d_out), strides[6],
+                                 strides[7], static_cast<const uint16_t*>(v), strides[4], strides[5], lse,
+                                 reinterpret_cast<float2*>(a.plan + a.s.rows),
+                                 reinterpret_cast<float*>(a.plan + a.s.do_norm),
+                                 reinterpret_cast<float*>(a.plan + a.s.v_norm), total_q, total_k, total_q ? heads : 0, dim))
+        return rc;
   }
   return dim <= 64 ? launch_bwd<64, BF16>(m, a, st) : launch_bwd<128, BF16>(m, a, st);
 }
