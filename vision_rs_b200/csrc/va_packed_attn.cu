@@ -14,21 +14,32 @@
 //     the query heads of a key head read its keys once, over a part of the
 //     keys; two CTAs an SM.  The last CTA of a tile's parts to arrive joins
 //     them in the parts' order (single tokens, few queries).
-// Warps: 4 a tile for the softmax (a thread owns a row), 1 a tile to issue
-// its MMAs, 1 TMA producer.  Per 128-key step: S = Q·Kᵀ into TMEM, the row's p = 2^(s −
-// reference) back into the same columns as 16-bit P, O += P·V with P as the
-// TMEM operand.  The reference only follows the row maximum when it grows by
-// more than 2^8, so O is rarely rescaled.  P is held in the inputs' 16-bit
-// type (rows of at most 128 keys: with its remainder as a second operand); its
-// rounding adds about as much error as that of the output.  Sums, maxima and
-// O stay f32.
+// Warps: 4 a tile for the softmax (a thread owns a row), 1 a tile to issue its
+// MMAs, 1 TMA producer.  Per 64-key step: S = Q·Kᵀ into one of the tile's two
+// score buffers in TMEM, the row's p = 2^(s − reference) back into the same
+// columns as 16-bit P, O += P·V with P as the TMEM operand; the scores of step
+// h + 2 follow step h's product into its buffer while the softmax is on h + 1.
+// The reference only follows the row maximum when it grows by more than 2^8,
+// so O is rarely rescaled.  P is held in the inputs' 16-bit type (rows of at
+// most 128 keys: with its remainder as a second operand); its rounding adds
+// about as much error as that of the output.  Sums, maxima and O stay f32.
+//
+// Measured (sustained; B200): prompts of 2049 and 8191 tokens, 16/2 heads of
+// 128, causal, 297 µs = 0.98 PFLOP/s (254 µs before the power limit acts;
+// floor 177): bound by issuing the MMAs and by the shared-memory reads of the
+// N = 64 score MMAs.  16 images of 257–1601 tokens, 6 heads of 64, 60 µs (floor
+// 21, the exponentials): bound by the softmax's latencies between them.  64
+// single tokens over 17–8192 keys, 32/8 heads of 128, 203 µs = 5.3 TB/s: HBM.
+// One 128-key buffer a tile instead of two of 64 keys: 339 against 264 µs for
+// the prompts; one issuing warp for both tiles: 410.
 //
 // What a row does not see stays out of it, whatever it holds (another
 // sequence's rows in a box, unused rows of a cache, later keys): scores of such
-// keys are replaced, not added to, and as 0 · NaN would be NaN, a warp of its
-// own checks the V blocks that hold them: rows past the unit's last key become
-// zeros, values that are not finite are left out of the product and given back
-// to the rows that do see them.  The MMAs stop at the last 16-key group in use.
+// keys are replaced, not added to, and as 0 · NaN would be NaN, the V blocks
+// that hold them are checked (by a warp of its own, or by the producer of a
+// one-tile unit): rows past the unit's last key become zeros, values that are
+// not finite are left out of the product and given back to the rows that do
+// see them.  The MMAs stop at the last 16-key group in use.
 #include <cudaTypedefs.h>
 
 #include <type_traits>

@@ -25,10 +25,18 @@
 // dK (256 columns) and two buffers of S and dP (4 × 64) fill the 512 TMEM
 // columns at 128 dims.
 //
+// Measured (sustained; B200): 4 documents of 1025–4095 tokens, 12/3 heads of
+// 128, causal, bf16: dQ 165 µs, dK/dV 210–240 µs, rows 10 µs (three products
+// of the dQ kernel's seven-product share at 1,647 TFLOP/s: 98 µs, the other
+// four: 130); bound by the chain scores → P and dS → products of a buffer,
+// which one other buffer covers by half (tensor pipe 36–45%).  Issued by one
+// warp for both kinds of products the pair took 570 µs.
+//
 // P and dS are 16-bit operands.  f16 has few exponents, so there P carries
 // 2^15 and dS a power of two chosen for its row (key or query) such that the
 // largest possible |dS| stays below 2^15: |dO_i·V_j| ≤ ‖dO_i‖·‖V_j‖; the f32
-// sums are scaled back at the end.  bf16 needs neither.
+// sums are scaled back at the end.  bf16 needs neither.  Sequences and rows of
+// at most 128 keys keep P's and dS's remainders as second operands.
 //
 // Rows of other sequences in a tile are masked by selection, and the rows of
 // the summed operand past the sequence's end are zeroed (0 · NaN is NaN).

@@ -12,11 +12,13 @@
 // remainder in turns, position · inv_freq / 2π − nearest integer, is exact to
 // 10^-11 in f64 and goes on in f32 (sincospif).
 //
-// Bound: HBM, each element read and written once.  A block owns a few tokens:
-// it computes their rot/2 (cos, sin) pairs once into shared memory, and its
-// threads then walk (token, head) rows with 16-byte accesses, all q and k
-// heads of a token in the same block, so the sines cost 1/heads of a pair
-// each.  One launch serves q and k.
+// Bound: HBM, each element read and written once.  A block owns one or a few
+// tokens: it computes their rot/2 (cos, sin) pairs once into shared memory,
+// and a thread keeps those of its chunk in registers over the heads that it
+// turns with 16-byte accesses, all q and k heads of a token in the same block.
+// One launch serves q and k.  Measured (B200): 16384 tokens, 32 + 8 heads of
+// 128, 64 rotated, f16, 63.5 µs = 0.81 of the copy rate (two heads in flight a
+// thread instead of six: 85 µs; pairs read from shared memory for each head: 95).
 #include "va_common.cuh"
 
 namespace va {
