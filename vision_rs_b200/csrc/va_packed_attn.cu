@@ -29,7 +29,7 @@
 // floor 177): bound by issuing the MMAs and by the shared-memory reads of the
 // N = 64 score MMAs.  16 images of 257–1601 tokens, 6 heads of 64, 60 µs (floor
 // 21, the exponentials): bound by the softmax's latencies between them.  64
-// single tokens over 17–8192 keys, 32/8 heads of 128, 203 µs = 5.3 TB/s: HBM.
+// single tokens over 17–8192 keys, 32/8 heads of 128, 190 µs = 5.7 TB/s: HBM.
 // One 128-key buffer a tile instead of two of 64 keys: 339 against 264 µs for
 // the prompts; one issuing warp for both tiles: 410.
 //

@@ -25,12 +25,12 @@
 // dK (256 columns) and two buffers of S and dP (4 × 64) fill the 512 TMEM
 // columns at 128 dims.
 //
-// Measured (sustained; B200): 4 documents of 1025–4095 tokens, 12/3 heads of
-// 128, causal, bf16: dQ 165 µs, dK/dV 210–240 µs, rows 10 µs (three products
-// of the dQ kernel's seven-product share at 1,647 TFLOP/s: 98 µs, the other
-// four: 130); bound by the chain scores → P and dS → products of a buffer,
-// which one other buffer covers by half (tensor pipe 36–45%).  Issued by one
-// warp for both kinds of products the pair took 570 µs.
+// Measured (B200): 4 documents of 1025–4095 tokens, 12/3 heads of 128, causal,
+// bf16: dQ 169 µs, dK/dV 245 µs, row sums 15 µs (cold); the 3 and 4 products of
+// the first two take 59 and 78 µs at 1,647 TFLOP/s.  Bound by a buffer's chain
+// scores → P and dS → products, which the other buffer covers by half (tensor
+// pipe 36–45%), and in dK/dV by the shared-memory reads of its N = 64 score
+// MMAs.  One warp to issue both kinds of products: 349 and 220 µs.
 //
 // P and dS are 16-bit operands.  f16 has few exponents, so there P carries
 // 2^15 and dS a power of two chosen for its row (key or query) such that the
