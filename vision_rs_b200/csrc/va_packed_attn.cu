@@ -25,11 +25,12 @@
 // about as much error as that of the output.  Sums, maxima and O stay f32.
 //
 // Measured (sustained; B200): prompts of 2049 and 8191 tokens, 16/2 heads of
-// 128, causal, 297 µs = 0.98 PFLOP/s (254 µs before the power limit acts;
+// 128, causal, 300 µs = 0.97 PFLOP/s (254 µs before the power limit acts;
 // floor 177): bound by issuing the MMAs and by the shared-memory reads of the
-// N = 64 score MMAs.  16 images of 257–1601 tokens, 6 heads of 64, 60 µs (floor
+// N = 64 score MMAs.  16 images of 257–1601 tokens, 6 heads of 64, 65 µs (floor
 // 21, the exponentials): bound by the softmax's latencies between them.  64
-// single tokens over 17–8192 keys, 32/8 heads of 128, 190 µs = 5.7 TB/s: HBM.
+// single tokens over 17–8192 keys, 32/8 heads of 128, 210 µs = 5.1 TB/s (189
+// before the power limit acts): HBM.
 // One 128-key buffer a tile instead of two of 64 keys: 339 against 264 µs for
 // the prompts; one issuing warp for both tiles: 410.
 //
