@@ -116,6 +116,34 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   return s;
 }
 
+// The plan's arithmetic (host and device).  Sums over tiles are 64-bit: the dK/dV steps of one document of 2^20 tokens with
+// 32 query heads over one key head already add up to 2^31.
+#ifdef __CUDACC__
+#define VA_PACKED_FN __host__ __device__ __forceinline__
+#else
+#define VA_PACKED_FN inline
+#endif
+using PackedSum = long long;
+VA_PACKED_FN int pk_min(int a, int b) { return a < b ? a : b; }
+VA_PACKED_FN int pk_max(int a, int b) { return a > b ? a : b; }
+// Key blocks that the queries [i0, i0 + n) of a sequence see.
+VA_PACKED_FN int key_blocks(int lq, int lk, int i0, int n, int causal) {
+  const int end = causal ? pk_min(lk, pk_max(0, lk - (lq - i0 - n))) : lk;
+  return (end + kPackBlock - 1) / kPackBlock;
+}
+// Steps of 64 queries, over the heads of a group, that see any of the keys from j0 on.
+VA_PACKED_FN int query_steps(int lq, int lk, int j0, int causal, int group) {
+  const int first = causal ? pk_max(0, j0 - (lk - lq)) / 64 : 0;
+  return pk_max(0, (lq + 63) / 64 - first) * group;
+}
+// Largest part of a tile, for `blocks` blocks in all: Σ ceil(b / part) ≤ tiles + blocks / part ≤ tiles + budget.
+VA_PACKED_FN int part_blocks(PackedSum blocks, int budget, int smallest) {
+  if (!budget) return 1 << 30;
+  const PackedSum part = (blocks + budget - 1) / budget;
+  return part > (1 << 30) ? 1 << 30 : pk_max((int)part, smallest);
+}
+VA_PACKED_FN int part_count(int blocks, int part) { return pk_max(1, (int)(((PackedSum)blocks + part - 1) / part)); }
+
 int packed_status_read(int* out, cudaStream_t st);
 int packed_status_clear(cudaStream_t st);
 int packed_bwd_status_read(int* out, cudaStream_t st);
@@ -124,6 +152,6 @@ int packed_bwd_status_clear(cudaStream_t st);
 int packed_map(CUtensorMap* m, const void* base, bool bf16, int rows, int heads, int dim, long long row_stride,
                long long head_stride, int box_heads, int box_rows, const char* what);
 // Argument checks shared by the entry points (VA_OK or an error that is set).
-int packed_check(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim);
+int packed_check(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim, int training);
 
 }  // namespace va

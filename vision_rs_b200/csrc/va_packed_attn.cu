@@ -653,7 +653,7 @@ template <bool BF16>
 int packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides, int num_seqs,
                int total_q, int total_k, int heads, int kv_heads, int dim, int causal, int training, float scale,
                void* plan, size_t plan_bytes, cudaStream_t st) {
-  if (int rc = packed_check(num_seqs, total_q, total_k, heads, kv_heads, dim)) return rc;
+  if (int rc = packed_check(num_seqs, total_q, total_k, heads, kv_heads, dim, training)) return rc;
   VA_CHECK_ARG(scale > 0.0f && scale < INFINITY, "packed attention: the scale must be positive and finite");
   if (total_q == 0) return VA_OK;
   VA_CHECK_ARG(q && out && lse && strides && (total_k == 0 || (k && v)), "packed attention: null pointer");

@@ -429,8 +429,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if constexpr (!BF16) {  // |dS_ij| ≤ max_i ‖dO_i‖ · ‖V_j‖ + max_i |Δ_i|
       const float* norms = reinterpret_cast<const float*>(a.plan + ps.do_norm);
       float top_n = 0.0f, top_d = 0.0f;
-      for (int i = tid; i < nh * kHalf * ps.group; i += C::kSoft) {
-        const int gh = i / (nh * kHalf), q = hb0 * kHalf + i - gh * nh * kHalf;
+      const unsigned head_rows = nh * kHalf;  // head_rows · group < 2^32 (packed_check)
+      for (unsigned i = tid; i < head_rows * ps.group; i += C::kSoft) {
+        const int gh = i / head_rows, q = hb0 * kHalf + (int)(i - gh * head_rows);
         if (q >= it.lq) continue;
         const long long at = (long long)(kvh * ps.group + gh) * ps.total_q + it.q0 + q;
         top_n = fmaxf(top_n, norms[at]);
@@ -945,7 +946,7 @@ int packed_bwd(const void* d_out, const void* q, const void* k, const void* v, c
                void* dq, void* dk, void* dv, const int64_t* strides, int num_seqs, int total_q, int total_k, int heads,
                int kv_heads, int dim, int causal, int training, float scale, void* plan, size_t plan_bytes,
                cudaStream_t st) {
-  if (int rc = packed_check(num_seqs, total_q, total_k, heads, kv_heads, dim)) return rc;
+  if (int rc = packed_check(num_seqs, total_q, total_k, heads, kv_heads, dim, 1)) return rc;
   VA_CHECK_ARG(training, "packed attention backward: the plan must be built for training");
   VA_CHECK_ARG(scale > 0.0f && scale < INFINITY, "packed attention: the scale must be positive and finite");
   VA_CHECK_ARG(strides && (total_q == 0 || (d_out && q && out && lse && dq)) && (total_k == 0 || (k && v && dk && dv)),

@@ -14,6 +14,8 @@
 // Offsets that decrease or pass the packed tensors' ends are clamped (no
 // access leaves the tensors) and reported in the header.  5–6 µs, most of it
 // the launch and the dependent loads; the attention's launch overlaps its end.
+#include <limits.h>
+
 #include "va_common.cuh"
 #include "va_packed.h"
 
@@ -48,21 +50,21 @@ __device__ __forceinline__ Seq load_seq(const int* cu_q, const int* cu_k, const 
 }
 
 // Exclusive sum over the block's threads; *total: of all.
-__device__ int block_scan(int v, int* total) {
-  __shared__ int warp_sum[32];
+template <typename T> __device__ T block_scan(T v, T* total) {
+  __shared__ T warp_sum[32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int x = v;
+  T x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const T y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();  // the previous call's readers are done
   if (lane == 31) warp_sum[w] = x;
   __syncthreads();
-  int before = 0, all = 0;
+  T before = 0, all = 0;
   for (int i = 0; i < kPlanThreads / 32; ++i) {
-    const int t = warp_sum[i];
+    const T t = warp_sum[i];
     if (i < w) before += t;
     all += t;
   }
@@ -87,23 +89,9 @@ __device__ __forceinline__ int seq_of_tile(const int* first, int num_seqs, int t
   return lo;
 }
 
-struct Range {
-  int b0, b1;
-};
-// Key blocks that the queries [i0, i0 + n) of a sequence see.
-__device__ __forceinline__ Range key_blocks(const Seq& s, int i0, int n, int causal) {
-  const int end = causal ? min(s.lk, max(0, i0 + n + s.lk - s.lq)) : s.lk;
-  return {0, (end + kPackBlock - 1) / kPackBlock};
-}
-// Steps of 64 queries, over the heads of a group, that see any of the keys from j0 on.
-__device__ __forceinline__ Range query_steps(const Seq& s, int j0, int causal, int group) {
-  const int first = causal ? max(0, j0 - (s.lk - s.lq)) / 64 : 0;
-  return {0, max(0, (s.lq + 63) / 64 - first) * group};
-}
-
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
   __shared__ int hist[kClasses], cursor[kClasses];
-  __shared__ int bad, most, first_smem[kPlanSeqs + 1];
+  __shared__ int bad, full, most, first_smem[kPlanSeqs + 1];
   const PackedShape& s = a.s;
   let_next_start();
   wait_for_previous();
@@ -114,11 +102,11 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
                    ? first_smem
                    : reinterpret_cast<int*>(a.plan + s.scratch) + (size_t)list * (s.num_seqs + 1);
   const int tile = list == 0 ? s.q_tile : kPackBlock;
-  if (tid == 0) bad = 0, most = 0;
+  if (tid == 0) bad = 0, full = 0, most = 0;
   for (int c = tid; c < kClasses; c += kPlanThreads) hist[c] = 0;
   __syncthreads();
 
-  int tiles = 0;
+  PackedSum sum_tiles = 0;
   for (int b0 = 0; b0 < s.num_seqs; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int n = 0;
@@ -126,70 +114,70 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
       const Seq q = load_seq(a.cu_q, a.cu_k, a.used_k, s.num_seqs, b, s.total_q, s.total_k, &bad);
       n = ((list == 2 ? q.lk : q.lq) + tile - 1) / tile;
     }
-    int sum;
-    const int before = block_scan(n, &sum);
-    if (b < s.num_seqs) first[b] = tiles + before;
-    tiles += sum;
+    PackedSum sum;
+    const PackedSum before = block_scan<PackedSum>(n, &sum);
+    if (b < s.num_seqs) first[b] = (int)min(sum_tiles + before, (PackedSum)INT_MAX);
+    sum_tiles += sum;
   }
-  if (tid == 0) first[s.num_seqs] = tiles;
+  if (tid == 0) first[s.num_seqs] = (int)min(sum_tiles, (PackedSum)INT_MAX);
   __syncthreads();
   // offsets that run backwards could name more rows than there are: keep to the lists' room
   const int room = list == 0 ? s.max_tiles : list == 1 ? s.max_dq_items : s.max_dkv_tiles;
-  if (tiles > room) {
-    if (tid == 0) bad = 1;
-    tiles = room;
-  }
+  if (sum_tiles > room && tid == 0) bad = 1;
+  const int tiles = (int)min(sum_tiles, (PackedSum)room);
 
   Seq own_seq{};  // the thread's first tile, which every pass below asks for
-  int own_i0 = 0;
-  Range own_range{-1, 0};
-  auto tile_of = [&](int t, Seq* q, int* i0) -> Range {
-    if (t == tid && own_range.b0 >= 0) {
+  int own_i0 = 0, own_blocks = -1;
+  auto tile_of = [&](int t, Seq* q, int* i0) -> int {  // its key blocks or query steps
+    if (t == tid && own_blocks >= 0) {
       *q = own_seq, *i0 = own_i0;
-      return own_range;
+      return own_blocks;
     }
     const int b = seq_of_tile(first, s.num_seqs, t);
     *q = load_seq(a.cu_q, a.cu_k, a.used_k, s.num_seqs, b, s.total_q, s.total_k, &bad);
     *i0 = (t - first[b]) * tile;
-    const Range r =
-        list == 2 ? query_steps(*q, *i0, s.causal, s.group) : key_blocks(*q, *i0, min(tile, q->lq - *i0), s.causal);
-    if (t == tid) own_seq = *q, own_i0 = *i0, own_range = r;
-    return r;
+    const int n = list == 2 ? query_steps(q->lq, q->lk, *i0, s.causal, s.group)
+                            : key_blocks(q->lq, q->lk, *i0, min(tile, q->lq - *i0), s.causal);
+    if (t == tid) own_seq = *q, own_i0 = *i0, own_blocks = n;
+    return n;
   };
 
-  int mine = 0, mine_most = 0;
+  PackedSum mine = 0;
+  int mine_most = 0;
   for (int t = tid; t < tiles; t += kPlanThreads) {
     Seq q;
     int i0;
-    const Range r = tile_of(t, &q, &i0);
-    mine += r.b1 - r.b0;
-    mine_most = max(mine_most, r.b1 - r.b0);
+    const int n = tile_of(t, &q, &i0);
+    mine += n;
+    mine_most = max(mine_most, n);
   }
   atomicMax(&most, mine_most);
-  int blocks;
-  block_scan(mine, &blocks);
-  // parts of at most `chunk` blocks: Σ ceil(b / chunk) ≤ tiles + blocks / chunk ≤ tiles + budget
+  PackedSum blocks;
+  block_scan<PackedSum>(mine, &blocks);
   const int budget = list == 0 ? s.split_budget : list == 2 ? s.dkv_budget : 0;
-  const int chunk = budget ? max((blocks + budget - 1) / budget, list == 0 ? kMinKeyBlocks : kMinQuerySteps) : 1 << 30;
+  const int chunk = part_blocks(blocks, budget, list == 0 ? kMinKeyBlocks : kMinQuerySteps);
   const int top = max(1, min(most, chunk));
+  // the lists' room: part_blocks keeps to it, and what would pass it all the same (offsets that change meanwhile) is left out
+  const int room_items = list == 0 ? s.max_items : list == 1 ? s.max_dq_items : s.max_dkv_items;
+  const int room_slots = list == 0 ? s.max_slots : list == 2 ? 2 * s.dkv_budget : 0;
 
-  auto parts_of = [&](const Range& r) { return max(1, (r.b1 - r.b0 + chunk - 1) / chunk); };
-  auto size_class = [&](int n, int parts) { return kClasses - 1 - (int)((long long)(n / parts) * (kClasses - 1) / top); };
+  auto size_class = [&](int n, int parts) {
+    return max(0, kClasses - 1 - (int)((long long)(n / parts) * (kClasses - 1) / top));
+  };
   int slots = 0, items = 0;
   for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
     const int t = t0 + tid;
     if (t < tiles) {
       Seq q;
       int i0;
-      const Range r = tile_of(t, &q, &i0);
-      const int p = parts_of(r);
-      atomicAdd(&hist[size_class(r.b1 - r.b0, p)], p);
+      const int n = tile_of(t, &q, &i0), p = part_count(n, chunk);
+      atomicAdd(&hist[size_class(n, p)], p);
     }
   }
   __syncthreads();
   {
     int sum;
-    const int n = tid < kClasses ? hist[tid] : 0, before = block_scan(n, &sum);
+    const int n = tid < kClasses ? hist[tid] : 0, before = block_scan<int>(n, &sum);
     if (tid < kClasses) cursor[tid] = before;
     items = sum;
   }
@@ -197,18 +185,20 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
   for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
     const int t = t0 + tid;
     Seq q{};
-    int i0 = 0, p = 0;
-    Range r{0, 0};
+    int i0 = 0, n = 0, p = 0;
     if (t < tiles) {
-      r = tile_of(t, &q, &i0);
-      p = parts_of(r);
+      n = tile_of(t, &q, &i0);
+      p = part_count(n, chunk);
     }
     int sum;
-    const int slot0 = slots + block_scan(p > 1 ? p : 0, &sum);
+    const int slot0 = slots + block_scan<int>(p > 1 ? p : 0, &sum);
     slots += sum;
     if (t >= tiles) continue;
-    const int n = r.b1 - r.b0;
     int at = atomicAdd(&cursor[size_class(n, p)], p);
+    if (at < 0 || at > room_items - p || (p > 1 && (slot0 < 0 || slot0 > room_slots - p))) {
+      full = 1;
+      continue;
+    }
     if (list == 2) {
       KItem* out = reinterpret_cast<KItem*>(a.plan + s.dkv_items);
       for (int k = 0; k < p; ++k, ++at)
@@ -220,29 +210,33 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
     QItem* out = reinterpret_cast<QItem*>(a.plan + (list == 0 ? s.items : s.dq_items));
     for (int k = 0; k < p; ++k, ++at)
       out[at] = QItem{q.q0 + i0, min(tile, q.lq - i0), q.k0, q.lk, i0 + q.lk - q.lq,
-                      r.b0 + (int)((long long)n * k / p), r.b0 + (int)((long long)n * (k + 1) / p),
+                      (int)((long long)n * k / p), (int)((long long)n * (k + 1) / p),
                       p > 1 ? slot0 + k : -1, slot0, p, t, 0};
   }
   if (budget) {  // arrival counters of the split tiles
     int* cnt = reinterpret_cast<int*>(a.plan + (list == 0 ? s.counters : s.dkv_counters));
-    for (int i = tid; i < tiles * (list == 0 ? s.units : s.kv_heads); i += kPlanThreads) cnt[i] = 0;
+    const long long cells = (long long)tiles * (list == 0 ? s.units : s.kv_heads);
+    for (long long i = tid; i < cells; i += kPlanThreads) cnt[i] = 0;
   }
   __syncthreads();
   if (tid == 0) {
-    hdr[list] = items;
-    hdr[kHdrBad + list] = bad;
+    hdr[list] = full ? 0 : items;  // a list with holes is not walked
+    hdr[kHdrBad + list] = bad | full;
   }
 }
 
 
 }  // namespace
 
-int packed_check(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim) {
+int packed_check(int num_seqs, int total_q, int total_k, int heads, int kv_heads, int dim, int training) {
   VA_CHECK_ARG(num_seqs > 0 && num_seqs <= kMaxSeqs && total_q >= 0 && total_k >= 0,
                "packed attention: %d sequences, %d queries, %d keys", num_seqs, total_q, total_k);
   VA_CHECK_ARG(total_q <= (1 << 30) && total_k <= (1 << 30), "packed attention: more than 2^30 tokens");
   VA_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= kPackBlock && heads <= 4096,
                "packed attention: %d query heads over %d key heads", heads, kv_heads);
+  // the backward counts a key head's (query, head) rows in 32 bits
+  VA_CHECK_ARG(!training || (long long)total_q * (heads / kv_heads) < (1LL << 32) - (1 << 16),
+               "packed attention: training with %d queries of %d heads a key head", total_q, heads / kv_heads);
   VA_CHECK_ARG(dim >= 8 && dim <= 128 && dim % 8 == 0, "packed attention: head size %d (a multiple of 8 up to 128)",
                dim);
   return VA_OK;
@@ -256,14 +250,14 @@ extern "C" {
 
 size_t va_packed_plan_bytes(int num_seqs, int total_q, int total_k, int num_heads, int num_kv_heads, int head_dim,
                             int causal, int training) {
-  if (packed_check(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim)) return 0;
+  if (packed_check(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim, training)) return 0;
   return packed_shape(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim, causal != 0, training != 0).total;
 }
 
 int va_packed_plan_build(const int32_t* cu_q, const int32_t* cu_k, const int32_t* used_k, int num_seqs, int total_q, int total_k,
                          int num_heads, int num_kv_heads, int head_dim, int causal, int training, void* plan,
                          size_t plan_bytes, va_stream_t stream) {
-  if (int rc = packed_check(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim)) return rc;
+  if (int rc = packed_check(num_seqs, total_q, total_k, num_heads, num_kv_heads, head_dim, training)) return rc;
   VA_CHECK_ARG(cu_q && cu_k, "packed plan: null offsets");
   VA_CHECK_ARG(!(used_k && training), "packed plan: reserved rows have no gradient, train without used_k");
   PlanArgs a{cu_q, cu_k, used_k, static_cast<uint8_t*>(plan),
