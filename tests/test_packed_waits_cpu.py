@@ -1,0 +1,38 @@
+"""The ways out of the packed-attention kernels after a bounded wait gave up,
+read from their source: no GPU is made to hang for it.
+
+A thread that leaves a loop by itself leaves its peers at an aligned barrier, a
+vote or a warp-wide TMEM instruction that waits for it without a limit.  So the
+warps that run the softmax or the scores go through their loops to the end, and
+vote once before they store."""
+import os
+import re
+
+import pytest
+
+from conftest import ROOT
+
+
+def _source(name):
+    text = open(os.path.join(ROOT, "vision_rs_b200", "csrc", name)).read()
+    return re.sub(r"//[^\n]*", "", text)  # without comments
+
+
+def _roles(name):
+    """Bodies of the warps that come last in each kernel's chain of roles: softmax (forward) or scores (backward)."""
+    text = _source(name)
+    starts = {"va_packed_attn.cu": [r"const int m = TILES == 2 \? warp >> 2 : 0, row"],
+              "va_packed_attn_bwd.cu": [r"const int g = warp >> 2, key = ", r"const int g = warp >> 2, row = "]}[name]
+    for start in starts:
+        at = re.search(start, text).start()
+        yield text[at:text.index("__syncthreads();", at)]
+
+
+@pytest.mark.parametrize("name", ["va_packed_attn.cu", "va_packed_attn_bwd.cu"])
+def test_no_thread_leaves_alone(name):
+    assert "bar.arrive" not in _source(name)
+    for body in _roles(name):
+        assert "break;" not in body and "_leave" not in body
+        assert not re.search(r"for \([^;]*;[^;]*\bok\b", body)  # no loop ends on one thread's wait
+        assert not re.search(r"if \([^)]*\bok = ", body)        # nor is a step left out for it
+        assert "__all_sync(0xffffffffu, ok" in body              # the warp agrees before it stores

@@ -390,13 +390,17 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     // warps without a row of the unit only keep the barriers going
     const bool idle = (m * kPackBlock + (warp & 3) * 32) >= rows;
     const int n = steps[m];
+    // A wait that gives up is passed over, as are the thread's later ones: the loop goes on to its end, so the lanes of a
+    // warp never part at its votes and TMEM instructions; nothing is written then.
+    auto wait = [&](uint64_t* bar, int parity, int where) {
+      ok = ok && mbar_wait(bar, parity, &sm.abort, &g_packed_status, where);
+    };
     // Parts of a step's work on its 64 scores u:
-    auto fetch = [&](int h, uint32_t (&u)[2][32]) -> bool {  // starts reading them
-      if (!mbar_wait(&sm.s_full[m][h & 1], (h >> 1) & 1, &sm.abort, &g_packed_status, 8)) return false;
+    auto fetch = [&](int h, uint32_t (&u)[2][32]) {  // starts reading them
+      wait(&sm.s_full[m][h & 1], (h >> 1) & 1, 8);
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld32(ts + (h & 1) * kHalf + c * 32, u[c]);
-      return true;
     };
     auto top_of = [&](int h, uint32_t (&u)[2][32]) -> float {  // has them, hides keys, largest in log2 units
       tmem_ld_wait();
@@ -420,13 +424,13 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
       return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
     };
-    auto follow = [&](int h, float top) -> bool {  // the reference follows, O is rescaled
+    auto follow = [&](int h, float top) {  // the reference follows, O is rescaled
       const bool grow = mine && (top > ref + kRescaleAt || ref == -INFINITY);
-      if (!__any_sync(0xffffffffu, grow)) return true;
+      if (!__any_sync(0xffffffffu, grow)) return;
       const float next = grow ? fmaxf(ref, top) : ref;  // a row's result does not depend on its warp's other rows
       if (h > 0) {
         const float f = next == -INFINITY ? 1.0f : ex2(ref - next);
-        if (!mbar_wait(&sm.o_done[m][(h & 1) ^ 1], ((h - 1) >> 1) & 1, &sm.abort, &g_packed_status, 9)) return false;
+        wait(&sm.o_done[m][(h & 1) ^ 1], ((h - 1) >> 1) & 1, 9);
         tc_fence_after();
         for (int c = 0; c < dim16; c += 16) {
           uint32_t o[16];
@@ -440,7 +444,6 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         sum *= f;
       }
       ref = next;
-      return true;
     };
     float part[4];
     auto exps = [&](int h, const uint32_t (&u)[32], int c, auto fine) {  // P of 32 keys
@@ -466,16 +469,16 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       mbar_arrive(&sm.p_full[m][h & 1]);
     };
     if (idle) {
-      for (int h = 0; ok && h < n; ++h)
-        if ((ok = mbar_wait(&sm.s_full[m][h & 1], (h >> 1) & 1, &sm.abort, &g_packed_status, 8)))
-          mbar_arrive(&sm.p_full[m][h & 1]);
+      for (int h = 0; h < n; ++h) {
+        wait(&sm.s_full[m][h & 1], (h >> 1) & 1, 8);
+        mbar_arrive(&sm.p_full[m][h & 1]);
+      }
     } else {
       auto steps_of = [&](auto fine) {
         for (int h = 0; h < n; ++h) {
           uint32_t u[2][32];
-          if (!(ok = fetch(h, u))) break;
-          const float top = top_of(h, u);
-          if (!(ok = follow(h, top))) break;
+          fetch(h, u);
+          follow(h, top_of(h, u));
           part[0] = part[1] = part[2] = part[3] = 0.0f;
           exps(h, u[0], 0, fine);
           exps(h, u[1], 1, fine);
@@ -486,8 +489,8 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       else steps_of(std::false_type{});
     }
     // ── output ──
-    if (ok && n > 0) ok = mbar_wait(&sm.o_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, &sm.abort, &g_packed_status, 10);
-    if (ok && !idle) {
+    if (n > 0) wait(&sm.o_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, 10);
+    if (__all_sync(0xffffffffu, ok) && !idle) {
       tc_fence_after();
       // a row without a key; one of NaN scores has no maximum either, but its sum is NaN
       const bool none = n <= 0 || (ref == -INFINITY && sum == sum);

@@ -98,11 +98,12 @@ struct BwdArgs {
   float scale;
 };
 
-// The four warps of a score group meet; one that gives up arrives without waiting.
-__device__ __forceinline__ void group_leave(int g) { asm volatile("bar.arrive %0, 128;" ::"r"(g + 1) : "memory"); }
-// All score groups.
+// The score warps never leave a loop early: a wait that gives up is passed over, as are the thread's later ones, so that
+// every thread meets every one of these barriers and the lanes of a warp stay together at its TMEM instructions.  The
+// result is not written then.
+// All score groups meet.
 template <int N> __device__ __forceinline__ void scores_sync() { asm volatile("bar.sync 4, %0;" ::"n"(N) : "memory"); }
-template <int N> __device__ __forceinline__ void scores_leave() { asm volatile("bar.arrive 4, %0;" ::"n"(N) : "memory"); }
+// The four warps of one meet.
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(g + 1) : "memory"); }
 
 // Largest power of two p with bound·p < 2^15 (1 for a bound of zero; the exponent is kept within ±60).
@@ -476,10 +477,6 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         reinterpret_cast<float*>(sm.stats[g][k & 1][1])[key] = -ahead.y;
       }
       group_sync(g);
-      if (*(volatile int*)&sm.abort) {
-        ok = false;
-        break;
-      }
       const int i0 = (hb0 + block) * kHalf;
       advance(C::kGroups);
       ahead = fetch(h + C::kGroups);
@@ -487,10 +484,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // queries [lo, hi) of the step see this key
       const int lo = ps.causal ? j - off - i0 : 0, hi = it.lq - i0;
       const bool whole = hi >= kHalf && (!ps.causal || it.j0 + it.keys - 1 - off <= i0);
-      if (!(ok = mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 8))) {
-        group_leave(g);
-        break;
-      }
+      ok = ok && mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 8);
       tc_fence_after();
       const float4 *nl = sm.stats[g][k & 1][0], *nd = sm.stats[g][k & 1][1];
       // 16 queries at a time: their statistics are read while the scores come
@@ -583,8 +577,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       tc_fence_before();
       mbar_arrive(&sm.p_full[g]);
     }
-    if (n > 0) ok = mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 9) && ok;
-    if (ok && !sm.abort && g < 2) {  // group 0 stores dV, group 1 dK
+    if (n > 0) ok = ok && mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 9);
+    if (__all_sync(0xffffffffu, ok && !*(volatile int*)&sm.abort) && g < 2) {  // group 0 stores dV, group 1 dK
       tc_fence_after();
       const uint32_t acc = tmem + lanes + kColAcc + g * DP;
       const float f = g == 0 ? (BF16 ? 1.0f : 3.0517578125e-05f) : 1.0f / mult;
@@ -808,28 +802,27 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (n > 0 && g < 2) {
       // group 0 moves Q, group 1 dO from shared memory to TMEM: a thread its row
       ok = mbar_wait(&sm.a_full, 0, &sm.abort, &g_packed_bwd_status, 17);
-      if (ok) {
 #pragma unroll
-        for (int b = 0; b < DP / 64; ++b) {
-          uint32_t u[32];
+      for (int b = 0; b < DP / 64; ++b) {
+        uint32_t u[32];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(sm.a[g] + b * kPackBlock * 128 + sw128_off(row, c));
-            u[4 * c] = w.x, u[4 * c + 1] = w.y, u[4 * c + 2] = w.z, u[4 * c + 3] = w.w;
-          }
-          tmem_st32(tmem + lanes + (g == 0 ? kColQ : kColDO) + b * 32, u);
+        for (int c = 0; c < 8; ++c) {
+          const uint4 w = *reinterpret_cast<const uint4*>(sm.a[g] + b * kPackBlock * 128 + sw128_off(row, c));
+          u[4 * c] = w.x, u[4 * c + 1] = w.y, u[4 * c + 2] = w.z, u[4 * c + 3] = w.w;
         }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&sm.a_ready);
+        tmem_st32(tmem + lanes + (g == 0 ? kColQ : kColDO) + b * 32, u);
       }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.a_ready);
     }
     if (n > 0 && n <= kFineSteps) {
       // Rows that see at most 128 keys: all their scores are in the two buffers, so Δ_i = Σ_j P_ij dP_ij is summed from
       // them.  dO·O carries the rounding of the stored O, which matters here (O is an average of few values): it
       // would add as much error to dQ and dK as the rounding of dS.  The dK/dV kernel reads the better Δ too.
       float t = 0.0f;
-      if (ok && g < n && (ok = mbar_wait(&sm.s_full[g], 0, &sm.abort, &g_packed_bwd_status, 20))) {
+      if (g < n) {
+        ok = ok && mbar_wait(&sm.s_full[g], 0, &sm.abort, &g_packed_bwd_status, 20);
         tc_fence_after();
         const int limit = see - g * kHalf;
 #pragma unroll
@@ -848,17 +841,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
       }
       if (g < 2) sm.row_part[g][row] = t;
-      if (ok) {
-        scores_sync<C::kSoft>();
-        ok = !*(volatile int*)&sm.abort;
-      } else {
-        scores_leave<C::kSoft>();
-      }
+      scores_sync<C::kSoft>();
+      ok = ok && !*(volatile int*)&sm.abort;
       stat.y = sm.row_part[0][row] + sm.row_part[1][row];
       if (mine && ok && g == 0) reinterpret_cast<float2*>(a.plan + ps.rows)[at].y = stat.y;
     }
-    for (int h = g, k = 0; ok && h < n; h += C::kGroups, ++k) {
-      if (!(ok = mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 18))) break;
+    for (int h = g, k = 0; h < n; h += C::kGroups, ++k) {
+      ok = ok && mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 18);
       tc_fence_after();
       const int limit = see - h * kHalf;
       auto scores = [&](auto masked, auto fine) {
@@ -896,8 +885,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc_fence_before();
       mbar_arrive(&sm.p_full[g]);
     }
-    if (n > 0) ok = mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 19) && ok;
-    if (ok && !sm.abort) {  // each group stores half of the 16-column chunks
+    if (n > 0) ok = ok && mbar_wait(&sm.fin, 0, &sm.abort, &g_packed_bwd_status, 19);
+    if (__all_sync(0xffffffffu, ok && !*(volatile int*)&sm.abort)) {  // each group stores half of the 16-column chunks
       tc_fence_after();
       uint16_t* out = static_cast<uint16_t*>(a.dq) + (it.q0 + row) * a.dq_row + head * a.dq_head;
       for (int c = g * 16; c < dim16; c += C::kGroups * 16)
