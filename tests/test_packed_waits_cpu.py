@@ -36,3 +36,15 @@ def test_no_thread_leaves_alone(name):
         assert not re.search(r"for \([^;]*;[^;]*\bok\b", body)  # no loop ends on one thread's wait
         assert not re.search(r"if \([^)]*\bok = ", body)        # nor is a step left out for it
         assert "__all_sync(0xffffffffu, ok" in body              # the warp agrees before it stores
+
+
+@pytest.mark.parametrize("name,first", [("va_packed_attn.cu", "q_full"), ("va_packed_attn_bwd.cu", "a_full")])
+def test_loads_in_flight_are_waited_for(name, first):
+    """The producer waits (with a limit) for its last loads on every way out: a CTA that ends before they land lets them
+    write into its successor's shared memory."""
+    text = _source(name)
+    issue = text.index("++issued;")
+    drain = re.search(r"max\(0, issued - (C::kSlots|kStages)\)", text).start()
+    between = text[issue:drain]
+    assert issue < drain and not re.search(r"if \(!?ok\)", between)
+    assert re.search(r"mbar_try_wait\(&sm\.%s, 0\) && clock64\(\)" % first, text[drain:drain + 600])

@@ -227,13 +227,11 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             tma_load_3d(sm.q[m] + b * ROWS * 128, &map_q, &sm.q_full, b * 64, ps.few ? head * group : head,
                         it.q0 + m * kPackBlock);
       }
-      bool ok = true;
       int issued = 0;
       for (int g = 0; g < 2 * nkb; ++g) {
         const int st = g % C::kSlots, kb = it.kb0 + (g >> 1);
         if (g >= C::kSlots &&
-            !(ok = __all_sync(0xffffffffu, mbar_wait(&sm.kv_empty[st], (g / C::kSlots - 1) & 1, &sm.abort,
-                                                     &g_packed_status, 1))))
+            !__all_sync(0xffffffffu, mbar_wait(&sm.kv_empty[st], (g / C::kSlots - 1) & 1, &sm.abort, &g_packed_status, 1)))
           break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&sm.kv_full[st], C::kSlotBytes);
@@ -244,21 +242,20 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ++issued;
         if ((g & 1) && kb >= checked) {
           if constexpr (TILES == 1) {
-            if (!(ok = check_v(kb))) break;
+            if (!check_v(kb)) break;
           } else if (lane == 0) {
             mbar_arrive(&sm.v_sent[kb - checked]);
           }
         }
       }
-      if (!ok) {  // loads issued here land (bounded) before the CTA can exit
-        for (int g = max(0, issued - C::kSlots); g < issued; ++g) {
-          const long long c0 = clock64();
-          while (!mbar_try_wait(&sm.kv_full[g % C::kSlots], (g / C::kSlots) & 1) && clock64() - c0 < kSpinCycles) {
-          }
-        }
+      // loads issued here land (bounded) before the CTA can exit, also when it was another role that gave up
+      for (int g = max(0, issued - C::kSlots); g < issued; ++g) {
         const long long c0 = clock64();
-        while (!mbar_try_wait(&sm.q_full, 0) && clock64() - c0 < kSpinCycles) {
+        while (!mbar_try_wait(&sm.kv_full[g % C::kSlots], (g / C::kSlots) & 1) && clock64() - c0 < kSpinCycles) {
         }
+      }
+      const long long c0 = clock64();
+      while (!mbar_try_wait(&sm.q_full, 0) && clock64() - c0 < kSpinCycles) {
       }
     }
     __syncwarp();

@@ -174,12 +174,10 @@ __device__ __forceinline__ void store16(uint32_t taddr, bool zero, float f, bool
 template <int DP, typename At>
 __device__ __forceinline__ void produce(BwdSmem<DP>& sm, const CUtensorMap* m0, const CUtensorMap* m1, int n, At at) {
   constexpr int NB = DP / 64, kStages = BwdCfg<DP>::kStages;
-  bool ok = true;
   int issued = 0;
   for (int h = 0; h < n; ++h) {
     const int st = h % kStages;
-    if (h >= kStages && !(ok = mbar_wait(&sm.empty[st], (h / kStages - 1) & 1, &sm.abort, &g_packed_bwd_status, 1)))
-      break;
+    if (h >= kStages && !mbar_wait(&sm.empty[st], (h / kStages - 1) & 1, &sm.abort, &g_packed_bwd_status, 1)) break;
     int head, row;
     at(h, &head, &row);
     mbar_arrive_expect_tx(&sm.full[st], 2 * BwdSmem<DP>::kStep);
@@ -189,15 +187,14 @@ __device__ __forceinline__ void produce(BwdSmem<DP>& sm, const CUtensorMap* m0, 
     }
     ++issued;
   }
-  if (!ok) {  // loads issued here land (bounded) before the CTA can exit
-    for (int h = max(0, issued - kStages); h < issued; ++h) {
-      const long long c0 = clock64();
-      while (!mbar_try_wait(&sm.full[h % kStages], (h / kStages) & 1) && clock64() - c0 < kSpinCycles) {
-      }
-    }
+  // loads issued here land (bounded) before the CTA can exit, also when it was another role that gave up
+  for (int h = max(0, issued - kStages); h < issued; ++h) {
     const long long c0 = clock64();
-    while (!mbar_try_wait(&sm.a_full, 0) && clock64() - c0 < kSpinCycles) {
+    while (!mbar_try_wait(&sm.full[h % kStages], (h / kStages) & 1) && clock64() - c0 < kSpinCycles) {
     }
+  }
+  const long long c0 = clock64();
+  while (!mbar_try_wait(&sm.a_full, 0) && clock64() - c0 < kSpinCycles) {
   }
 }
 
