@@ -15,3 +15,25 @@ def test_plan_of_one_long_document(cuda, n, heads):
     plan.check()
     units = plan.buf[:12].view(torch.int32).tolist()
     assert n // 128 <= units[2] <= n // 128 + 148 and units[1] == n // 128
+
+
+def test_a_unit_of_more_than_a_second(cuda):
+    """256 queries a head over 200 million keys: each unit works for longer than a wait's limit (2·10^9 cycles), with a
+    last V block that is checked.  Keys of zeros: every weight is 1/n.  One value in 256 is one and the others zero: their
+    sum stays below 2^20, where the product's f32 sums (which drop what lies 2^-25 below the running sum) are exact."""
+    import math
+    from vision_rs_b200 import packed
+    n, H, D = 200_000_005, 76, 8
+    q = torch.randn(256, H, D, device=cuda).bfloat16()
+    k, v = (torch.zeros(n, 1, D, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    v[::256] = 1
+    plan = packed.PackedPlan(packed.cu_seqlens([256]), packed.cu_seqlens([n]), 256, n, H, 1, D)
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    o, lse = packed.packed_attention_forward(q, k, v, plan)
+    b.record()
+    b.synchronize()
+    assert a.elapsed_time(b) > 1100.0  # or this test shows nothing
+    # the weights' sum: steps of 64 stay exact in 32 bits, the last keys are rounded to 16 in 2·10^8
+    mean = (n + 255) // 256 / n
+    assert ((o.double() - mean).abs() <= 2.0 ** -8 * mean).all() and ((lse - math.log(n)).abs() <= 1e-6 * math.log(n)).all()

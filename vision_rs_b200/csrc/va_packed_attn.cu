@@ -85,6 +85,7 @@ template <int DP, int TILES, int ROWS> struct FwdSmem {
   uint64_t s_full[TILES][2], p_full[TILES][2], o_done[TILES][2], v_sent[kMaxChecked], v_ready[kMaxChecked], fin;
   uint32_t tmem_base;
   int abort;
+  int sent;  // blocks that the producer has sent
   int last;
   int loose;  // a checked V block held something that is not finite
 };
@@ -156,6 +157,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     sm.loose = 0;
     mbar_init(&sm.fin, TILES);
     sm.abort = 0;
+    sm.sent = 0;
     fence_mbar_init();
   }
   if (warp == TILES * 4) {
@@ -247,6 +249,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             mbar_arrive(&sm.v_sent[kb - checked]);
           }
         }
+        if (TILES == 2 && lane == 0) *(volatile int*)&sm.sent = issued;
       }
       // loads issued here land (bounded) before the CTA can exit, also when it was another role that gave up
       for (int g = max(0, issued - C::kSlots); g < issued; ++g) {
@@ -260,9 +263,11 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
     __syncwarp();
   } else if (TILES == 2 && warp == TILES * 5 + 1) {
-    // (the slot's barrier is in the phase of a block's load only once the load is sent)
+    // (the slot's barrier is in the phase of a block's load only once the load is sent, which may be as far ahead as the
+    // unit is long)
     for (int kb = checked; kb < it.kb0 + nkb; ++kb)
-      if (!__all_sync(0xffffffffu, mbar_wait(&sm.v_sent[kb - checked], 0, &sm.abort, &g_packed_status, 12)) ||
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait_behind(&sm.v_sent[kb - checked], 0, &sm.abort, &sm.sent, &g_packed_status, 12)) ||
           !check_v(kb))
         break;
     __syncwarp();

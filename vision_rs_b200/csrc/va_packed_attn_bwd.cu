@@ -88,7 +88,9 @@ template <int DP> struct BwdSmem {
   uint64_t s_full[C::kGroups], p_full[C::kGroups], g_done[C::kGroups], fin;
   uint32_t tmem_base;
   int abort, last;
+  int scanned;  // f16: how far the score warps are with the norms that bound dS, before their first step
 };
+constexpr unsigned kScanChunk = 4096;  // turns of that loop between two updates of `scanned`
 
 struct BwdArgs {
   uint8_t* plan;
@@ -138,6 +140,7 @@ template <int DP> __device__ __forceinline__ uint32_t bwd_setup(BwdSmem<DP>& sm,
     }
     mbar_init(&sm.fin, 2);
     sm.abort = 0;
+    sm.scanned = 0;
     fence_mbar_init();
   }
   if (warp == BwdCfg<DP>::kWarps) {
@@ -177,7 +180,8 @@ __device__ __forceinline__ void produce(BwdSmem<DP>& sm, const CUtensorMap* m0, 
   int issued = 0;
   for (int h = 0; h < n; ++h) {
     const int st = h % kStages;
-    if (h >= kStages && !mbar_wait(&sm.empty[st], (h / kStages - 1) & 1, &sm.abort, &g_packed_bwd_status, 1)) break;
+    if (h >= kStages && !mbar_wait_behind(&sm.empty[st], (h / kStages - 1) & 1, &sm.abort, &sm.scanned, &g_packed_bwd_status, 1))
+      break;
     int head, row;
     at(h, &head, &row);
     mbar_arrive_expect_tx(&sm.full[st], 2 * BwdSmem<DP>::kStep);
@@ -203,6 +207,10 @@ __device__ __forceinline__ void produce(BwdSmem<DP>& sm, const CUtensorMap* m0, 
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_status, where));
+}
+// For what comes after the score warps' scan of the norms.
+template <typename Smem> __device__ __forceinline__ bool wait_scores(Smem& sm, uint64_t* bar, uint32_t parity, int where) {
+  return __all_sync(0xffffffffu, mbar_wait_behind(bar, parity, &sm.abort, &sm.scanned, &g_packed_bwd_status, where));
 }
 template <typename Smem> __device__ __forceinline__ void issue_end(Smem& sm, uint32_t lead) {
   mma_commit_p(&sm.fin, lead);  // every MMA issued here completes before the CTA tears down
@@ -348,7 +356,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             __syncwarp();
           }
         }
-        if (h >= C::kGroups && !(ok = wait_all(&sm.g_done[buf], par ^ 1, &sm.abort, 6))) break;
+        if (h >= C::kGroups && !(ok = wait_scores(sm, &sm.g_done[buf], par ^ 1, 6))) break;
         tc_fence_after();
         const uint64_t bq = dq0 + (uint64_t)(st * 2 * kTileStep), bo = bq + kTileStep;
         const uint32_t ts = tm + buf * 128;
@@ -389,7 +397,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const int st = h % kStages;
         int ks = kHalf / 16;
         if (++b == blocks) b = 0, ks = min(ks, (tail + 15) >> 4);
-        if (!(ok = wait_all(&sm.p_full[buf], par, &sm.abort, 4))) break;
+        if (!(ok = wait_scores(sm, &sm.p_full[buf], par, 4))) break;
         tc_fence_after();
         const uint64_t gq = dq0 + (uint64_t)(st * 2 * kTileStep), go = gq + kTileStep;
         const uint32_t tp = tm + buf * 128;
@@ -428,12 +436,17 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const float* norms = reinterpret_cast<const float*>(a.plan + ps.do_norm);
       float top_n = 0.0f, top_d = 0.0f;
       const unsigned head_rows = nh * kHalf;  // head_rows · group < 2^32 (packed_check)
-      for (unsigned i = tid; i < head_rows * ps.group; i += C::kSoft) {
-        const int gh = i / head_rows, q = hb0 * kHalf + (int)(i - gh * head_rows);
-        if (q >= it.lq) continue;
-        const long long at = (long long)(kvh * ps.group + gh) * ps.total_q + it.q0 + q;
-        top_n = fmaxf(top_n, norms[at]);
-        top_d = fmaxf(top_d, fabsf(pairs[at].y));
+      const long long all = (long long)head_rows * ps.group;
+      for (long long i0 = 0; i0 < all; i0 += C::kSoft * kScanChunk) {
+        const unsigned end = (unsigned)min(all, i0 + C::kSoft * kScanChunk);
+        for (unsigned i = (unsigned)i0 + tid; i < end; i += C::kSoft) {
+          const int gh = i / head_rows, q = hb0 * kHalf + (int)(i - gh * head_rows);
+          if (q >= it.lq) continue;
+          const long long at = (long long)(kvh * ps.group + gh) * ps.total_q + it.q0 + q;
+          top_n = fmaxf(top_n, norms[at]);
+          top_d = fmaxf(top_d, fabsf(pairs[at].y));
+        }
+        if (tid == 0) *(volatile int*)&sm.scanned = (int)(i0 / (C::kSoft * kScanChunk)) + 1;
       }
       for (int o = 16; o; o >>= 1) {
         top_n = fmaxf(top_n, __shfl_xor_sync(0xffffffffu, top_n, o));
@@ -706,7 +719,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       auto next_buffer = [&] {
         if (++buf == C::kGroups) buf = 0, par ^= 1;
       };
-      bool ok = wait_all(&sm.a_ready, 0, &sm.abort, 12);
+      bool ok = wait_scores(sm, &sm.a_ready, 0, 12);
       for (int h = 0; ok && h < steps; ++h) {
         const int st = h % kStages;
         if (!(ok = wait_all(&sm.full[st], (h / kStages) & 1, &sm.abort, 13))) break;
@@ -715,7 +728,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (h >= C::kGroups && !(ok = wait_all(&sm.g_done[buf], par ^ 1, &sm.abort, 16))) break;
+        if (h >= C::kGroups && !(ok = wait_scores(sm, &sm.g_done[buf], par ^ 1, 16))) break;
         tc_fence_after();
         const uint64_t bk = dk0 + (uint64_t)(st * 2 * kTileStep), bv = bk + kTileStep;
         const uint32_t ts = tm + buf * 128;
@@ -752,7 +765,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       bool ok = true;
       for (int h = 0; h < steps; ++h) {
         const int st = h % kStages, ks = h == steps - 1 ? (tail + 15) >> 4 : kHalf / 16;
-        if (!(ok = wait_all(&sm.p_full[buf], par, &sm.abort, 14))) break;
+        if (!(ok = wait_scores(sm, &sm.p_full[buf], par, 14))) break;
         tc_fence_after();
         const uint64_t gk = dk0 + (uint64_t)(st * 2 * kTileStep);
         auto one = [&](int s) {
@@ -787,7 +800,11 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if constexpr (!BF16) {  // |dS_ij| ≤ ‖dO_i‖ · max_j ‖V_j‖ + |Δ_i|
       const float* vn = reinterpret_cast<const float*>(a.plan + ps.v_norm) + (long long)kvh * ps.total_k + it.k0;
       float top = 0.0f;
-      for (int i = tid; i < see_end; i += C::kSoft) top = fmaxf(top, vn[i]);
+      for (int i0 = 0; i0 < see_end; i0 += C::kSoft * kScanChunk) {
+        const int end = min(see_end, i0 + (int)(C::kSoft * kScanChunk));
+        for (int i = i0 + tid; i < end; i += C::kSoft) top = fmaxf(top, vn[i]);
+        if (tid == 0) *(volatile int*)&sm.scanned = i0 / (int)(C::kSoft * kScanChunk) + 1;
+      }
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (lane == 0) sm.red[warp] = top;
       scores_sync<C::kSoft>();

@@ -64,6 +64,28 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same for an event that comes only after another role's work of any length: the limit counts from the last change of
+// *progress, which that role moves on while it works.
+__device__ __forceinline__ bool mbar_wait_behind(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                 volatile int* progress, int* status, int where) {
+  if (mbar_try_wait(bar, parity)) return true;
+  long long t0 = clock64();
+  int seen = *progress;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    const int now = *progress;
+    if (now != seen) {
+      seen = now;
+      t0 = clock64();
+    } else if (clock64() - t0 > kSpinCycles) {
+      *abort_flag = 1;
+      if (status) atomicCAS(status, 0, 1000 + where);
+      return false;
+    }
+  }
+}
+
 // ── TMA ─────────────────────────────────────────────────────────────────────
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
