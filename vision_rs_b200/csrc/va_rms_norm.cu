@@ -485,6 +485,10 @@ template <typename T> int rms_norm_bwd(NormBwdArgs a, float* dw, void* ws, size_
     return set_error(VA_ERR_WORKSPACE, "rms_norm backward: workspace %zu < %zu bytes", ws_bytes, need);
   if (reinterpret_cast<uintptr_t>(ws) & 15)
     return set_error(VA_ERR_ALIGN, "rms_norm backward: workspace needs 16-byte alignment");
+  if (a.rows == 0) {  // no row to read, w neither: it may be null
+    const cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)a.cols * 4, st);
+    return e == cudaSuccess ? VA_OK : set_error(VA_ERR_LAUNCH, "rms_norm backward: %s", cudaGetErrorString(e));
+  }
   a.partial = static_cast<float*>(ws);
   constexpr int VEC = 16 / sizeof(T);
   const bool vec = a.cols % VEC == 0 && aligned16(a.dy) && aligned16(a.h) && aligned16(a.w) && aligned16(a.grad_h) &&
