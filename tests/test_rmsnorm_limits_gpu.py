@@ -16,3 +16,19 @@ def test_backward_of_no_rows_reads_nothing(cuda, sfx, cols):
     _lib.call(f"va_rms_norm_bwd_{sfx}", None, None, None, 0, None, None, dw.data_ptr(), 0, cols, 1e-6, ws.data_ptr(), need,
               torch.cuda.current_stream().cuda_stream)
     assert (dw == 0).all()
+
+
+def test_backward_workspace(cuda):
+    """A host tensor, or one whose elements are not where its size says, never reaches a kernel; a smaller one is not used."""
+    from vision_rs_b200 import _lib, rmsnorm
+    g = torch.Generator().manual_seed(0)
+    dy, h, w = (torch.randn(*s, generator=g).to(cuda) for s in ((40, 96), (40, 96), (96,)))
+    need = _lib.lib().va_rms_norm_bwd_workspace_bytes(40, 96)
+    ref = rmsnorm.rms_norm_backward(dy, h, w)
+    for bad in (torch.empty(need, dtype=torch.uint8), torch.empty(1, dtype=torch.uint8, device=cuda).expand(need),
+                torch.empty(2 * need, dtype=torch.uint8, device=cuda)[::2]):
+        with pytest.raises(ValueError):
+            rmsnorm.rms_norm_backward(dy, h, w, workspace=bad)
+    for ws in (torch.empty(need, dtype=torch.uint8, device=cuda), torch.empty(need // 4 + 8, device=cuda),
+               torch.empty(16, dtype=torch.uint8, device=cuda)):
+        assert all(torch.equal(a, b) for a, b in zip(ref, rmsnorm.rms_norm_backward(dy, h, w, workspace=ws)))

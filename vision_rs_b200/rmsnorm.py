@@ -85,7 +85,8 @@ def rms_norm_forward_f8(x, w, residual=None, eps: float = 1e-6, group: int = 0, 
 def rms_norm_backward(grad_y, h, w, eps: float = 1e-6, grad_h=None, workspace=None, stream=None):
     """``(grad, grad_w)``: the gradient of ``x`` and of ``residual`` alike
     (with ``grad_h``, the gradient that reaches ``h`` itself, added), and
-    f32 ``[cols]`` of the weight.  ``h`` is the sum that the forward returned."""
+    f32 ``[cols]`` of the weight.  ``h`` is the sum that the forward returned.
+    A ``workspace`` smaller than needed is not used."""
     if stream is not None:
         with _launch.on(stream):
             return rms_norm_backward(grad_y, h, w, eps, grad_h, workspace)
@@ -93,6 +94,8 @@ def rms_norm_backward(grad_y, h, w, eps: float = 1e-6, grad_h=None, workspace=No
     pw, w32 = _weight(w, h, index, cols)
     py = _same(grad_y, "grad_y", h, index)
     pg = None if grad_h is None else _same(grad_h, "grad_h", h, index)
+    if workspace is not None and (workspace.get_device() != index or not workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous CUDA tensor on the rows' device")
     need = _launch.entry("va_rms_norm_bwd_workspace_bytes")(rows, cols)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = h.new_empty(need, dtype=torch.uint8)
