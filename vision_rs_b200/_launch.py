@@ -36,7 +36,14 @@ def run(name: str, index: int, *args) -> None:
         raise _lib.VisionAttnError(name, rc, _lib.lib().va_get_last_error_string().decode(errors="replace"))
 
 
-def on(stream):
-    """Context in which ``stream`` (a torch stream or a raw handle) is the
-    current one, so that what a call allocates belongs to it as well."""
-    return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream)))
+def on(stream, index: int):
+    """Context in which ``stream`` (a torch stream or a raw handle) of device
+    ``index``, the tensors', is the current one, so that what a call allocates
+    belongs to it as well."""
+    if index < 0:
+        raise ValueError("a stream was given, but the tensors are not on a CUDA device")
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(stream), device=index)
+    elif stream.device.index != index:
+        raise ValueError(f"a stream of {stream.device} was given for tensors on cuda:{index}")
+    return torch.cuda.stream(stream)

@@ -54,7 +54,7 @@ class PackedPlan:
     def __init__(self, cu_q, cu_k, total_q: int, total_k: int, num_heads: int, num_kv_heads: int, head_dim: int,
                  causal: bool = False, training: bool = False, used_k=None, stream=None):
         if stream is not None:
-            with _launch.on(stream):
+            with _launch.on(stream, cu_q.get_device()):
                 return self.__init__(cu_q, cu_k, total_q, total_k, num_heads, num_kv_heads, head_dim, causal, training,
                                      used_k)
         index = cu_q.get_device()
@@ -80,7 +80,7 @@ class PackedPlan:
     def check(self, stream=None):
         """Raises if the offsets were out of order or range (synchronises)."""
         if stream is not None:
-            with _launch.on(stream):
+            with _launch.on(stream, self.index):
                 return self.check()
         bad = C.c_int(0)
         _launch.run("va_packed_plan_status", self.index, self.ptr, self.sizes[7], C.byref(bad))
@@ -113,7 +113,7 @@ def packed_attention_forward(q, k, v, plan: PackedPlan, scale: float | None = No
     """``(out [total_q, heads, dim], lse f32 [heads, total_q])``; ``scale``
     defaults to dim^-½.  A query that sees no key has out 0 and lse −∞."""
     if stream is not None:
-        with _launch.on(stream):
+        with _launch.on(stream, plan.index):
             return packed_attention_forward(q, k, v, plan, scale, out, lse)
     sizes, index, dtype = plan.sizes, plan.index, q.dtype
     name = _FWD.get(dtype)
@@ -140,7 +140,7 @@ def packed_attention_backward(grad_out, q, k, v, out, lse, plan: PackedPlan, sca
     plan must be built with ``training=True``.  ``grads``: three tensors to
     write, which may be slices of one packed gradient."""
     if stream is not None:
-        with _launch.on(stream):
+        with _launch.on(stream, plan.index):
             return packed_attention_backward(grad_out, q, k, v, out, lse, plan, scale, grads)
     sizes, index, dtype = plan.sizes, plan.index, q.dtype
     name = _BWD.get(dtype)

@@ -52,7 +52,7 @@ def rms_norm_forward(x, w, residual=None, eps: float = 1e-6, out=None, out_h=Non
     """``(y, h)``; without a residual ``h`` is ``x`` itself.  ``out_h`` may be
     ``x`` or ``residual`` (the sum is then updated in place)."""
     if stream is not None:
-        with _launch.on(stream):
+        with _launch.on(stream, x.get_device()):
             return rms_norm_forward(x, w, residual, eps, out, out_h)
     index, rows, cols = _rows(x)
     pw, w32 = _weight(w, x, index, cols)
@@ -68,7 +68,7 @@ def rms_norm_forward_f8(x, w, residual=None, eps: float = 1e-6, group: int = 0, 
     ``[..., cols/group]`` (``group`` 0: one for each row) with
     ``y ≈ q · scale`` and the largest magnitude of each group at 448."""
     if stream is not None:
-        with _launch.on(stream):
+        with _launch.on(stream, x.get_device()):
             return rms_norm_forward_f8(x, w, residual, eps, group, out_h)
     index, rows, cols = _rows(x)
     if group < 0 or (group and cols % group):
@@ -88,7 +88,7 @@ def rms_norm_backward(grad_y, h, w, eps: float = 1e-6, grad_h=None, workspace=No
     f32 ``[cols]`` of the weight.  ``h`` is the sum that the forward returned.
     A ``workspace`` smaller than needed is not used."""
     if stream is not None:
-        with _launch.on(stream):
+        with _launch.on(stream, h.get_device()):
             return rms_norm_backward(grad_y, h, w, eps, grad_h, workspace)
     index, rows, cols = _rows(h)
     pw, w32 = _weight(w, h, index, cols)

@@ -47,7 +47,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, stretch: float = 1.0
 
 def _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, stream):
     if stream is not None:
-        with _launch.on(stream):
+        with _launch.on(stream, q.get_device()):
             return _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, None)
     dtype, index = q.dtype, q.get_device()
     name = _ENTRY.get(dtype)
