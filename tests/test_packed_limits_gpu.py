@@ -37,3 +37,26 @@ def test_a_unit_of_more_than_a_second(cuda):
     # the weights' sum: steps of 64 stay exact in 32 bits, the last keys are rounded to 16 in 2·10^8
     mean = (n + 255) // 256 / n
     assert ((o.double() - mean).abs() <= 2.0 ** -8 * mean).all() and ((lse - math.log(n)).abs() <= 1e-6 * math.log(n)).all()
+
+
+def test_rotary_in_place_and_overlapping(cuda):
+    """In place (slices of one product, head-major, one alone) gives the bits of a separate output; other overlaps are refused."""
+    from vision_rs_b200 import rotary
+    T, H, Hk, D = 37, 6, 2, 64
+    qkv = torch.randn(T, H + 2 * Hk, D, generator=torch.Generator().manual_seed(0)).to(cuda, torch.bfloat16)
+    pos, inv = torch.arange(T, device=cuda), rotary.rotary_frequencies(D)
+    split = lambda t: t.split([H, Hk, Hk], dim=1)
+    q, k, v = split(qkv)
+    ref = rotary.rotary_forward(q, k, pos, inv)
+    for which in ((0, 1), (0,), (1,)):
+        buf = qkv.clone()
+        a, b, c = split(buf)
+        out = (a if 0 in which else torch.empty_like(a), b if 1 in which else torch.empty_like(b))
+        got = rotary.rotary_forward(a, b, pos, inv, out=out)
+        assert all(torch.equal(x, y) for x, y in zip(got, ref)) and torch.equal(c, v)
+    major = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k)]
+    assert all(torch.equal(x, y) for x, y in zip(rotary.rotary_forward(*major, pos, inv, out=tuple(major)), ref))
+    for bad in ((qkv[:, 1:H + 1], torch.empty_like(k)), (k, k), (q, q[:, :Hk]), (q[:1].expand(T, H, D), k)):
+        with pytest.raises(ValueError):
+            rotary.rotary_forward(q, k, pos, inv, out=bad)
+    assert torch.equal(qkv[:, :H], q)

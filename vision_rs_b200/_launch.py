@@ -47,3 +47,49 @@ def on(stream, index: int):
     elif stream.device.index != index:
         raise ValueError(f"a stream of {stream.device} was given for tensors on cuda:{index}")
     return torch.cuda.stream(stream)
+
+
+def _starts(t):
+    """Byte addresses of the heads' first elements of ``[tokens, heads, dim]``, sorted."""
+    tokens, heads, _ = t.shape
+    row, head, _ = t.stride()
+    at = torch.arange(tokens)[:, None] * row + torch.arange(heads) * head
+    return (at * t.element_size() + t.data_ptr()).flatten().sort().values
+
+
+def overlap(a, b) -> bool:
+    """Whether two tensors ``[tokens, heads, dim]`` of one type (dimensions
+    contiguous, strides not negative) share an element."""
+    (ta, ha, d), (tb, hb, e) = a.shape, b.shape
+    if not (ta and ha and d and tb and hb and e):
+        return False
+    (row_a, head_a, _), (row_b, head_b, _) = a.stride(), b.stride()
+    size, pa, pb = a.element_size(), a.data_ptr(), b.data_ptr()
+    end_a = pa + ((ta - 1) * row_a + (ha - 1) * head_a + d) * size
+    end_b = pb + ((tb - 1) * row_b + (hb - 1) * head_b + e) * size
+    if end_a <= pb or end_b <= pa:
+        return False
+    # slices of one packed tensor: a period of the buffer holds both, one beside the other
+    for period, other, of_a, of_b in ((row_a, row_b, (ha - 1) * head_a + d, (hb - 1) * head_b + e),
+                                      (head_a, head_b, (ta - 1) * row_a + d, (tb - 1) * row_b + e)):
+        if period == other and period >= max(of_a, of_b) and (pb - pa) % size == 0:
+            apart = (pb - pa) // size % period
+            if of_a <= apart <= period - of_b:
+                return False
+    starts, other = _starts(a), _starts(b)
+    after = torch.searchsorted(other, starts).clamp(max=len(other) - 1)  # the nearest of b's at or behind each of a's
+    before = (after - 1).clamp(min=0)
+    gap = other[after] - starts
+    near = ((gap >= 0) & (gap < d * size)) | (((starts - other[before]) >= 0) & ((starts - other[before]) < e * size))
+    return bool((near | ((gap < 0) & (-gap < e * size))).any())
+
+
+def overlaps_itself(t) -> bool:
+    """Whether two elements of ``[tokens, heads, dim]`` are one in memory."""
+    tokens, heads, d = t.shape
+    row, head, _ = t.stride()
+    (near, n), (far, m) = sorted(((row, tokens), (head, heads))) if tokens > 1 and heads > 1 else \
+        ((0, 1), (row, tokens) if tokens > 1 else (head, heads))
+    if (n == 1 or near >= d) and (m <= 1 or far >= (n - 1) * near + d):
+        return False
+    return bool((_starts(t).diff() < d * t.element_size()).any())

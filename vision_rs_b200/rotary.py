@@ -45,6 +45,21 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, stretch: float = 1.0
     return inv.to(device)
 
 
+def _refuse_overlap(q, k, qo, ko):
+    """Other threads write a head's output while its input is read: only exactly in place is that the same element's."""
+    outs, ins = [o for o in (qo, ko) if o is not None], [i for i in (q, k) if i is not None]
+    if any(_launch.overlaps_itself(o) for o in outs):
+        raise ValueError("an output's elements share memory")
+    in_place = [o.data_ptr() == i.data_ptr() and o.stride() == i.stride() for o, i in zip(outs, ins)]
+    if all(in_place):
+        if len(outs) < 2 or not _launch.overlap(qo, ko):
+            return
+    elif not any(_launch.overlap(o, i) for n, o in enumerate(outs) for m, i in enumerate(ins) if n != m or not in_place[n]) \
+            and not (len(outs) == 2 and _launch.overlap(qo, ko)):
+        return
+    raise ValueError("outputs may be the inputs exactly in place, but not overlap them or each other otherwise")
+
+
 def _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, stream):
     if stream is not None:
         with _launch.on(stream, q.get_device()):
@@ -95,6 +110,13 @@ def _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, stream
         pko = ko.data_ptr()
     if one != 1 and dim > 1:
         raise ValueError("a head's dimensions must be contiguous")
+    if out is not None:
+        # (the usual case at once: slices of one packed product, in place; a token's heads in a row, q's beside k's)
+        of_q, of_k = (heads - 1) * q_head + dim, (kv_heads - 1) * k_head + dim if kv_heads else 0
+        apart = (pk - q.data_ptr()) // q.element_size() % max(q_row, 1) if kv_heads else of_q
+        if not (qo is q and ko is k and q_head >= dim and (kv_heads == 0 or (k_row == q_row and k_head >= dim))
+                and of_q <= apart <= q_row - of_k):
+            _refuse_overlap(q, k, qo, ko)
     _launch.run(name, index, q.data_ptr(), pk, qo.data_ptr(), pko,
                 _Strides(q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head), positions.data_ptr(),
                 position_bytes, inv_freq.data_ptr(), tokens, heads, kv_heads, dim, rot, interleaved, backward, factor)
@@ -104,7 +126,7 @@ def _apply(q, k, positions, inv_freq, interleaved, factor, backward, out, stream
 def rotary_forward(q, k, positions, inv_freq, interleaved: bool = False, factor: float = 1.0, out=None, stream=None):
     """Turned ``(q, k)``; ``k`` may be None.  ``factor`` multiplies the turned
     dimensions.  ``out``: a pair of tensors to write, which may be ``(q, k)``
-    themselves."""
+    themselves, but not overlap them (or each other) in another way."""
     return _apply(q, k, positions, inv_freq, interleaved, factor, 0, out, stream)
 
 
