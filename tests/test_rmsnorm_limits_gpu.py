@@ -32,3 +32,31 @@ def test_backward_workspace(cuda):
     for ws in (torch.empty(need, dtype=torch.uint8, device=cuda), torch.empty(need // 4 + 8, device=cuda),
                torch.empty(16, dtype=torch.uint8, device=cuda)):
         assert all(torch.equal(a, b) for a, b in zip(ref, rmsnorm.rms_norm_backward(dy, h, w, workspace=ws)))
+
+
+@pytest.mark.parametrize("cols", [384, 50])
+def test_outputs_in_place_and_overlapping(cuda, cols):
+    """Exactly in place gives the bits of separate outputs; rows shifted against their inputs are refused."""
+    from vision_rs_b200 import rmsnorm
+    g = torch.Generator().manual_seed(1)
+    R = 30
+    big = torch.randn(R + 8, cols, generator=g).to(cuda)
+    res, w = torch.randn(R, cols, generator=g).to(cuda), torch.randn(cols, generator=g).to(cuda)
+    x = big[:R]
+    y, h = rmsnorm.rms_norm_forward(x.clone(), w, res)
+    for pick in ((0, None), (None, 0), (1, 0), (0, 1), (None, 1)):
+        a, b = x.clone(), res.clone()
+        out, out_h = (None if i is None else (a, b)[i] for i in pick)
+        got = rmsnorm.rms_norm_forward(a, w, b, out=out, out_h=out_h)
+        assert torch.equal(got[0], y) and torch.equal(got[1], h)
+    q, s, h8 = rmsnorm.rms_norm_forward_f8(x.clone(), w, res)
+    b = res.clone()
+    got = rmsnorm.rms_norm_forward_f8(x.clone(), w, b, out_h=b)
+    assert torch.equal(got[0].view(torch.uint8), q.view(torch.uint8)) and torch.equal(got[1], s) and torch.equal(got[2], h8)
+    one = torch.empty_like(x)
+    for bad in (dict(out=big[2:R + 2]), dict(out_h=big[1:R + 1]), dict(out=one, out_h=one),
+                dict(out=big[8:], out_h=x)):
+        with pytest.raises(ValueError):
+            rmsnorm.rms_norm_forward(x, w, res, **bad)
+    with pytest.raises(ValueError):
+        rmsnorm.rms_norm_forward_f8(x, w, res, out_h=big[3:R + 3])

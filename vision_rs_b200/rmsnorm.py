@@ -37,11 +37,19 @@ def _weight(w, x, index, cols):
     return w.data_ptr(), f32
 
 
+def _apart(name, p, nbytes, *others):
+    """Rows shifted against each other would be read and written by different blocks; exactly in place is fine."""
+    for o in others:
+        if o is not None and o != p and abs(o - p) < nbytes:
+            raise ValueError(f"{name} overlaps another tensor of the call, and not exactly in place")
+    return p
+
+
 def _sum(x, residual, out_h, index):
     """Addresses of the residual and of the tensor for the sum, and that tensor (x itself without either)."""
     pr = None if residual is None else _same(residual, "residual", x, index)
     if out_h is not None:
-        return pr, _same(out_h, "out_h", x, index), out_h
+        return pr, _apart("out_h", _same(out_h, "out_h", x, index), x.nbytes, x.data_ptr(), pr), out_h
     if residual is None:
         return None, None, x
     h = torch.empty_like(x)
@@ -50,16 +58,23 @@ def _sum(x, residual, out_h, index):
 
 def rms_norm_forward(x, w, residual=None, eps: float = 1e-6, out=None, out_h=None, stream=None):
     """``(y, h)``; without a residual ``h`` is ``x`` itself.  ``out_h`` may be
-    ``x`` or ``residual`` (the sum is then updated in place)."""
+    ``x`` or ``residual`` (the sum is then updated in place), and ``out`` either
+    that is not ``out_h``."""
     if stream is not None:
         with _launch.on(stream, x.get_device()):
             return rms_norm_forward(x, w, residual, eps, out, out_h)
     index, rows, cols = _rows(x)
     pw, w32 = _weight(w, x, index, cols)
     pr, ph, h = _sum(x, residual, out_h, index)
-    y = torch.empty_like(x) if out is None else out
-    _launch.run(_FWD[x.dtype], index, x.data_ptr(), pr, pw, w32, ph,
-                y.data_ptr() if out is None else _same(out, "out", x, index), rows, cols, eps)
+    px = x.data_ptr()
+    if out is None:
+        y = torch.empty_like(x)
+        py = y.data_ptr()
+    else:
+        y, py = out, _apart("out", _same(out, "out", x, index), x.nbytes, px, pr, ph)
+        if py == ph and rows:
+            raise ValueError("out and out_h are one tensor")
+    _launch.run(_FWD[x.dtype], index, px, pr, pw, w32, ph, py, rows, cols, eps)
     return y, h
 
 
