@@ -60,3 +60,32 @@ def test_rotary_in_place_and_overlapping(cuda):
         with pytest.raises(ValueError):
             rotary.rotary_forward(q, k, pos, inv, out=bad)
     assert torch.equal(qkv[:, :H], q)
+
+
+def test_calls_that_share_a_plan_follow_one_another(cuda):
+    """A call on a second stream waits for the first stream's call, and the first stream's next one for it."""
+    from vision_rs_b200 import packed
+    lk, H, Hk, D = [3000, 40, 900], 8, 2, 64
+    g = torch.Generator().manual_seed(0)
+    new = lambda n, h: torch.randn(n, h, D, generator=g).to(cuda, torch.bfloat16)
+    k, v, qs = new(sum(lk), Hk), new(sum(lk), Hk), [new(3, H) for _ in range(3)]
+    make = lambda: packed.PackedPlan(packed.cu_seqlens([1] * 3), packed.cu_seqlens(lk), 3, sum(lk), H, Hk, D, causal=True)
+    refs = [packed.packed_attention_forward(q, k, v, make())[0] for q in qs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    plan = make()
+    torch.cuda.synchronize()
+    for first, second in (streams, streams[::-1], (torch.cuda.current_stream(), streams[0]), (streams[0].cuda_stream, streams[1])):
+        done, outs = [], []
+        for n, s in enumerate((first, second, first)):
+            ext = s if isinstance(s, torch.cuda.Stream) else torch.cuda.ExternalStream(s)
+            with torch.cuda.stream(ext):
+                if n == 0:
+                    torch.cuda._sleep(40_000_000)  # ~20 ms
+                outs.append(packed.packed_attention_forward(qs[n], k, v, plan, stream=s)[0])
+                done.append(torch.cuda.Event())
+                done[-1].record()
+        done[1].synchronize()
+        assert done[0].query()
+        done[2].synchronize()
+        assert done[1].query() and all(torch.equal(a, b) for a, b in zip(outs, refs))
+    plan.check()

@@ -45,8 +45,11 @@ def _plan_bytes(*sizes) -> int:
 
 class PackedPlan:
     """Work lists of packed-sequence attention for one batch's sequences and
-    one head layout (with the kernels' partial results: calls that share a
-    plan must not overlap on the GPU).  With ``used_k`` (int32 ``[n]`` on the
+    one head layout, with the kernels' partial results: calls that share a
+    plan follow one another on the GPU.  A call on another stream than the
+    last one's waits for that stream's work so far; within a capture the
+    caller orders the streams (and a graph that holds a plan's calls must not
+    overlap other calls with it).  With ``used_k`` (int32 ``[n]`` on the
     device) only that many of a sequence's key rows hold keys: a cache with
     room to grow.  The offsets stay on the device and are read on ``stream``; ``check()`` raises if they were not
     ascending offsets from 0 to the totals."""
@@ -73,7 +76,7 @@ class PackedPlan:
         self.index = index
         self.buf = cu_q.new_empty(need, dtype=torch.uint8)
         self.ptr = self.buf.data_ptr()
-        self.stream = _launch.raw_stream(index)
+        self.stream = self.home = _launch.raw_stream(index)  # of the last call, and of the buffer
         _launch.run("va_packed_plan_build", index, cu_q.data_ptr(), cu_k.data_ptr(),
                     None if used_k is None else used_k.data_ptr(), *sizes, self.ptr, need)
 
@@ -82,14 +85,25 @@ class PackedPlan:
         if stream is not None:
             with _launch.on(stream, self.index):
                 return self.check()
+        if _launch.raw_stream(self.index) != self.stream:
+            self._move()
         bad = C.c_int(0)
         _launch.run("va_packed_plan_status", self.index, self.ptr, self.sizes[7], C.byref(bad))
         if bad.value:
             raise ValueError("cu_q or cu_k are not ascending offsets from 0 to the number of tokens")
 
-    def _use(self):
-        """For a call on another stream than the plan's own: the buffer must outlive it."""
-        self.buf.record_stream(torch.cuda.current_stream(self.index))
+    def _move(self):
+        """Before a call on another stream than the last one's."""
+        now = torch.cuda.current_stream(self.index)
+        if now.cuda_stream != self.home:
+            self.buf.record_stream(now)  # the buffer must outlive the call
+        with _launch.on(self.stream or torch.cuda.default_stream(self.index), self.index):
+            last, captured = torch.cuda.current_stream(self.index), torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self.index):
+            if captured or torch.cuda.is_current_stream_capturing():
+                return
+        now.wait_stream(last)
+        self.stream = now.cuda_stream
 
 
 def _heads(t, name, dtype, index, shape):
@@ -127,7 +141,7 @@ def packed_attention_forward(q, k, v, plan: PackedPlan, scale: float | None = No
     out = q.new_empty_strided(sq, (h * d, d, 1)) if out is None else _dense(out, "out", sq, dtype, index)
     lse = q.new_empty((h, tq), dtype=torch.float32) if lse is None else _dense(lse, "lse", (h, tq), torch.float32, index)
     if _launch.raw_stream(index) != plan.stream:
-        plan._use()
+        plan._move()
     _launch.run(name, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
                 _Strides6(q_row, q_head, k_row, k_head, v_row, v_head), *sizes, d ** -0.5 if scale is None else scale,
                 plan.ptr, plan.nbytes)
@@ -158,7 +172,7 @@ def packed_attention_backward(grad_out, q, k, v, out, lse, plan: PackedPlan, sca
                          *_heads(gq, "grad_q", dtype, index, sq), *_heads(gk, "grad_k", dtype, index, sk),
                          *_heads(gv, "grad_v", dtype, index, sk))
     if _launch.raw_stream(index) != plan.stream:
-        plan._use()
+        plan._move()
     _launch.run(name, index, grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                 lse.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), strides, *sizes,
                 d ** -0.5 if scale is None else scale, plan.ptr, plan.nbytes)
