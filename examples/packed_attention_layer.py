@@ -80,10 +80,14 @@ class Cache:
         self.first = room * torch.arange(n + 1, dtype=torch.int32, device="cuda")
         self.one = torch.arange(n + 1, dtype=torch.int32, device="cuda")
         self.used = torch.zeros(n, dtype=torch.int32, device="cuda")
+        self.room, self.length = room, 0  # the host counts along: every sequence grows by one a step
 
     def token(self, layer: PackedAttentionLayer, x, residual, eight_bits=False):
         """One new token of every sequence: ``x [n, hidden]`` → ``(O, h)``."""
         n = x.shape[0]
+        if self.length == self.room:  # the next row is another sequence's, or none
+            raise ValueError(f"the cache holds {self.room} tokens a sequence")
+        self.length += 1
         q, k, v = layer._split(layer._qkv(x, residual, eight_bits)[0])
         h = x + residual
         q, k = rotary.rotary_forward(q, k, self.used, layer.inv_freq)  # the position is the number of tokens so far
