@@ -89,3 +89,31 @@ def test_calls_that_share_a_plan_follow_one_another(cuda):
         done[2].synchronize()
         assert done[1].query() and all(torch.equal(a, b) for a, b in zip(outs, refs))
     plan.check()
+
+
+@pytest.mark.parametrize("lens", [[30, 60], [900, 700, 1100, 800]])
+def test_results_over_inputs(cuda, lens):
+    """out over a contiguous q gives the bits of a separate out; results over other inputs are refused."""
+    from vision_rs_b200 import packed
+    H, Hk, D, T = 16, 8, 64, sum(lens)
+    g = torch.Generator().manual_seed(0)
+    new = lambda h: torch.randn(T, h, D, generator=g).to(cuda, torch.bfloat16)
+    q, k, v, do, qkv = new(H), new(Hk), new(Hk), new(H), new(H + 2 * Hk)
+    cu = packed.cu_seqlens(lens)
+    plan = packed.PackedPlan(cu, cu, T, T, H, Hk, D, causal=True, training=True)
+    out, lse = packed.packed_attention_forward(q, k, v, plan)
+    q2 = q.clone()
+    o2, lse2 = packed.packed_attention_forward(q2, k, v, plan, out=q2)
+    assert o2 is q2 and torch.equal(o2, out) and torch.equal(lse2, lse)
+    sq, sk, sv = qkv.split([H, Hk, Hk], dim=1)
+    flat = qkv.view(-1)
+    for bad in (flat[:T * H * D].view(T, H, D), flat[-T * H * D:].view(T, H, D)):
+        with pytest.raises(ValueError):
+            packed.packed_attention_forward(sq, sk, sv, plan, out=bad)
+    grads = packed.packed_attention_backward(do, q, k, v, out, lse, plan)
+    buf = torch.empty_like(qkv)
+    got = packed.packed_attention_backward(do, q, k, v, out, lse, plan, grads=buf.split([H, Hk, Hk], dim=1))
+    assert all(torch.equal(a, b) for a, b in zip(grads, got))
+    for bad in ((q, k, v), (do, grads[1], grads[2]), (out, grads[1], grads[2]), (grads[0], grads[1], k)):
+        with pytest.raises(ValueError):
+            packed.packed_attention_backward(do, q, k, v, out, lse, plan, grads=bad)

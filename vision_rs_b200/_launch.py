@@ -57,18 +57,23 @@ def _starts(t):
     return (at * t.element_size() + t.data_ptr()).flatten().sort().values
 
 
+def span(t):
+    """Addresses of the first byte of ``[tokens, heads, dim]`` and past the last."""
+    tokens, heads, d = t.shape
+    row, head, _ = t.stride()
+    p = t.data_ptr()
+    return p, p + ((tokens - 1) * row + (heads - 1) * head + d) * t.element_size() if tokens and heads and d else p
+
+
 def overlap(a, b) -> bool:
     """Whether two tensors ``[tokens, heads, dim]`` of one type (dimensions
     contiguous, strides not negative) share an element."""
+    (pa, end_a), (pb, end_b) = span(a), span(b)
+    if pa == end_a or pb == end_b or end_a <= pb or end_b <= pa:
+        return False
     (ta, ha, d), (tb, hb, e) = a.shape, b.shape
-    if not (ta and ha and d and tb and hb and e):
-        return False
     (row_a, head_a, _), (row_b, head_b, _) = a.stride(), b.stride()
-    size, pa, pb = a.element_size(), a.data_ptr(), b.data_ptr()
-    end_a = pa + ((ta - 1) * row_a + (ha - 1) * head_a + d) * size
-    end_b = pb + ((tb - 1) * row_b + (hb - 1) * head_b + e) * size
-    if end_a <= pb or end_b <= pa:
-        return False
+    size = a.element_size()
     # slices of one packed tensor: a period of the buffer holds both, one beside the other
     for period, other, of_a, of_b in ((row_a, row_b, (ha - 1) * head_a + d, (hb - 1) * head_b + e),
                                       (head_a, head_b, (ta - 1) * row_a + d, (tb - 1) * row_b + e)):

@@ -123,9 +123,26 @@ def _dense(t, name, shape, dtype, index):
     return t
 
 
+def _refuse_overlap(written, read):
+    """Results must not lie over what other blocks, or a later kernel, of the call still read.  Each: (tensor, shape,
+    (row, head) strides), whose ends are compared first (small calls are paced by the host)."""
+    lo, hi = 1 << 64, 0
+    for t, (n, heads, d), (row, head) in written:
+        if n:
+            p = t.data_ptr()
+            lo, hi = min(lo, p), max(hi, p + 2 * ((n - 1) * row + (heads - 1) * head + d))
+    for t, (n, heads, d), (row, head) in read:
+        p = t.data_ptr()
+        if p < hi and lo < p + 2 * ((n - 1) * row + (heads - 1) * head + d) \
+                and any(_launch.overlap(w, t) for w, _, _ in written):
+            raise ValueError("a result overlaps an input of the call")
+
+
 def packed_attention_forward(q, k, v, plan: PackedPlan, scale: float | None = None, out=None, lse=None, stream=None):
     """``(out [total_q, heads, dim], lse f32 [heads, total_q])``; ``scale``
-    defaults to dim^-½.  A query that sees no key has out 0 and lse −∞."""
+    (positive) defaults to dim^-½.  A query that sees no key has out 0 and lse
+    −∞.  ``out`` may be q itself where that is contiguous, but not overlap the
+    inputs in another way."""
     if stream is not None:
         with _launch.on(stream, plan.index):
             return packed_attention_forward(q, k, v, plan, scale, out, lse)
@@ -135,15 +152,18 @@ def packed_attention_forward(q, k, v, plan: PackedPlan, scale: float | None = No
         raise ValueError("q must be bf16 or f16")
     _, tq, tk, h, hk, d, _, _ = sizes
     sq, sk = (tq, h, d), (tk, hk, d)
-    q_row, q_head = _heads(q, "q", dtype, index, sq)
-    k_row, k_head = _heads(k, "k", dtype, index, sk)
-    v_row, v_head = _heads(v, "v", dtype, index, sk)
-    out = q.new_empty_strided(sq, (h * d, d, 1)) if out is None else _dense(out, "out", sq, dtype, index)
+    qs, ks, vs = _heads(q, "q", dtype, index, sq), _heads(k, "k", dtype, index, sk), _heads(v, "v", dtype, index, sk)
+    if out is None:
+        out = q.new_empty_strided(sq, (h * d, d, 1))
+    else:
+        _dense(out, "out", sq, dtype, index)
+        in_place = out.data_ptr() == q.data_ptr() and qs == (h * d, d)  # a tile's queries are read by its own unit alone
+        _refuse_overlap([(out, sq, (h * d, d))], [(k, sk, ks), (v, sk, vs)] + ([] if in_place else [(q, sq, qs)]))
     lse = q.new_empty((h, tq), dtype=torch.float32) if lse is None else _dense(lse, "lse", (h, tq), torch.float32, index)
     if _launch.raw_stream(index) != plan.stream:
         plan._move()
     _launch.run(name, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                _Strides6(q_row, q_head, k_row, k_head, v_row, v_head), *sizes, d ** -0.5 if scale is None else scale,
+                _Strides6(*qs, *ks, *vs), *sizes, d ** -0.5 if scale is None else scale,
                 plan.ptr, plan.nbytes)
     return out, lse
 
@@ -152,7 +172,8 @@ def packed_attention_backward(grad_out, q, k, v, out, lse, plan: PackedPlan, sca
                               stream=None):
     """``(grad_q, grad_k, grad_v)`` from the forward's inputs and results; the
     plan must be built with ``training=True``.  ``grads``: three tensors to
-    write, which may be slices of one packed gradient."""
+    write, which may be slices of one packed gradient, but not lie over the
+    inputs (dQ is written before dK's kernel reads q)."""
     if stream is not None:
         with _launch.on(stream, plan.index):
             return packed_attention_backward(grad_out, q, k, v, out, lse, plan, scale, grads)
@@ -167,10 +188,13 @@ def packed_attention_backward(grad_out, q, k, v, out, lse, plan: PackedPlan, sca
     _dense(out, "out", sq, dtype, index)
     _dense(lse, "lse", (h, tq), torch.float32, index)
     gq, gk, gv = (q.new_empty(sq), k.new_empty(sk), v.new_empty(sk)) if grads is None else grads
-    strides = _Strides14(*_heads(q, "q", dtype, index, sq), *_heads(k, "k", dtype, index, sk),
-                         *_heads(v, "v", dtype, index, sk), *_heads(grad_out, "grad_out", dtype, index, sq),
-                         *_heads(gq, "grad_q", dtype, index, sq), *_heads(gk, "grad_k", dtype, index, sk),
-                         *_heads(gv, "grad_v", dtype, index, sk))
+    qs, ks, vs = _heads(q, "q", dtype, index, sq), _heads(k, "k", dtype, index, sk), _heads(v, "v", dtype, index, sk)
+    gos, gqs = _heads(grad_out, "grad_out", dtype, index, sq), _heads(gq, "grad_q", dtype, index, sq)
+    gks, gvs = _heads(gk, "grad_k", dtype, index, sk), _heads(gv, "grad_v", dtype, index, sk)
+    if grads is not None:
+        _refuse_overlap([(gq, sq, gqs), (gk, sk, gks), (gv, sk, gvs)],
+                        [(grad_out, sq, gos), (q, sq, qs), (k, sk, ks), (v, sk, vs), (out, sq, (h * d, d))])
+    strides = _Strides14(*qs, *ks, *vs, *gos, *gqs, *gks, *gvs)
     if _launch.raw_stream(index) != plan.stream:
         plan._move()
     _launch.run(name, index, grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
