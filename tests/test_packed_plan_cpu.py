@@ -36,8 +36,8 @@ int main(int, char** v) {
     items += p;
     slots += p > 1 ? p : 0;
   }
-  printf("%d %lld %d %lld %d %lld %d %d\n", tiles, (long long)blocks, part, items,
-         bwd ? s.max_dkv_items : s.max_items, slots, bwd ? 2 * s.dkv_budget : s.max_slots, tile);
+  printf("%d %lld %d %lld %d %lld %d %d %d\n", tiles, (long long)blocks, part, items,
+         bwd ? s.max_dkv_items : s.max_items, slots, bwd ? 2 * s.dkv_budget : s.max_slots, tile, packed_sums_wide(s));
 }
 """
 
@@ -73,7 +73,8 @@ def _blocks(bwd, lq, lk, group, causal, tile):
     ("f", 1, 8192, 32, 8, 1), ("f", 3000, 1 << 30, 12, 1, 0), ("f", 36000, 1 << 28, 1, 1, 1), ("f", 1, 0, 4, 1, 1),
     ("f", 64, 7 * 128, 8, 1, 0), ("f", 700, 20, 4, 4, 1), ("f", 1 << 30, 1 << 30, 1, 1, 1)])
 def test_parts_keep_to_the_lists(plan, kind, lq, lk, heads, kv, causal):
-    tiles, blocks, part, items, room, slots, slot_room, tile = plan(kind, lq, lk, heads, kv, causal)
+    tiles, blocks, part, items, room, slots, slot_room, tile, wide = plan(kind, lq, lk, heads, kv, causal)
+    assert wide or max(blocks, tiles) < 1 << 31  # the kernel sums in 32 bits then
     if tiles <= 1 << 20:
         assert blocks == _blocks(kind == "b", lq, lk, heads // kv, causal, tile)
     assert blocks >= 0 and tiles <= items <= room and slots <= slot_room
@@ -85,3 +86,9 @@ def test_training_sizes_past_32_bits_are_refused():
     assert size(1, 1 << 20, 1 << 20, 32, 1, 8, 1, 1) > 0
     assert size(1, 1 << 26, 1 << 20, 64, 1, 8, 1, 0) > 0
     assert size(1, 1 << 26, 1 << 20, 64, 1, 8, 1, 1) == 0 and b"training" in _lib.lib().va_get_last_error_string()
+
+
+def test_ordinary_sizes_sum_in_32_bits(plan):
+    for args in (("b", 4095, 4095, 12, 3, 1), ("b", 1 << 17, 1 << 17, 32, 8, 1), ("f", 64, 1 << 20, 32, 8, 1)):
+        assert plan(*args)[-1] == 0
+    assert plan("b", 1 << 20, 1 << 20, 32, 1, 1)[-1] == 1

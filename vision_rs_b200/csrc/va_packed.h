@@ -116,8 +116,8 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   return s;
 }
 
-// The plan's arithmetic (host and device).  Sums over tiles are 64-bit: the dK/dV steps of one document of 2^20 tokens with
-// 32 query heads over one key head already add up to 2^31.
+// The plan's arithmetic (host and device).  Sums over tiles may need 64 bits: the dK/dV steps of one document of 2^20 tokens
+// with 32 query heads over one key head already add up to 2^31 (packed_sums_wide).
 #ifdef __CUDACC__
 #define VA_PACKED_FN __host__ __device__ __forceinline__
 #else
@@ -142,7 +142,16 @@ VA_PACKED_FN int part_blocks(PackedSum blocks, int budget, int smallest) {
   const PackedSum part = (blocks + budget - 1) / budget;
   return part > (1 << 30) ? 1 << 30 : pk_max((int)part, smallest);
 }
-VA_PACKED_FN int part_count(int blocks, int part) { return pk_max(1, (int)(((PackedSum)blocks + part - 1) / part)); }
+VA_PACKED_FN int part_count(int blocks, int part) { return pk_max(1, (blocks + part - 1) / part); }  // blocks < 2^27
+
+// Whether a sum over tiles can pass 31 bits, whatever the offsets say (each sequence's are clamped to the totals; a list
+// has at most its room of tiles).
+inline bool packed_sums_wide(const PackedShape& s) {
+  const double seqs = s.num_seqs, q = s.total_q, k = s.total_k, most = 2147483647.0;
+  if (seqs * (q / s.q_tile + 1) > most || s.max_tiles * (k / kPackBlock + 1) > most) return true;
+  return s.training && (seqs * (std::max(q, k) / kPackBlock + 1) > most ||
+                        s.max_dkv_tiles * (q / 64 + 1) * s.group > most || s.max_dq_items * (k / kPackBlock + 1) > most);
+}
 
 int packed_status_read(int* out, cudaStream_t st);
 int packed_status_clear(cudaStream_t st);

@@ -89,7 +89,8 @@ __device__ __forceinline__ int seq_of_tile(const int* first, int num_seqs, int t
   return lo;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
+// Sum: int, or PackedSum where packed_sums_wide says so (0.3–0.5 µs more).
+template <typename Sum> __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
   __shared__ int hist[kClasses], cursor[kClasses];
   __shared__ int bad, full, most, first_smem[kPlanSeqs + 1];
   const PackedShape& s = a.s;
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
   for (int c = tid; c < kClasses; c += kPlanThreads) hist[c] = 0;
   __syncthreads();
 
-  PackedSum sum_tiles = 0;
+  Sum sum_tiles = 0;
   for (int b0 = 0; b0 < s.num_seqs; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int n = 0;
@@ -114,17 +115,17 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
       const Seq q = load_seq(a.cu_q, a.cu_k, a.used_k, s.num_seqs, b, s.total_q, s.total_k, &bad);
       n = ((list == 2 ? q.lk : q.lq) + tile - 1) / tile;
     }
-    PackedSum sum;
-    const PackedSum before = block_scan<PackedSum>(n, &sum);
-    if (b < s.num_seqs) first[b] = (int)min(sum_tiles + before, (PackedSum)INT_MAX);
+    Sum sum;
+    const Sum before = block_scan<Sum>(n, &sum);
+    if (b < s.num_seqs) first[b] = (int)min(sum_tiles + before, (Sum)INT_MAX);
     sum_tiles += sum;
   }
-  if (tid == 0) first[s.num_seqs] = (int)min(sum_tiles, (PackedSum)INT_MAX);
+  if (tid == 0) first[s.num_seqs] = (int)min(sum_tiles, (Sum)INT_MAX);
   __syncthreads();
   // offsets that run backwards could name more rows than there are: keep to the lists' room
   const int room = list == 0 ? s.max_tiles : list == 1 ? s.max_dq_items : s.max_dkv_tiles;
   if (sum_tiles > room && tid == 0) bad = 1;
-  const int tiles = (int)min(sum_tiles, (PackedSum)room);
+  const int tiles = (int)min(sum_tiles, (Sum)room);
 
   Seq own_seq{};  // the thread's first tile, which every pass below asks for
   int own_i0 = 0, own_blocks = -1;
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
     return n;
   };
 
-  PackedSum mine = 0;
+  Sum mine = 0;
   int mine_most = 0;
   for (int t = tid; t < tiles; t += kPlanThreads) {
     Seq q;
@@ -152,8 +153,8 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PlanArgs a) {
     mine_most = max(mine_most, n);
   }
   atomicMax(&most, mine_most);
-  PackedSum blocks;
-  block_scan<PackedSum>(mine, &blocks);
+  Sum blocks;
+  block_scan<Sum>(mine, &blocks);
   const int budget = list == 0 ? s.split_budget : list == 2 ? s.dkv_budget : 0;
   const int chunk = part_blocks(blocks, budget, list == 0 ? kMinKeyBlocks : kMinQuerySteps);
   const int top = max(1, min(most, chunk));
@@ -266,7 +267,8 @@ int va_packed_plan_build(const int32_t* cu_q, const int32_t* cu_k, const int32_t
     return set_error(VA_ERR_WORKSPACE, "packed plan: %zu < %zu bytes", plan_bytes, a.s.total);
   if (reinterpret_cast<uintptr_t>(plan) & 255)
     return set_error(VA_ERR_ALIGN, "packed plan: the buffer needs 256-byte alignment");
-  return launch_behind("packed plan", packed_plan_kernel, training ? 3 : 1, kPlanThreads, 0, (cudaStream_t)stream, a);
+  auto kernel = packed_sums_wide(a.s) ? packed_plan_kernel<PackedSum> : packed_plan_kernel<int>;
+  return launch_behind("packed plan", kernel, training ? 3 : 1, kPlanThreads, 0, (cudaStream_t)stream, a);
 }
 
 int va_packed_plan_status(const void* plan, int training, int* bad_offsets, va_stream_t stream) {
