@@ -576,8 +576,11 @@ VA_API int va_packed_attention_fwd_f16(const void *q, const void *k, const void 
  * be built with `training`.  strides: as the forward's six, then grad_out row,
  * head, grad_q row, head, grad_k row, head, grad_v row, head.  Rows of keys
  * and queries that see nothing get zeros.  The bits do not depend on scheduling.
- * Another sequence's rows may hold anything; within a sequence a value that is
- * not finite may reach gradients of rows up to 127 positions before it. */
+ * What a row does not see may hold anything, as in the forward: another
+ * sequence's rows, and (causal) a key or value in the gradients of the queries
+ * before it, a query or its grad_out in those of the keys after it.  A gradient that
+ * depends on a value that is not finite is not finite (NaN also where its limit is
+ * infinite).  Results must not lie over the inputs. */
 VA_API int va_packed_attention_bwd_bf16(const va_bf16 *grad_out, const va_bf16 *q, const va_bf16 *k, const va_bf16 *v,
                                         const va_bf16 *out, const float *lse, va_bf16 *grad_q, va_bf16 *grad_k, va_bf16 *grad_v,
                                         const int64_t *strides, int num_seqs, int total_q, int total_k,

@@ -181,9 +181,6 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     for (int i = lane; i < ((used + 15) / 16 * 16 - used) * (DP / 8); i += 32)
       *cell(used + i / (DP / 8), i % (DP / 8)) = make_uint4(0, 0, 0, 0);
     if (hidden < see_end) {
-      constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
-      // an exponent of ones carries into its half's top bit
-      auto flags = [&](uint32_t w) { return (w & kExp) + kOne; };
       uint32_t any = 0;  // all cells are read without a branch between them; the rare second pass mends
 #pragma unroll
       for (int c = 0; c < DP / 64; ++c) {
@@ -192,18 +189,18 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll 8
         for (int i = lane; i < cells; i += 32) {
           const uint4 x = base[i];
-          any |= flags(x.x) | flags(x.y) | flags(x.z) | flags(x.w);
+          any |= not_finite2<BF16>(x.x) | not_finite2<BF16>(x.y) | not_finite2<BF16>(x.z) | not_finite2<BF16>(x.w);
         }
       }
       bool found = false;
-      if (__any_sync(0xffffffffu, (any & 0x80008000u) != 0)) {
+      if (__any_sync(0xffffffffu, any != 0)) {
         for (int i = lane; i < used * (DP / 8); i += 32) {
           uint4* p = cell(i / (DP / 8), i % (DP / 8));
           const uint4 x = *p;
-          auto keep = [&](uint32_t w) {  // without the halves whose top bit is flagged
-            const uint32_t t = (flags(w) & 0x80008000u) >> 15;
-            found |= t != 0;
-            return w & ~(t * 0xffffu);
+          auto keep = [&](uint32_t w) {
+            const uint32_t kept = finite2<BF16>(w);
+            found |= kept != w;
+            return kept;
           };
           *p = make_uint4(keep(x.x), keep(x.y), keep(x.z), keep(x.w));
         }

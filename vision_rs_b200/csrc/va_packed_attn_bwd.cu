@@ -40,8 +40,15 @@
 // sums are scaled back at the end.  bf16 needs neither.  Sequences and rows of
 // at most 128 keys keep P's and dS's remainders as second operands.
 //
-// Rows of other sequences in a tile are masked by selection, and the rows of
-// the summed operand past the sequence's end are zeroed (0 · NaN is NaN).
+// What a row does not see stays out of its gradient, whatever it holds: scores
+// of hidden pairs and of other sequences' rows are masked by selection.  As
+// 0 · NaN is NaN, the rows of the summed operand past the sequence's end are
+// zeroed, and in steps with hidden pairs the score groups look through it while
+// the score MMAs run and leave out what is not finite.  A query or a key that is
+// not finite reaches what depends on it through P and dS all the same; a dO
+// value is given back to dV of the keys that its row sees.  Measured: backward
+// of the 4 documents below 422.5 → 426 µs (a warp of its own for it: 436, the
+// gradients' issuing warp: 443).
 #include <cudaTypedefs.h>
 
 #include <type_traits>
@@ -88,6 +95,7 @@ template <int DP> struct BwdSmem {
   uint64_t s_full[C::kGroups], p_full[C::kGroups], g_done[C::kGroups], fin;
   uint32_t tmem_base;
   int abort, last;
+  int loose;    // something that is not finite was left out of a step's tiles (dK/dV: it may be dO's)
   int scanned;  // f16: how far the score warps are with the norms that bound dS, before their first step
 };
 constexpr unsigned kScanChunk = 4096;  // turns of that loop between two updates of `scanned`
@@ -98,7 +106,30 @@ struct BwdArgs {
   void *dq, *dk, *dv;
   long long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
   float scale;
+  const uint16_t* d_out;
+  long long do_row, do_head;
 };
+
+// A score group's share of `bytes` of a step's tiles (the thread's cells of 16 bytes, in whatever order the swizzle has
+// them): whether they hold anything that is not finite, and the tiles without that.
+template <bool BF16, int BYTES> __device__ __forceinline__ bool holds_loose(const uint8_t* tile, int t) {
+  uint32_t any = 0;
+#pragma unroll 4
+  for (int i = t; i < BYTES / 16; i += 128) {
+    const uint4 x = reinterpret_cast<const uint4*>(tile)[i];
+    any |= not_finite2<BF16>(x.x) | not_finite2<BF16>(x.y) | not_finite2<BF16>(x.z) | not_finite2<BF16>(x.w);
+  }
+  return any != 0;
+}
+template <bool BF16, int BYTES> __device__ __noinline__ void drop_loose(uint8_t* tile, int t, int* flag) {
+  for (int i = t; i < BYTES / 16; i += 128) {
+    uint4* p = reinterpret_cast<uint4*>(tile) + i;
+    const uint4 x = *p;
+    *p = make_uint4(finite2<BF16>(x.x), finite2<BF16>(x.y), finite2<BF16>(x.z), finite2<BF16>(x.w));
+  }
+  fence_proxy_async_smem();
+  *(volatile int*)flag = 1;
+}
 
 // The score warps never leave a loop early: a wait that gives up is passed over, as are the thread's later ones, so that
 // every thread meets every one of these barriers and the lanes of a warp stay together at its TMEM instructions.  The
@@ -140,6 +171,7 @@ template <int DP> __device__ __forceinline__ uint32_t bwd_setup(BwdSmem<DP>& sm,
     }
     mbar_init(&sm.fin, 2);
     sm.abort = 0;
+    sm.loose = 0;
     sm.scanned = 0;
     fence_mbar_init();
   }
@@ -288,11 +320,38 @@ packed_rows_kernel(const uint16_t* __restrict__ out, const uint16_t* __restrict_
   }
 }
 
+// dO values that were left out of a unit's product, to dV of the thread's key, whose row it has stored.  (Not inlined: the
+// kernel's loops need its registers.)
+template <bool BF16>
+__device__ __noinline__ void give_back(const BwdArgs& a, const KItem* item, int kvh, int key) {
+  const PackedShape& ps = a.s;
+  const KItem it = *item;
+  const int off = it.lk - it.lq, j = it.j0 + key, hb0 = ps.causal ? max(0, it.j0 - off) / kHalf : 0;
+  const int nh = (it.lq + kHalf - 1) / kHalf - hb0, last = it.j0 + it.keys - 1 - off;
+  auto value = [](uint16_t w) { return BF16 ? __uint_as_float((uint32_t)w << 16) : __half2float(__ushort_as_half(w)); };
+  uint16_t* out = static_cast<uint16_t*>(a.dv) + (it.k0 + key) * a.dv_row + kvh * a.dv_head;
+  float* part = reinterpret_cast<float*>(a.plan + ps.part_dkv) +
+                (((long long)it.slot * ps.kv_heads + kvh) * 2 * kPackBlock + key) * ps.dim;
+  for (int h = it.h0; h < it.h1; ++h) {
+    const int i0 = (hb0 + h % nh) * kHalf;
+    if (it.lq > kFineSteps * kHalf && !(ps.causal && last > i0)) continue;
+    for (int i = ps.causal ? max(i0, j - off) : i0; i < min(i0 + kHalf, it.lq); ++i) {
+      const uint16_t* row = a.d_out + (it.q0 + i) * a.do_row + (kvh * ps.group + h / nh) * a.do_head;
+      for (int c = 0; c < ps.dim; ++c) {
+        const float x = value(row[c]);
+        if (fabsf(x) < INFINITY) continue;
+        if (it.slot < 0) out[c] = (uint16_t)pack2<BF16>(value(out[c]) + x, 0.0f);
+        else part[c] += x;
+      }
+    }
+  }
+}
+
 // ── dK and dV ────────────────────────────────────────────────────────────────
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool CAUSAL>
 __global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
 packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, BwdArgs a) {
+                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ BwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using C = BwdCfg<DP>;
@@ -307,7 +366,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int dim16 = (ps.dim + 15) & ~15;
   // 64-query blocks of a head from the first that sees a key of the tile, and the unit's steps (block b0 of head g0 first)
-  const int hb0 = ps.causal ? max(0, it.j0 - (it.lk - it.lq)) / kHalf : 0, nh = max(0, (it.lq + kHalf - 1) / kHalf - hb0);
+  const int hb0 = CAUSAL ? max(0, it.j0 - (it.lk - it.lq)) / kHalf : 0, nh = max(0, (it.lq + kHalf - 1) / kHalf - hb0);
   const int n = it.h1 - it.h0, g0 = nh > 0 ? it.h0 / nh : 0, b0 = it.h0 - g0 * nh;
   const bool fine = it.lq <= kFineSteps * kHalf;
   const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
@@ -443,8 +502,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const int gh = i / head_rows, q = hb0 * kHalf + (int)(i - gh * head_rows);
           if (q >= it.lq) continue;
           const long long at = (long long)(kvh * ps.group + gh) * ps.total_q + it.q0 + q;
-          top_n = fmaxf(top_n, norms[at]);
-          top_d = fmaxf(top_d, fabsf(pairs[at].y));
+          const float nq = norms[at], dq = fabsf(pairs[at].y);
+          // (a row that is not finite sets no scale: the keys that it sees get NaN, the others do not depend on it)
+          if (nq < INFINITY) top_n = fmaxf(top_n, nq);
+          if (dq < INFINITY) top_d = fmaxf(top_d, dq);
         }
         if (tid == 0) *(volatile int*)&sm.scanned = (int)(i0 / (C::kSoft * kScanChunk)) + 1;
       }
@@ -462,6 +523,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
     const float mult_p = BF16 ? 1.0f : mult * 3.0517578125e-05f;  // dS from P·2^15
     const int off = it.lk - it.lq, j = it.j0 + key;
+    auto hides_queries = [&](int i0) { return CAUSAL && it.j0 + it.keys - 1 - off > i0; };  // from some key of the tile
     bool ok = true;
     // (lse, Δ) of a step's query, fetched a step ahead by the group's first 64 threads
     int fg = g0, fb = b0;  // head and block of the step that is fetched next
@@ -492,9 +554,16 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       ahead = fetch(h + C::kGroups);
       block = fb;
       // queries [lo, hi) of the step see this key
-      const int lo = ps.causal ? j - off - i0 : 0, hi = it.lq - i0;
-      const bool whole = hi >= kHalf && (!ps.causal || it.j0 + it.keys - 1 - off <= i0);
+      const int lo = CAUSAL ? j - off - i0 : 0, hi = it.lq - i0;
+      const bool hides = hides_queries(i0), whole = hi >= kHalf && !hides;
+      bool loose = false;
+      // (fine: a weight's remainder may be zero or negative, and times infinity that is not the weight's product)
+      if (CAUSAL && (hides || fine)) {
+        ok = ok && mbar_wait(&sm.full[h % kStages], (h / kStages) & 1, &sm.abort, &g_packed_bwd_status, 10);
+        loose = holds_loose<BF16, 2 * BwdSmem<DP>::kStep>(sm.ring[h % kStages][0], key);
+      }
       ok = ok && mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 8);
+      if (loose) drop_loose<BF16, 2 * BwdSmem<DP>::kStep>(sm.ring[h % kStages][0], key, &sm.loose);
       tc_fence_after();
       const float4 *nl = sm.stats[g][k & 1][0], *nd = sm.stats[g][k & 1][1];
       // 16 queries at a time: their statistics are read while the scores come
@@ -615,6 +684,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           __syncwarp();
         }
       }
+      if (g == 0 && mine && *(volatile int*)&sm.loose)
+        give_back<BF16>(a, reinterpret_cast<const KItem*>(a.plan + ps.dkv_items) + unit, kvh, key);
     }
   }
   tc_fence_before();
@@ -670,10 +741,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 }
 
 // ── dQ ───────────────────────────────────────────────────────────────────────
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool CAUSAL>
 __global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
 packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, BwdArgs a) {
+                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ BwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<DP>& sm = *reinterpret_cast<BwdSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using C = BwdCfg<DP>;
@@ -687,7 +758,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const QItem it = reinterpret_cast<const QItem*>(a.plan + ps.dq_items)[unit];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int dim16 = (ps.dim + 15) & ~15;
-  const int see_end = ps.causal ? min(it.lk, max(0, it.see + it.tokens)) : it.lk;  // one past the last key that is seen
+  const int see_end = CAUSAL ? min(it.lk, max(0, it.see + it.tokens)) : it.lk;  // one past the last key that is seen
   const int n = (see_end + kHalf - 1) / kHalf;
   constexpr uint32_t kColQ = kColAcc + DP, kColDO = kColQ + DP / 2;
   const uint32_t tmem = bwd_setup<DP>(sm, tid, warp);
@@ -792,7 +863,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + g * 128;
     const bool mine = row < it.tokens;
-    const int see = !mine ? 0 : ps.causal ? min(it.lk, it.see + row + 1) : it.lk;
+    const int see = !mine ? 0 : CAUSAL ? min(it.lk, it.see + row + 1) : it.lk;
     float2 stat = make_float2(INFINITY, 0.0f);
     const long long at = (long long)head * ps.total_q + it.q0 + row;
     if (mine) stat = reinterpret_cast<const float2*>(a.plan + ps.rows)[at];
@@ -802,7 +873,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       float top = 0.0f;
       for (int i0 = 0; i0 < see_end; i0 += C::kSoft * kScanChunk) {
         const int end = min(see_end, i0 + (int)(C::kSoft * kScanChunk));
-        for (int i = i0 + tid; i < end; i += C::kSoft) top = fmaxf(top, vn[i]);
+        for (int i = i0 + tid; i < end; i += C::kSoft) top = fmaxf(top, vn[i] < INFINITY ? vn[i] : 0.0f);
         if (tid == 0) *(volatile int*)&sm.scanned = i0 / (int)(C::kSoft * kScanChunk) + 1;
       }
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -861,7 +932,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (mine && ok && g == 0) reinterpret_cast<float2*>(a.plan + ps.rows)[at].y = stat.y;
     }
     for (int h = g, k = 0; h < n; h += C::kGroups, ++k) {
+      bool loose = false;
+      if (CAUSAL && (h + 1) * kHalf > it.see + 1) {  // keys that some query of the tile does not see
+        ok = ok && mbar_wait(&sm.full[h % kStages], (h / kStages) & 1, &sm.abort, &g_packed_bwd_status, 11);
+        loose = holds_loose<BF16, BwdSmem<DP>::kStep>(sm.ring[h % kStages][0], row);
+      }
       ok = ok && mbar_wait(&sm.s_full[g], k & 1, &sm.abort, &g_packed_bwd_status, 18);
+      if (loose) drop_loose<BF16, BwdSmem<DP>::kStep>(sm.ring[h % kStages][0], row, &sm.loose);
       tc_fence_after();
       const int limit = see - h * kHalf;
       auto scores = [&](auto masked, auto fine) {
@@ -921,23 +998,23 @@ struct BwdMaps {
   CUtensorMap q_tile, do_tile, k_tile, v_tile, q_step, do_step, k_step, v_step;
 };
 
-template <int DP, bool BF16> int launch_bwd(const BwdMaps& m, const BwdArgs& a, cudaStream_t st) {
+template <int DP, bool BF16, bool CAUSAL> int launch_bwd(const BwdMaps& m, const BwdArgs& a, cudaStream_t st) {
   constexpr int smem = (int)sizeof(BwdSmem<DP>) + 1024;
   static PerDeviceOnce once;
   if (int rc = once.run([&]() -> int {
-        if (int rc = set_smem(packed_dkv_kernel<DP, BF16>, smem)) return rc;
-        return set_smem(packed_dq_kernel<DP, BF16>, smem);
+        if (int rc = set_smem(packed_dkv_kernel<DP, BF16, CAUSAL>, smem)) return rc;
+        return set_smem(packed_dq_kernel<DP, BF16, CAUSAL>, smem);
       }))
     return rc;
   const long long g1 = (long long)a.s.max_dkv_items * a.s.kv_heads, g2 = (long long)a.s.max_dq_items * a.s.heads;
   VA_CHECK_ARG(g1 < (1LL << 31) && g2 < (1LL << 31), "packed attention backward: too many units");
   if (g2 > 0) {
-    if (int rc = launch_behind("packed attention dQ", packed_dq_kernel<DP, BF16>, (unsigned)g2, BwdCfg<DP>::kThreads, smem, st,
+    if (int rc = launch_behind("packed attention dQ", packed_dq_kernel<DP, BF16, CAUSAL>, (unsigned)g2, BwdCfg<DP>::kThreads, smem, st,
                                m.q_tile, m.do_tile, m.k_step, m.v_step, a))
       return rc;
   }
   if (g1 > 0) {
-    if (int rc = launch_behind("packed attention dK/dV", packed_dkv_kernel<DP, BF16>, (unsigned)g1, BwdCfg<DP>::kThreads, smem, st,
+    if (int rc = launch_behind("packed attention dK/dV", packed_dkv_kernel<DP, BF16, CAUSAL>, (unsigned)g1, BwdCfg<DP>::kThreads, smem, st,
                                m.q_step, m.do_step, m.k_tile, m.v_tile, a))
       return rc;
   }
@@ -962,6 +1039,7 @@ int packed_bwd(const void* d_out, const void* q, const void* k, const void* v, c
   if (reinterpret_cast<uintptr_t>(plan) & 255)
     return set_error(VA_ERR_ALIGN, "packed attention backward: the plan needs 256-byte alignment");
   a.dq = dq, a.dk = dk, a.dv = dv, a.scale = scale;
+  a.d_out = static_cast<const uint16_t*>(d_out), a.do_row = strides[6], a.do_head = strides[7];
   a.dq_row = strides[8], a.dq_head = strides[9], a.dk_row = strides[10], a.dk_head = strides[11];
   a.dv_row = strides[12], a.dv_head = strides[13];
   for (int i = 8; i < 14; ++i)
@@ -1000,7 +1078,10 @@ int packed_bwd(const void* d_out, const void* q, const void* k, const void* v, c
                                  reinterpret_cast<float*>(a.plan + a.s.v_norm), total_q, total_k, total_q ? heads : 0, dim))
         return rc;
   }
-  return dim <= 64 ? launch_bwd<64, BF16>(m, a, st) : launch_bwd<128, BF16>(m, a, st);
+  auto go = [&](auto dp) -> int {
+    return causal ? launch_bwd<dp, BF16, true>(m, a, st) : launch_bwd<dp, BF16, false>(m, a, st);
+  };
+  return dim <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
 
 }  // namespace

@@ -64,24 +64,25 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-// The same for an event that comes only after another role's work of any length: the limit counts from the last change of
-// *progress, which that role moves on while it works.
+// The same for an event that comes only after another role's work of any length: once the limit is reached, it starts again
+// if *progress (not negative), which that role moves on while it works, has changed since the last time.
 __device__ __forceinline__ bool mbar_wait_behind(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                  volatile int* progress, int* status, int where) {
   if (mbar_try_wait(bar, parity)) return true;
   long long t0 = clock64();
-  int seen = *progress;
+  int seen = -1;
   while (true) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
-    const int now = *progress;
-    if (now != seen) {
+    if (clock64() - t0 > kSpinCycles) {
+      const int now = *progress;
+      if (now == seen) {
+        *abort_flag = 1;
+        if (status) atomicCAS(status, 0, 1000 + where);
+        return false;
+      }
       seen = now;
       t0 = clock64();
-    } else if (clock64() - t0 > kSpinCycles) {
-      *abort_flag = 1;
-      if (status) atomicCAS(status, 0, 1000 + where);
-      return false;
     }
   }
 }
@@ -338,6 +339,15 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
+// The top bit of each 16-bit half that is not finite: an exponent of ones carries into it.
+template <bool BF16> __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+  return ((w & kExp) + kOne) & 0x80008000u;
+}
+// The word without those halves.
+template <bool BF16> __device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  return w & ~((not_finite2<BF16>(w) >> 15) * 0xffffu);
+}
 // Two f32 values as two 16-bit words and what those leave out, as two more.
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (BF16) return pack_bf16x2(a, b);
