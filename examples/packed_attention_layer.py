@@ -124,10 +124,10 @@ def main():
           f"backward {timed(lambda: layer.backward(g, g, saved)):.0f} us")
 
     # a causal tower, token by token
-    tower, n = PackedAttentionLayer(1024, 16, causal=True), 32
+    tower, n = PackedAttentionLayer(768, 12, causal=True), 32
     for eight_bits in (False, True):
         cache = Cache(tower, n, 512)
-        tokens = [torch.randn(n, 1024, device="cuda").bfloat16() for _ in range(2)]
+        tokens = [torch.randn(n, 768, device="cuda").bfloat16() for _ in range(2)]
         us = timed(lambda: cache.token(tower, *tokens, eight_bits=eight_bits), 100)
         print(f"{n} sequences, one token each, {'8-bit' if eight_bits else 'bf16'} product: {us:.0f} us a step")
 
