@@ -506,7 +506,9 @@ VA_API int va_rotary_f32(const float *q, const float *k, float *q_out, float *k_
  * counts as at least 2^-100.
  * bwd: dh = r·(g − h·r²·mean(g·h)) + grad_h with g = dy·w (grad_h optional,
  * the gradient that reaches h along the residual), dw f32 [cols] = Σ dy·h·r,
- * summed in an order that depends on the sizes alone.  All rows contiguous. */
+ * summed in an order that depends on the sizes alone (rows 0: dw is set to zero
+ * and nothing is read).  All rows contiguous; outputs may lie exactly over x or
+ * residual (dh over dy, h or grad_h), but not shifted against them. */
 VA_API int va_rms_norm_fwd_bf16(const va_bf16 *x, const va_bf16 *residual, const void *w, int w_is_f32,
                                 va_bf16 *h, va_bf16 *y, long long rows, int cols, float eps, va_stream_t stream);
 VA_API int va_rms_norm_fwd_f16(const void *x, const void *residual, const void *w, int w_is_f32, void *h,
@@ -546,14 +548,19 @@ VA_API int va_rms_norm_bwd_f32(const float *dy, const float *h, const void *w, i
  * contiguous; lse f32 [num_heads, total_q] (natural log).
  * The sequences are given to va_packed_plan_build: cu_q and cu_k, int32
  * [num_seqs + 1] on the device, the rows where each sequence's queries and
- * keys begin (cu[0] = 0, cu[num_seqs] = total).  It fills the plan (256-byte
- * aligned, va_packed_plan_bytes) on the stream, without a copy to the host;
- * used_k (optional, int32 [num_seqs], not with `training`): how many of the
- * rows between cu_k[b] and cu_k[b + 1] hold keys, for a cache with room to grow.
- * later calls with the same sizes read it, layer after layer, and keep their
- * partial results in it: calls that share a plan must not overlap.
+ * keys begin (cu[0] = 0, cu[num_seqs] = total).  used_k (optional, int32
+ * [num_seqs], not with `training`): how many of the rows between cu_k[b] and
+ * cu_k[b + 1] hold keys, for a cache with room to grow.  The plan (256-byte
+ * aligned, va_packed_plan_bytes) is filled on the stream, without a copy to the
+ * host; later calls with the same sizes read it, layer after layer, and keep
+ * their partial results in it: calls that share a plan must not overlap.
  * va_packed_plan_status reads whether offsets were out of order or range (they
- * are clamped; synchronises). */
+ * are clamped; synchronises).  out may be q itself where that is contiguous, but
+ * must not lie over the inputs otherwise.  Totals up to 2^30; with `training`
+ * total_q · (num_heads/num_kv_heads) below 2^32 − 2^16.  Sums over more than 10^5
+ * keys of like weight lose accuracy (f32 sums of the tensor core: n equal weights
+ * and values of one sign come out low by about n · 2^-27.5; not for few queries,
+ * whose keys are split). */
 VA_API size_t va_packed_plan_bytes(int num_seqs, int total_q, int total_k, int num_heads, int num_kv_heads,
                                    int head_dim, int causal, int training);
 VA_API int va_packed_plan_build(const int32_t *cu_q, const int32_t *cu_k, const int32_t *used_k, int num_seqs,

@@ -13,8 +13,11 @@
 namespace va {
 
 constexpr int kPackBlock = 128;   // keys (and rows of a tile) a step
-// A tile is cut into parts of at least so many key blocks (forward) or query steps (dK/dV): smaller ones cost more to join
-// than they save (a forward block takes ~1 us, joining ~4 us).
+// The largest part of a tile is at least so many key blocks (forward) or query steps (dK/dV); a tile a little longer is cut
+// in two, so parts are at least half of that.  Measured (graph replays, plan built before): 4 single tokens, 32/8 heads of 128,
+// over 7, 8, 9 and 11 blocks 13.5, 14.1, 15.3 and 17.0 us, 15.3, 17.0, 18.4 and 21.9 with no part below the constant; 64
+// tokens, whose tiles fill the GPU uncut, over 8 and 11 blocks 64.9 and 82.0 us against 50.8 and 66.6.  Backward of 2
+// documents of 50 steps, 16 heads of 128: 361 against 378.
 constexpr int kMinKeyBlocks = 6, kMinQuerySteps = 32;
 constexpr int kMaxSeqs = 1 << 20;
 constexpr int kPlanSeqs = 2048;   // sequences whose tile counts fit the plan kernel's shared memory
@@ -84,7 +87,7 @@ inline PackedShape packed_shape(int num_seqs, int total_q, int total_k, int head
   s.max_tiles = (int)std::min<long long>((total_q + s.q_tile - 1) / s.q_tile + (long long)num_seqs, total_q);
   // Parts over the number of tiles: about two units for each place a CTA has on the GPU (forward), one an SM (dK/dV, whose
   // parts are larger to join: 507 us for a causal step of 10 k tokens against 516 with half as many more and 520 with
-  // twice), and no more than the longest possible tiles allow (none where no tile can pass the smallest part).
+  // twice, in short bursts; under sustained load the step takes 546), and no more than the longest possible tiles allow (none where no tile can pass the smallest part).
   auto budget = [](int most, long long tiles, long long longest, int smallest) {
     return longest <= smallest ? 0 : (int)std::min<long long>(most, (tiles * longest + smallest - 1) / smallest);
   };

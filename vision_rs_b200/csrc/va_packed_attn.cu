@@ -24,15 +24,22 @@
 // most 128 keys: with its remainder as a second operand); its rounding adds
 // about as much error as that of the output.  Sums, maxima and O stay f32.
 //
+// O is summed by the tensor core, which drops what lies about 2^-25 below the
+// running sum: with n equal weights and values of one sign an unsplit tile's
+// output is low by about n·2^-27.5 (measured: 0.06% at 2^17 keys, 0.6% at 2^20,
+// 2.4% at 2^22); values around zero and tiles in parts show nothing.
+//
 // Measured (sustained; B200): prompts of 2049 and 8191 tokens, 16/2 heads of
-// 128, causal, 300 µs = 0.97 PFLOP/s (254 µs before the power limit acts;
+// 128, causal, 296 µs = 0.99 PFLOP/s (254 µs before the power limit acts;
 // floor 177): bound by issuing the MMAs and by the shared-memory reads of the
-// N = 64 score MMAs.  16 images of 257–1601 tokens, 6 heads of 64, 65 µs (floor
+// N = 64 score MMAs.  16 images of 257–1601 tokens, 6 heads of 64, 64 µs (floor
 // 21, the exponentials): bound by the softmax's latencies between them.  64
-// single tokens over 17–8192 keys, 32/8 heads of 128, 210 µs = 5.1 TB/s (189
+// single tokens over 17–8192 keys, 32/8 heads of 128, 219 µs = 4.9 TB/s (189
 // before the power limit acts): HBM.
-// One 128-key buffer a tile instead of two of 64 keys: 339 against 264 µs for
-// the prompts; one issuing warp for both tiles: 410.
+// An earlier form took 339 µs for the prompts where this one took 264 (short
+// bursts): one 128-key score buffer a tile, one issuing warp for both tiles, an
+// election for each MMA, scalar f32 arithmetic.  What each of these costs by
+// itself was not measured.
 //
 // What a row does not see stays out of it, whatever it holds (another
 // sequence's rows in a box, unused rows of a cache, later keys): scores of such

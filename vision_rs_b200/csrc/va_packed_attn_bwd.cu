@@ -26,13 +26,13 @@
 // columns at 128 dims.
 //
 // Measured (B200): 4 documents of 1025–4095 tokens, 12/3 heads of 128, causal,
-// bf16: 537 µs for plan, forward and backward under sustained load (CUDA
-// events).  Shares from a profiler's launch list (single cold launches): row
-// sums 15 µs, dQ 169, dK/dV 245; their 3 and 4 products take 88 and 117 µs at
-// 1,647 TFLOP/s.  The tensor pipe is 45% busy in dQ and was 36% in dK/dV with
-// 549 blocks (402 now): a buffer's chain scores → P and dS → products is
-// covered only in part by the other buffer.  With one warp to issue both kinds
-// of products and dK/dV's tiles not yet split: dQ 220 µs, dK/dV 349.
+// bf16: 546 µs for plan, forward and backward under sustained load (CUDA
+// events).  Shares under a profiler (single cold launches): row sums 15 µs, dQ
+// 170, dK/dV 251; their 3 and 4 products take 88 and 117 µs at 1,647 TFLOP/s.
+// The tensor pipe is 45% busy in dQ and 39% in dK/dV (402 blocks): a buffer's
+// chain scores → P and dS → products is covered only in part by the other
+// buffer.  With one warp to issue both kinds of products and dK/dV's tiles not
+// yet split: dQ 220 µs, dK/dV 349.
 //
 // P and dS are 16-bit operands.  f16 has few exponents, so there P carries
 // 2^15 and dS a power of two chosen for its row (key or query) such that the

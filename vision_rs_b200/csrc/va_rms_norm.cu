@@ -18,7 +18,7 @@
 // partial row; a second kernel adds the partials in a fixed order, so the
 // result does not depend on scheduling (no atomics).
 //
-// Measured (B200): 16384 × 4096 bf16 to 8 bits 75 µs (0.95 of the copy
+// Measured (B200): 16384 × 4096 bf16 to 8 bits 75–78 µs (0.93–0.95 of the copy
 // rate; 128 × 4 or 512 × 1 threads and vectors a row instead of 256 × 2: 105,
 // 101 µs); 25616 × 384 f32 60 µs for the pair (launch list: 21, 26 and 5).
 #include <cuda_fp8.h>

@@ -17,7 +17,7 @@
 // and a thread keeps those of its chunk in registers over the heads that it
 // turns with 16-byte accesses, all q and k heads of a token in the same block.
 // One launch serves q and k.  Measured (B200): 16384 tokens, 32 + 8 heads of
-// 128, 64 rotated, f16, 63.5 µs = 0.81 of the copy rate (two heads in flight a
+// 128, 64 rotated, f16, 63–65 µs = 0.8 of the copy rate (two heads in flight a
 // thread instead of six: 85 µs; pairs read from shared memory for each head: 95).
 #include "va_common.cuh"
 

@@ -28,7 +28,10 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, stretch: float = 1.0
     was trained on.  Without ``trained_length`` every frequency is divided by
     it (positions interpolated).  With it, a pair that makes fewer than
     ``slow_turns`` turns over the trained length is divided, one with more
-    than ``fast_turns`` is kept, and those between are blended linearly."""
+    than ``fast_turns`` is kept, and those between are blended linearly in the
+    number of turns.  (A blend that is linear in the pair's index instead,
+    between the indices of the same two thresholds, gives the pairs between
+    other frequencies: a model trained with that needs its own ``inv_freq``.)"""
     if rot_dim <= 0 or rot_dim % 2:
         raise ValueError(f"rot_dim must be positive and even, got {rot_dim}")
     if not base > 0 or not stretch > 0:
