@@ -48,3 +48,12 @@ def test_loads_in_flight_are_waited_for(name, first):
     between = text[issue:drain]
     assert issue < drain and not re.search(r"if \(!?ok\)", between)
     assert re.search(r"mbar_try_wait\(&sm\.%s, 0\) && clock64\(\)" % first, text[drain:drain + 600])
+
+
+@pytest.mark.parametrize("name", ["va_packed_attn.cu", "va_packed_attn_bwd.cu"])
+def test_every_part_arrives(name):
+    """A part that gave up counts too: else the plan's counter is off by one and its next call joins the parts too early."""
+    text = _source(name)
+    arrive = text.index("sm.last = atomicAdd(cnt, 1)")
+    leave = text.rindex("return;", 0, arrive)
+    assert "if (it.slot < 0) return;" == text[text.rindex("if (", 0, leave):leave + len("return;")]

@@ -565,8 +565,9 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (warp == TILES * 4) tmem_dealloc(tmem, C::kTmemCols);
 
   if constexpr (TILES == 1) {
-    if (it.slot < 0 || sm.abort) return;
-    // ── the last of a tile's parts joins them: O = Σ w_k O_k, w_k = exp(lse_k − lse) ──
+    if (it.slot < 0) return;
+    // ── the last of a tile's parts joins them: O = Σ w_k O_k, w_k = exp(lse_k − lse).  A part whose wait gave up arrives too:
+    // this call's result is void (the status says so), the counter is whole for the next ──
     if (tid == 0) {
       __threadfence();
       int* cnt = reinterpret_cast<int*>(const_cast<uint8_t*>(a.plan) + ps.counters) + (long long)it.counter * ps.units + head;

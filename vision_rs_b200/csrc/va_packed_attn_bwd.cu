@@ -692,8 +692,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncthreads();
   if (warp == C::kWarps) tmem_dealloc(tmem, 512);
 
-  if (it.slot < 0 || sm.abort) return;
-  // ── the last of a tile's parts to arrive adds them in their order ──
+  if (it.slot < 0) return;
+  // ── the last of a tile's parts to arrive adds them in their order (one whose wait gave up arrives too: this call's result
+  // is void, the counter is whole for the next) ──
   if (tid == 0) {
     __threadfence();
     int* cnt = reinterpret_cast<int*>(a.plan + ps.dkv_counters) + (long long)it.counter * ps.kv_heads + kvh;
